@@ -8,6 +8,8 @@ without the library, so that it can create it.
 import importlib
 
 __all__ = ["neoGemmV1", "neogemm", "matmul", "matmul_fused", "linear", "matmul_host", "workspace_bytes",
+           "grouped_matmul", "grouped_matmul_dx", "grouped_matmul_dw", "MxFp4", "quantize_mxfp4",
+           "dequantize_mxfp4", "matmul_mxfp4", "grouped_matmul_mxfp4",
            "device_status", "clear_device_status", "last_config", "set_override", "set_tuning",
            "NeoGemmError"]
 

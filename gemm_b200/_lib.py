@@ -54,6 +54,23 @@ def _load() -> ctypes.CDLL:
     lib.neogemm_noalloc_clear_status.argtypes = []
     lib.neogemm_debug_wait_expiry_noalloc.restype = c_int
     lib.neogemm_debug_wait_expiry_noalloc.argtypes = [ctypes.c_uint]
+    lib.neogemm_grouped_nt.restype = c_int
+    lib.neogemm_grouped_nt.argtypes = ([c_void_p] * 4 + [c_int] + [c_int64] * 8 +
+                                       [c_int, c_void_p])
+    lib.neogemm_grouped_dx.restype = c_int
+    lib.neogemm_grouped_dx.argtypes = list(lib.neogemm_grouped_nt.argtypes)
+    lib.neogemm_grouped_dw.restype = c_int
+    lib.neogemm_grouped_dw.argtypes = [c_void_p] * 4 + [c_int] + [c_int64] * 6 + [c_void_p]
+    lib.neogemm_mxfp4_quantize.restype = c_int
+    lib.neogemm_mxfp4_quantize.argtypes = ([c_void_p, c_int, c_void_p, c_void_p] + [c_int64] * 5 +
+                                           [c_void_p])
+    lib.neogemm_mxfp4_dequantize.restype = c_int
+    lib.neogemm_mxfp4_dequantize.argtypes = [c_void_p] * 3 + [c_int64] * 3 + [c_void_p]
+    lib.neogemm_mxfp4_nt.restype = c_int
+    lib.neogemm_mxfp4_nt.argtypes = [c_void_p] * 5 + [c_int64] * 4 + [c_void_p]
+    lib.neogemm_grouped_mxfp4_nt.restype = c_int
+    lib.neogemm_grouped_mxfp4_nt.argtypes = ([c_void_p] * 6 + [c_int] + [c_int64] * 5 +
+                                             [c_int, c_void_p])
     lib.neogemm_workspace_bytes.restype = c_size_t
     lib.neogemm_workspace_bytes.argtypes = [c_int64, c_int64, c_int64, c_int]
     lib.neogemm_bf16_nt_host.restype = c_int

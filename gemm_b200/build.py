@@ -9,6 +9,7 @@ Everything is built in-tree so that the shared objects travel with the source di
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -18,6 +19,7 @@ PKG_DIR = Path(__file__).resolve().parent
 ROOT = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libneogemm.so"
+OBJ_DIR = ROOT / "build"
 ORACLE_DIR = ROOT / "oracle"
 ORACLE_LIB = ORACLE_DIR / "liboracle.so"
 
@@ -49,16 +51,44 @@ def library_sources():
 
 
 def build_library(force: bool = False, verbose: bool = False) -> Path:
-    """nvcc: csrc/*.cu -> gemm_b200/libneogemm.so for sm_100a."""
-    srcs = library_sources()
-    if not force and _newer(LIB_PATH, srcs):
+    """nvcc: csrc/*.cu -> gemm_b200/libneogemm.so for sm_100a, one object per source (in
+    ``build/``, compiled side by side; only what changed unless ``force``)."""
+    if not force and _newer(LIB_PATH, library_sources()):
         return LIB_PATH
-    cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-o", str(LIB_PATH)]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += [str(p) for p in sorted(CSRC.glob("*.cu"))]
-    subprocess.run(cmd, check=True, cwd=str(ROOT))
+    objects, running = [], []
+    shared = [p for p in library_sources() if p.suffix != ".cu"]
+    OBJ_DIR.mkdir(exist_ok=True)
+    for src in sorted(CSRC.glob("*.cu")):
+        obj = OBJ_DIR / (src.stem + ".o")
+        objects.append(str(obj))
+        # The GEMM kernels take minutes to compile and depend on few of the headers.
+        headers = [h for h in shared if _includes(src, h)]
+        if not force and _newer(obj, [src, *headers]):
+            continue
+        cmd = [_nvcc(), *NVCC_FLAGS, "-c", "-o", str(obj), str(src)]
+        if verbose:
+            cmd += ["-Xptxas", "-v"]
+        running.append((cmd, subprocess.Popen(cmd, cwd=str(ROOT))))
+    failed = [cmd for cmd, process in running if process.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", str(LIB_PATH), *objects], check=True,
+                   cwd=str(ROOT))
     return LIB_PATH
+
+
+def _includes(src: Path, header: Path, seen=None) -> bool:
+    """Whether ``src`` includes ``header``, directly or through another one."""
+    seen = set() if seen is None else seen
+    for name in re.findall(r'#include "([^"]+)"', src.read_text()):
+        path = (src.parent / name).resolve()
+        if path == header.resolve():
+            return True
+        if path not in seen and path.exists():
+            seen.add(path)
+            if _includes(path, header, seen):
+                return True
+    return False
 
 
 def build_oracle(force: bool = False) -> Path:

@@ -27,6 +27,7 @@
 // lets copies in flight land and frees tensor memory.  The kernel never traps or spins forever.
 #pragma once
 
+#include "device_errors.cuh"
 #include "ptx.cuh"
 
 namespace neogemm {
@@ -34,18 +35,6 @@ namespace neogemm {
 enum EpilogueMode : int {
   kEpiTmaStore = 0,  // row-major D, 16-byte-aligned pitch: staged through swizzled smem + TMA store
   kEpiDirect = 1,    // arbitrary (row, col) strides straight from registers, bounds-checked
-};
-
-// Device-side error codes written to the status word (first error wins).
-enum DeviceError : int {
-  kDevOk = 0,
-  kDevTimeoutProducer = 1,   // TMA warp gave up waiting for a free ring slot
-  kDevTimeoutMmaFull = 2,    // MMA warp gave up waiting for operand bytes
-  kDevTimeoutMmaTmem = 3,    // MMA warp gave up waiting for a drained accumulator
-  kDevTimeoutEpilogue = 4,   // epilogue gave up waiting for a finished accumulator
-  kDevTmemAddress = 5,       // tensor-memory allocation did not start at column 0 (pair mode)
-  kDevBounds = 6,            // an index left its buffer (access skipped); aux: 1 partials, 2 counters, 3 C
-  kDevTimeoutScheduler = 7,  // a role gave up waiting on the dynamic-claim queue
 };
 
 struct GemmParams {

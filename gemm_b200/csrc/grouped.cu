@@ -1,0 +1,376 @@
+// Host side of the grouped and MXFP4 products (contracts: include/neogemm.h; kernel:
+// grouped_sm100.cuh).
+#include "../../include/neogemm.h"
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "grouped_sm100.cuh"
+#include "host.cuh"
+
+namespace neogemm {
+namespace {
+
+constexpr int kMaxDevices = 64;
+constexpr int64_t kMaxExtent = 0x7fffffffll - 4096;   // room for tile coordinates past the end
+
+struct KernelEntry {
+  int op, cta_group, columns, stages;
+  const void* fn;
+  int smem_bytes, threads;
+};
+
+template <class Cfg>
+KernelEntry make_entry() {
+  return KernelEntry{Cfg::kOp, Cfg::kCtaGroup, Cfg::kCols, Cfg::kStages,
+                     reinterpret_cast<const void*>(&grouped_kernel<Cfg>), Cfg::kSmemBytes,
+                     Cfg::kThreads};
+}
+
+// [operation][0 narrow, 1 wide]
+const KernelEntry kKernels[4][2] = {
+    {make_entry<GroupedConfig<kGroupedNt, 1, 64, 8>>(), make_entry<GroupedConfig<kGroupedNt, 2, 256, 6>>()},
+    {make_entry<GroupedConfig<kGroupedDx, 1, 64, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 256, 6>>()},
+    {make_entry<GroupedConfig<kGroupedDw, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 256, 6>>()},
+    {make_entry<GroupedConfig<kMxNt, 1, 128, 5>>(), make_entry<GroupedConfig<kMxNt, 1, 128, 5>>()},
+};
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tensor map of `rank` dimensions, innermost first; strides (bytes) of dimensions 1 and up.
+int encode(const DeviceView& dev, CUtensorMap* map, CUtensorMapDataType type, int rank,
+           const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+           bool swizzle) {
+  const cuuint32_t ones[3] = {1, 1, 1};
+  cuuint64_t d[3], s[2];
+  cuuint32_t b[3];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i > 0) s[i - 1] = strides[i - 1];
+    if (i > 0 && (strides[i - 1] >= (1ull << 40) || strides[i - 1] % 16 != 0)) return NEOGEMM_ERR_UNSUPPORTED;
+  }
+  const CUresult r = dev.encode(
+      map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, b, ones,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NEOGEMM_OK : NEOGEMM_ERR_DESCRIPTOR;
+}
+
+int encode_matrix(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t inner,
+                  int64_t rows, int64_t pitch, uint32_t box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(pitch) * 2};
+  const uint32_t box[2] = {64, box_rows};
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, true);
+}
+
+int encode_stack(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t inner,
+                 int64_t rows, int64_t stack, int64_t pitch, int64_t stack_pitch, uint32_t box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(rows),
+                            static_cast<uint64_t>(stack)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(pitch) * 2,
+                               static_cast<uint64_t>(stack == 1 ? rows * pitch : stack_pitch) * 2};
+  const uint32_t box[3] = {64, box_rows, 1};
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, true);
+}
+
+int launch(const DeviceView& dev, const KernelEntry& k, int64_t tiles_at_most,
+           const CUtensorMap (&maps)[4], const GroupedParams& params, cudaStream_t stream) {
+  static std::mutex mu;
+  static bool attr_done[kMaxDevices][4][2] = {};
+  const int which = &k == &kKernels[k.op][1] ? 1 : 0;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    bool& done = attr_done[dev.index][k.op][which];
+    if (!done && cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      k.smem_bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return NEOGEMM_ERR_LAUNCH;
+    }
+    done = true;
+  }
+  const int64_t workers = std::max<int64_t>(
+      1, std::min<int64_t>(dev.sm_count / k.cta_group, tiles_at_most));
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(workers * k.cta_group), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(k.threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(k.smem_bytes);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int nattr = 0;
+  if (k.cta_group == 2) {
+    attr[nattr].id = cudaLaunchAttributeClusterDimension;
+    attr[nattr].val.clusterDim.x = 2;
+    attr[nattr].val.clusterDim.y = 1;
+    attr[nattr].val.clusterDim.z = 1;
+    ++nattr;
+  }
+  if (tuning_value(10) != 0) {
+    // The kernel's set-up overlaps the tail of the stream's previous kernel (see launcher.cu).
+    attr[nattr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[nattr].val.programmaticStreamSerializationAllowed = 1;
+    ++nattr;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = nattr;
+  void* args[5] = {const_cast<CUtensorMap*>(&maps[0]), const_cast<CUtensorMap*>(&maps[1]),
+                   const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]),
+                   const_cast<GroupedParams*>(&params)};
+  if (cudaLaunchKernelExC(&cfg, k.fn, args) != cudaSuccess) {
+    cudaGetLastError();
+    return NEOGEMM_ERR_LAUNCH;
+  }
+  record_config(k.cta_group, k.columns, k.stages, 1, static_cast<int>(cfg.gridDim.x), 0);
+  return NEOGEMM_OK;
+}
+
+// Checks that every entry point shares.
+int check_extents(const void* offsets, int64_t groups, int64_t T, int64_t N, int64_t K,
+                  int offsets_are_64) {
+  if (groups < 0 || T < 0 || N < 0 || K < 0) return NEOGEMM_ERR_BAD_ARG;
+  if (groups > kMaxGroups || T > kMaxExtent || N > kMaxExtent || K > kMaxExtent)
+    return NEOGEMM_ERR_UNSUPPORTED;
+  if (groups > 0 && offsets == nullptr) return NEOGEMM_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(offsets) & (offsets_are_64 ? 7 : 3)) != 0)
+    return NEOGEMM_ERR_UNSUPPORTED;
+  return NEOGEMM_OK;
+}
+
+int zero_rows(void* out, int64_t pitch, int64_t rows, int64_t width, cudaStream_t stream) {
+  DeviceView dev;
+  const int rc = acquire_device(&dev);
+  if (rc != NEOGEMM_OK) return rc;
+  if (cudaMemset2DAsync(out, static_cast<size_t>(pitch) * 2, 0, static_cast<size_t>(width) * 2,
+                        static_cast<size_t>(rows), stream) != cudaSuccess) {
+    cudaGetLastError();
+    return NEOGEMM_ERR_CUDA;
+  }
+  return NEOGEMM_OK;
+}
+
+// Average rows per group from which the wide tiles (a CTA pair, 256 x 256) are taken.
+constexpr int64_t kWideRows = 96;
+
+bool take_wide(int64_t average_rows) {
+  const int forced = tuning_value(13);
+  return forced >= 0 ? forced != 0 : average_rows >= kWideRows;
+}
+
+// Y or dX: rows of the batch in, rows out.
+int grouped_rows(int op, const void* R, const void* W, void* out, const void* offsets,
+                 int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K, int64_t ldr,
+                 int64_t ldw, int64_t stack_w, int64_t ldo, int zero_rest, cudaStream_t stream) {
+  int rc = check_extents(offsets, groups, T, N, K, offsets_are_64);
+  if (rc != NEOGEMM_OK) return rc;
+  const int64_t depth = op == kGroupedDx ? N : K;    // contraction
+  const int64_t lanes = op == kGroupedDx ? K : N;    // width of the result
+  if (T == 0 || lanes == 0) return NEOGEMM_OK;
+  if (out == nullptr || ldo < lanes) return NEOGEMM_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(out) & 1) != 0) return NEOGEMM_ERR_UNSUPPORTED;
+  if (groups == 0) return zero_rest ? zero_rows(out, ldo, T, lanes, stream) : NEOGEMM_OK;
+  if (depth > 0) {
+    if (R == nullptr || W == nullptr || ldr < depth || ldw < K) return NEOGEMM_ERR_BAD_ARG;
+    if (groups > 1 && stack_w < 0) return NEOGEMM_ERR_BAD_ARG;
+    if (ldr % 8 != 0 || ldw % 8 != 0 || (groups > 1 && stack_w % 8 != 0) || !aligned16(R) ||
+        !aligned16(W))
+      return NEOGEMM_ERR_UNSUPPORTED;
+  }
+  DeviceView dev;
+  rc = acquire_device(&dev);
+  if (rc != NEOGEMM_OK) return rc;
+
+  const KernelEntry& k = kKernels[op][take_wide(T / groups) ? 1 : 0];
+  CUtensorMap maps[4];
+  std::memset(maps, 0, sizeof(maps));
+  if (depth > 0) {
+    rc = encode_stack(dev, &maps[0], W, K, N, groups, ldw, stack_w, op == kGroupedDx ? 64 : 128);
+    if (rc == NEOGEMM_OK) rc = encode_matrix(dev, &maps[1], R, depth, T, ldr, 32);
+    if (rc != NEOGEMM_OK) return rc;
+  }
+  GroupedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.offsets = offsets;
+  p.offsets_are_64 = offsets_are_64;
+  p.groups = static_cast<int>(groups);
+  p.rows = static_cast<int>(T);
+  p.lanes = static_cast<int>(lanes);
+  p.depth = static_cast<int>(depth);
+  const int64_t lane_tiles = ceil_div(lanes, 128 * k.cta_group);
+  const int64_t tiles = lane_tiles * (std::min(groups, T) + T / k.columns);
+  if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
+  p.lane_tiles = static_cast<int>(lane_tiles);
+  p.zero_rest = zero_rest;
+  p.vector_out = ldo % 8 == 0 && aligned16(out);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_pitch = ldo;
+  p.status = dev.status;
+  return launch(dev, k, tiles, maps, p, stream);
+}
+
+// Scale tiles as a matrix of 512-byte rows, read two at a time.
+int encode_scales(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t tiles) {
+  const uint64_t dims[2] = {128, static_cast<uint64_t>(tiles)};
+  const uint64_t strides[1] = {512};
+  const uint32_t box[2] = {128, 2};
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, base, dims, strides, box, false);
+}
+
+int encode_codes(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t K, int64_t rows,
+                 int64_t stack, uint32_t box_rows) {
+  const uint64_t bytes = static_cast<uint64_t>(K) / 2;
+  const uint64_t dims[3] = {bytes, static_cast<uint64_t>(rows), static_cast<uint64_t>(stack)};
+  const uint64_t strides[2] = {bytes, bytes * static_cast<uint64_t>(rows)};
+  const uint32_t box[3] = {128, box_rows, 1};
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, stack > 0 ? 3 : 2, base, dims, strides, box,
+                true);
+}
+
+int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void* Y,
+            const void* offsets, int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+            int64_t ldy, int zero_rest, cudaStream_t stream) {
+  if (T == 0 || N == 0) return NEOGEMM_OK;
+  if (Y == nullptr || ldy < N) return NEOGEMM_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(Y) & 1) != 0 || K % 64 != 0) return NEOGEMM_ERR_UNSUPPORTED;
+  if (groups == 0) return zero_rest ? zero_rows(Y, ldy, T, N, stream) : NEOGEMM_OK;
+  if (K > 0) {
+    if (Xc == nullptr || Xs == nullptr || Wc == nullptr || Ws == nullptr) return NEOGEMM_ERR_BAD_ARG;
+    if (!aligned16(Xc) || !aligned16(Xs) || !aligned16(Wc) || !aligned16(Ws))
+      return NEOGEMM_ERR_UNSUPPORTED;
+  }
+  DeviceView dev;
+  int rc = acquire_device(&dev);
+  if (rc != NEOGEMM_OK) return rc;
+
+  const KernelEntry& k = kKernels[kMxNt][take_wide(T / groups) ? 1 : 0];
+  const int64_t k_tiles = ceil_div(K, 128), w_tiles = ceil_div(N, 128), x_tiles = ceil_div(T, 128);
+  if (groups * w_tiles * k_tiles > kMaxExtent || x_tiles * k_tiles > kMaxExtent)
+    return NEOGEMM_ERR_UNSUPPORTED;
+  CUtensorMap maps[4];
+  std::memset(maps, 0, sizeof(maps));
+  if (K > 0) {
+    rc = encode_codes(dev, &maps[0], Wc, K, N, groups, 128);
+    if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps[1], Xc, K, T, 0, 32);
+    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[2], Ws, groups * w_tiles * k_tiles);
+    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[3], Xs, x_tiles * k_tiles);
+    if (rc != NEOGEMM_OK) return rc;
+  }
+  GroupedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.offsets = offsets;
+  p.offsets_are_64 = offsets_are_64;
+  p.groups = static_cast<int>(groups);
+  p.rows = static_cast<int>(T);
+  p.lanes = static_cast<int>(N);
+  p.depth = static_cast<int>(K);
+  const int64_t lane_tiles = ceil_div(N, 128 * k.cta_group);
+  // Tiles keep to the grid of the columns, so a group may touch one more than its length says.
+  const int64_t tiles = lane_tiles * (std::min(groups, T) + T / k.columns + 1);
+  if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
+  p.lane_tiles = static_cast<int>(lane_tiles);
+  p.zero_rest = zero_rest;
+  p.vector_out = ldy % 8 == 0 && aligned16(Y);
+  p.out = static_cast<__nv_bfloat16*>(Y);
+  p.out_pitch = ldy;
+  p.sf_row_blocks = static_cast<int>(w_tiles);
+  p.sf_k_blocks = static_cast<int>(k_tiles);
+  p.status = dev.status;
+  return launch(dev, k, tiles, maps, p, stream);
+}
+
+}  // namespace
+}  // namespace neogemm
+
+using namespace neogemm;
+
+extern "C" {
+
+int neogemm_grouped_nt(const void* X, const void* W, void* Y, const void* offsets,
+                       int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                       int64_t ldx, int64_t ldw, int64_t stack_w, int64_t ldy, int zero_rest,
+                       void* stream) {
+  return grouped_rows(kGroupedNt, X, W, Y, offsets, offsets_are_64, groups, T, N, K, ldx, ldw,
+                      stack_w, ldy, zero_rest, static_cast<cudaStream_t>(stream));
+}
+
+int neogemm_grouped_dx(const void* dY, const void* W, void* dX, const void* offsets,
+                       int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                       int64_t lddy, int64_t ldw, int64_t stack_w, int64_t lddx, int zero_rest,
+                       void* stream) {
+  return grouped_rows(kGroupedDx, dY, W, dX, offsets, offsets_are_64, groups, T, N, K, lddy, ldw,
+                      stack_w, lddx, zero_rest, static_cast<cudaStream_t>(stream));
+}
+
+int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offsets,
+                       int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                       int64_t lddy, int64_t ldx, void* stream) {
+  int rc = check_extents(offsets, groups, T, N, K, offsets_are_64);
+  if (rc != NEOGEMM_OK) return rc;
+  if (groups == 0 || N == 0 || K == 0) return NEOGEMM_OK;
+  if (dW == nullptr) return NEOGEMM_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(dW) & 1) != 0) return NEOGEMM_ERR_UNSUPPORTED;
+  if (T > 0) {
+    if (dY == nullptr || X == nullptr || lddy < N || ldx < K) return NEOGEMM_ERR_BAD_ARG;
+    if (lddy % 8 != 0 || ldx % 8 != 0 || !aligned16(dY) || !aligned16(X))
+      return NEOGEMM_ERR_UNSUPPORTED;
+  }
+  DeviceView dev;
+  rc = acquire_device(&dev);
+  if (rc != NEOGEMM_OK) return rc;
+
+  // The pair's tiles are 256 x 256 of a group's matrix whatever its rows.
+  const int forced = tuning_value(13);
+  const bool wide = forced >= 0 ? forced != 0 : N >= 256 && K >= 256;
+  const KernelEntry& k = kKernels[kGroupedDw][wide ? 1 : 0];
+  CUtensorMap maps[4];
+  std::memset(maps, 0, sizeof(maps));
+  if (T > 0) {
+    rc = encode_matrix(dev, &maps[0], dY, N, T, lddy, 64);
+    if (rc == NEOGEMM_OK) rc = encode_matrix(dev, &maps[1], X, K, T, ldx, 64);
+    if (rc != NEOGEMM_OK) return rc;
+  }
+  GroupedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.offsets = offsets;
+  p.offsets_are_64 = offsets_are_64;
+  p.groups = static_cast<int>(groups);
+  p.rows = static_cast<int>(T);
+  p.lanes = static_cast<int>(N);
+  p.cols = static_cast<int>(K);
+  p.depth = static_cast<int>(T);
+  const int64_t lane_tiles = ceil_div(N, 128 * k.cta_group), col_tiles = ceil_div(K, k.columns);
+  const int64_t tiles = groups * lane_tiles * col_tiles;
+  if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
+  p.lane_tiles = static_cast<int>(lane_tiles);
+  p.col_tiles = static_cast<int>(col_tiles);
+  p.vector_out = K % 8 == 0 && aligned16(dW);
+  p.out = static_cast<__nv_bfloat16*>(dW);
+  p.out_pitch = K;
+  p.out_stack = N * K;
+  p.status = dev.status;
+  return launch(dev, k, tiles, maps, p, static_cast<cudaStream_t>(stream));
+}
+
+int neogemm_mxfp4_nt(const void* A_codes, const void* A_scales, const void* B_codes,
+                     const void* B_scales, void* C, int64_t M, int64_t N, int64_t K, int64_t ldc,
+                     void* stream) {
+  if (M < 0 || N < 0 || K < 0) return NEOGEMM_ERR_BAD_ARG;
+  if (M > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
+  return mx_rows(A_codes, A_scales, B_codes, B_scales, C, nullptr, 0, 1, M, N, K, ldc, 0,
+                 static_cast<cudaStream_t>(stream));
+}
+
+int neogemm_grouped_mxfp4_nt(const void* X_codes, const void* X_scales, const void* W_codes,
+                             const void* W_scales, void* Y, const void* offsets,
+                             int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                             int64_t ldy, int zero_rest, void* stream) {
+  const int rc = check_extents(offsets, groups, T, N, K, offsets_are_64);
+  if (rc != NEOGEMM_OK) return rc;
+  return mx_rows(X_codes, X_scales, W_codes, W_scales, Y, offsets, offsets_are_64, groups, T, N, K,
+                 ldy, zero_rest, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,665 @@
+// Products of a ragged batch with one matrix per group, for sm_100a.  The rows of the batch are
+// sorted by group; group e owns rows [offsets[e], offsets[e+1]), read from device memory, so a
+// router's result never has to visit the host.  One kernel template serves
+//
+//   kGroupedNt   y[t,n]    = sum_k x[t,k] W[e][n,k]                 (bf16)
+//   kGroupedDx   dx[t,k]   = sum_n dy[t,n] W[e][n,k]                (bf16, gradient of the rows)
+//   kGroupedDw   dW[e][n,k] = sum_{t in e} dy[t,n] x[t,k]           (bf16, gradient of the matrices)
+//   kMxNt        y[t,n]    = sum_k x[t,k] W[e][n,k]                 (both in MXFP4: E2M1 codes, one
+//                                                                   E8M0 scale per 32 values of K)
+//
+// all with fp32 accumulation in tensor memory and one rounding to bf16.  The dense MXFP4 product is
+// the last one with a single group.
+//
+// Roles of a tile.  The matrix operand always takes the 128 tensor-memory lanes of a CTA (256 of a
+// pair) and the rows of the batch take the accumulator's COLUMNS.  Lanes come in steps of 128, but
+// the column count N of an MMA is a run-time value in steps of 16 (32 for a pair): a group of 40
+// rows costs an N = 48 product instead of a 128-row tile, which is what makes ragged groups and
+// single tokens cheap, and a group's rows are cut into equal tiles rather than full ones and a
+// remnant.  dW has no ragged output; there the group's rows are the contraction.
+//
+//   warp 0      TMA producer      warp 1      UMMA issuer (leader CTA of a pair)
+//   warps 2-5   epilogue: tcgen05.ld -> bf16 -> shared-memory transpose -> 16-byte row stores,
+//               overlapped with the next tile through a second accumulator
+//   warp 6      kGroupedDw only: clears the rows of a tile's last k-block that belong to the next
+//               group (both operands: a zero times a neighbour's Inf would still be NaN)
+//
+// Every CTA (pair) walks tiles worker, worker + workers, ... of the list
+// (group, lane tile, column tile); the list's prefix sums are built in shared memory at the start.
+// Every wait is bounded; on expiry the role records a code, raises the CTA's abort flag and falls
+// through to the tear-down.
+#pragma once
+
+#include "device_errors.cuh"
+#include "ptx.cuh"
+
+namespace neogemm {
+
+enum GroupedOp : int { kGroupedNt = 0, kGroupedDx = 1, kGroupedDw = 2, kMxNt = 3 };
+
+constexpr int kMaxGroups = 1024;
+
+struct GroupedParams {
+  const void* offsets;      // groups + 1 ascending row indices, or null: one group of all rows
+  int offsets_are_64;
+  int groups;
+  int rows;                 // rows of the batch
+  int lanes;                // extent of the axis on the tensor-memory lanes (N; K for dx)
+  int cols;                 // kGroupedDw: extent of the column axis (K)
+  int depth;                // contraction length (K; N for dx; for dW the rows of the batch)
+  int lane_tiles;           // tiles along `lanes`
+  int col_tiles;            // kGroupedDw: tiles along `cols`
+  int zero_rest;            // write zeros to the rows of no group (0: leave them)
+  int vector_out;           // 16-byte stores are possible (alignment of base and pitches)
+  __nv_bfloat16* out;
+  long long out_pitch;      // elements between rows of the result
+  long long out_stack;      // kGroupedDw: elements between the groups' matrices
+  int sf_row_blocks;        // kMxNt: 128-row blocks of scales per matrix of the stack
+  int sf_k_blocks;          // kMxNt: 128-value blocks of scales along K
+  int* status;
+};
+
+template <int kOp_, int kCtaGroup_, int kCols_, int kStages_>
+struct GroupedConfig {
+  static constexpr int kOp = kOp_;
+  static constexpr int kCtaGroup = kCtaGroup_;
+  static constexpr int kCols = kCols_;              // widest accumulator (UMMA N) of a tile
+  static constexpr int kStages = kStages_;
+  static constexpr int kLaneRows = 128;             // lanes per CTA
+  static constexpr int kLaneTile = kLaneRows * kCtaGroup;
+  static constexpr int kHalfCols = kCols / kCtaGroup;   // column rows a CTA fetches at most
+  static constexpr int kBlockK = (kOp == kMxNt) ? 256 : 64;   // values of K per 128-byte row
+  static constexpr int kStepK = (kOp == kMxNt) ? 64 : 16;     // values of K per MMA
+  static constexpr int kColStep = 16 * kCtaGroup;   // granularity of a tile's N
+  static constexpr int kBoxRows = 32;               // rows of a box of the ragged operand
+  // Shared memory of one ring slot.
+  static constexpr int kLaneBytes = kLaneRows * 128;
+  static constexpr int kColBytes = kHalfCols * 128;
+  static constexpr int kScaleCols = (kCols + 127) / 128;      // 128-row scale blocks of the columns
+  static constexpr int kScaleBytes = (kOp == kMxNt) ? 1024 * (1 + kScaleCols) : 0;
+  static constexpr int kStageBytes = kLaneBytes + kColBytes + kScaleBytes;
+  static constexpr int kEpiBytes = 4 * 2 * 2048;    // per epilogue warp two buffers of 32 x 32 bf16
+  static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
+  static constexpr int kBarrierBytes = (3 * kStages + 4) * 8 + 16;
+  static constexpr int kSmemBytes =
+      kStages * kStageBytes + kEpiBytes + kTableBytes + 12 + kBarrierBytes + 1024;
+  // Two accumulators, and behind them (MXFP4) the scales of every ring slot: per 128 values of K
+  // four columns per 128 rows.
+  static constexpr int kScaleTmemCols = (kOp == kMxNt) ? 8 * (1 + kScaleCols) : 0;
+  static constexpr int kTmemNeeded = 2 * kCols + kStages * kScaleTmemCols;
+  static constexpr int kTmemCols = (kCtaGroup == 2) ? 512 : kTmemNeeded <= 128 ? 128
+                                 : kTmemNeeded <= 256 ? 256 : 512;
+  static constexpr int kThreads = (kOp == kGroupedDw) ? 224 : 192;
+  // Arrivals that complete a ring slot's phase besides its bytes: the slot's producer, and for
+  // dW one per CTA (the last block of a tile is handed over by the warps that cleared its rows).
+  static constexpr int kFullArrivals = (kOp == kGroupedDw) ? kCtaGroup : 1;
+  static_assert(kStageBytes % 1024 == 0, "every slot must keep the swizzle's alignment");
+  static_assert(kSmemBytes <= 232448, "exceeds 227 KB of shared memory per CTA");
+  static_assert(kSmemBytes > 116224, "one CTA per SM: tensor memory is not shared");
+  static_assert(kTmemNeeded <= 512, "tensor memory");
+  static_assert(kCols % 32 == 0 && kCols <= 256 && kHalfCols % kBoxRows == 0, "columns");
+};
+
+// What a tile computes.  Every role derives it from the tile's number.
+struct GroupedTile {
+  int group;
+  int lane0;      // first index on the lanes
+  int col_row;    // row of the ragged operand (index of the column axis for dW) in column 0
+  int lo, hi;     // columns that are this tile's to store
+  int mma_n;      // columns computed: hi rounded up
+  int k_row;      // kGroupedDw: first row of the contraction
+  int k_len;      // contraction length
+  int blocks;     // k-blocks (0: the result is zero)
+};
+
+__device__ __forceinline__ void report_error(int* status, volatile int* abort_flag, int code,
+                                             int tile, int aux) {
+  *abort_flag = 1;
+  if (status != nullptr && atomicCAS(status, 0, code) == 0) {
+    status[1] = static_cast<int>(blockIdx.x);
+    status[2] = tile;
+    status[3] = aux;
+    __threadfence_system();
+  }
+}
+
+template <class Cfg>
+__device__ __forceinline__ int column_tiles(int begin, int end) {
+  if (Cfg::kOp == kMxNt)   // scale blocks are 128 rows: tiles keep to their grid
+    return end > begin ? (end - 1) / Cfg::kCols - begin / Cfg::kCols + 1 : 0;
+  return (end - begin + Cfg::kCols - 1) / Cfg::kCols;
+}
+
+template <class Cfg>
+__device__ __forceinline__ GroupedTile find_tile(const GroupedParams& p, int tile, const int* begin,
+                                                 const int* end, const int* first_tile) {
+  GroupedTile t;
+  if (Cfg::kOp == kGroupedDw) {
+    const int per_group = p.lane_tiles * p.col_tiles;
+    t.group = tile / per_group;
+    const int local = tile - t.group * per_group;
+    const int lane_tile = local / p.col_tiles;
+    t.lane0 = lane_tile * Cfg::kLaneTile;
+    t.col_row = (local - lane_tile * p.col_tiles) * Cfg::kCols;
+    t.lo = 0;
+    t.hi = min(Cfg::kCols, p.cols - t.col_row);
+    t.k_row = begin[t.group];
+    t.k_len = end[t.group] - t.k_row;
+  } else {
+    // Last group whose first tile is not behind this one: groups without tiles share their
+    // first tile with the next group and lose the comparison.
+    int a = 0, b = p.groups - 1;
+    while (a < b) {
+      const int m = (a + b + 1) >> 1;
+      if (first_tile[m] <= tile) a = m; else b = m - 1;
+    }
+    t.group = a;
+    const int g0 = begin[a], g1 = end[a];
+    const int tiles = column_tiles<Cfg>(g0, g1);
+    const int local = tile - first_tile[a];
+    const int lane_tile = local / tiles;
+    const int c = local - lane_tile * tiles;
+    t.lane0 = lane_tile * Cfg::kLaneTile;
+    if (Cfg::kOp == kMxNt) {
+      t.col_row = (g0 / Cfg::kCols + c) * Cfg::kCols;
+      t.lo = max(g0 - t.col_row, 0);
+      t.hi = min(g1 - t.col_row, Cfg::kCols);
+    } else {
+      // Equal shares, in steps of the MMA's column granularity.
+      const int share = ((g1 - g0 + tiles - 1) / tiles + Cfg::kColStep - 1) / Cfg::kColStep *
+                        Cfg::kColStep;
+      t.col_row = g0 + c * share;
+      t.lo = 0;
+      t.hi = max(min(share, g1 - t.col_row), 0);
+    }
+    t.k_row = 0;
+    t.k_len = p.depth;
+  }
+  t.mma_n = max((t.hi + Cfg::kColStep - 1) / Cfg::kColStep, 1) * Cfg::kColStep;
+  t.blocks = (t.k_len + Cfg::kBlockK - 1) / Cfg::kBlockK;
+  return t;
+}
+
+// Boxes of the column operand that CTA `rank` fetches: rows [first, first + count) of boxes, in
+// units of kBoxRows rows from the start of its half.  Rows nobody stores are not fetched.
+template <class Cfg>
+__device__ __forceinline__ void column_boxes(const GroupedTile& t, int rank, int* first, int* count) {
+  const int half = t.mma_n / Cfg::kCtaGroup;
+  const int lo = max(t.lo - rank * half, 0), hi = min(t.hi - rank * half, half);
+  *first = lo / Cfg::kBoxRows;
+  *count = hi > lo ? (hi - 1) / Cfg::kBoxRows - *first + 1 : 0;
+}
+
+// Bytes CTA `rank` fetches per k-block.
+template <class Cfg>
+__device__ __forceinline__ uint32_t block_bytes(const GroupedTile& t, int rank) {
+  uint32_t bytes = Cfg::kLaneBytes + Cfg::kScaleBytes;
+  if (Cfg::kOp == kGroupedDw) {
+    bytes += (t.mma_n / Cfg::kCtaGroup + 63) / 64 * 8192;
+  } else {
+    int first, count;
+    column_boxes<Cfg>(t, rank, &first, &count);
+    bytes += static_cast<uint32_t>(count) * (Cfg::kBoxRows * 128);
+  }
+  return bytes;
+}
+
+// tmap_l: the operand on the lanes; tmap_c: the one on the columns; tmap_sl, tmap_sc: their scales
+// (kMxNt).
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, 1)
+grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant__ CUtensorMap tmap_c,
+               const __grid_constant__ CUtensorMap tmap_sl,
+               const __grid_constant__ CUtensorMap tmap_sc, const GroupedParams p) {
+  using namespace ptx;
+  constexpr int kCtaGroup = Cfg::kCtaGroup;
+  constexpr int kStages = Cfg::kStages;
+  constexpr bool kDw = Cfg::kOp == kGroupedDw;
+  constexpr bool kMx = Cfg::kOp == kMxNt;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t ring = smem_base;
+  const uint32_t epi_base = ring + kStages * Cfg::kStageBytes;
+  const uint32_t bar_base = epi_base + Cfg::kEpiBytes;
+  const uint32_t full_bar = bar_base;                        // [kStages]
+  const uint32_t empty_bar = full_bar + 8 * kStages;         // [kStages]
+  const uint32_t clear_bar = empty_bar + 8 * kStages;        // [kStages] dW: last block has landed
+  const uint32_t tmem_full_bar = clear_bar + 8 * kStages;    // [2]
+  const uint32_t tmem_empty_bar = tmem_full_bar + 16;        // [2]
+  uint8_t* tail_gen = smem_gen + (tmem_empty_bar + 16 - smem_base);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail_gen);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_gen + 4);
+  int* begin = reinterpret_cast<int*>(tail_gen + 16);        // [kMaxGroups]
+  int* end = begin + kMaxGroups;                             // [kMaxGroups]
+  int* first_tile = end + kMaxGroups;                        // [kMaxGroups + 1]
+
+  const int warp = threadIdx.x >> 5;
+  const uint32_t lane = lane_id();
+  const int rank = (kCtaGroup == 2) ? static_cast<int>(cluster_ctarank()) : 0;
+  const bool is_leader = rank == 0;
+  const int worker = static_cast<int>(blockIdx.x) / kCtaGroup;
+  const int num_workers = static_cast<int>(gridDim.x) / kCtaGroup;
+
+  // ---------------------------------------------------------------- set-up
+  if (threadIdx.x == 0) {
+    griddep_launch_dependents();
+    *abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar + 8 * s, Cfg::kFullArrivals);
+      mbar_init(empty_bar + 8 * s, 1);
+      mbar_init(clear_bar + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tmem_full_bar + 8 * a, 1);
+      mbar_init(tmem_empty_bar + 8 * a, 4 * kCtaGroup);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0 && p.depth > 0) {   // without a contraction there are no maps
+    prefetch_tensormap(&tmap_l);
+    prefetch_tensormap(&tmap_c);
+    if (kMx) {
+      prefetch_tensormap(&tmap_sl);
+      prefetch_tensormap(&tmap_sc);
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
+    tmem_relinquish<1>();
+  }
+  // Global memory from here on: wait for the previous kernel of the stream.
+  griddep_wait();
+  // Row ranges of the groups, clamped to the batch: indices that are out of order or out of range
+  // cost the result, never an access.
+  for (int e = threadIdx.x; e < p.groups; e += Cfg::kThreads) {
+    long long b = 0, f = p.rows;
+    if (p.offsets != nullptr) {
+      if (p.offsets_are_64) {
+        b = static_cast<const long long*>(p.offsets)[e];
+        f = static_cast<const long long*>(p.offsets)[e + 1];
+      } else {
+        b = static_cast<const int*>(p.offsets)[e];
+        f = static_cast<const int*>(p.offsets)[e + 1];
+      }
+    }
+    if (b < 0 || f < b || f > p.rows) {
+      if (blockIdx.x == 0 && p.status != nullptr && atomicCAS(p.status, 0, kDevBounds) == 0) {
+        p.status[1] = 0;
+        p.status[2] = e;
+        p.status[3] = 4;
+        __threadfence_system();
+      }
+      b = b < 0 ? 0 : b > p.rows ? p.rows : b;
+      f = f < b ? b : f > p.rows ? p.rows : f;
+    }
+    begin[e] = static_cast<int>(b);
+    end[e] = static_cast<int>(f);
+  }
+  tcgen05_fence_before();
+  if (kCtaGroup == 2) cluster_sync_all(); else __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  if (kCtaGroup == 2 && tmem_base != 0 && threadIdx.x == 0)
+    report_error(p.status, abort_flag, kDevTmemAddress, 0, static_cast<int>(tmem_base));
+  if (!kDw && warp == 0) {
+    int sum = 0;
+    for (int base = 0; base < p.groups; base += 32) {
+      const int e = base + static_cast<int>(lane);
+      const int mine = e < p.groups ? column_tiles<Cfg>(begin[e], end[e]) * p.lane_tiles : 0;
+      int scan = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int other = __shfl_up_sync(0xffffffffu, scan, d);
+        if (static_cast<int>(lane) >= d) scan += other;
+      }
+      if (e < p.groups) first_tile[e] = sum + scan - mine;
+      sum += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (lane == 0) first_tile[p.groups] = sum;
+  }
+  __syncthreads();
+  const int num_tiles = kDw ? p.groups * p.lane_tiles * p.col_tiles : first_tile[p.groups];
+
+  // ---------------------------------------------------------------- roles
+  if (*abort_flag != 0) {
+    // The tensor-memory address check failed: nothing is issued.
+  } else if (warp == 0) {
+    // ======================= TMA producer =======================
+    uint32_t stage = 0, phase = 0;
+    const uint32_t leader_full = (kCtaGroup == 2) ? mapa_u32(full_bar, 0) : full_bar;
+    bool ok = true;
+    for (int tile = worker; ok && tile < num_tiles; tile += num_workers) {
+      const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
+      const uint32_t mine = block_bytes<Cfg>(t, rank);
+      const uint32_t both = mine + (kCtaGroup == 2 ? block_bytes<Cfg>(t, 1 - rank) : 0u);
+      int first_box = 0, boxes = 0;
+      if (!kDw) column_boxes<Cfg>(t, rank, &first_box, &boxes);
+      const int half = t.mma_n / kCtaGroup;
+      const int lane_row = t.lane0 + rank * Cfg::kLaneRows;
+      for (int kb = 0; kb < t.blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, abort_flag))) {
+          if (lane == 0)
+            report_error(p.status, abort_flag, kDevTimeoutProducer, tile, static_cast<int>(stage));
+          ok = false;
+          break;
+        }
+        const uint32_t sl = ring + stage * Cfg::kStageBytes;
+        const uint32_t sc = sl + Cfg::kLaneBytes;
+        if (elect_one()) {
+          const int k0 = kb * 64;   // first element of the block (byte pairs for MXFP4: 128 bytes)
+          const uint32_t bar = leader_full + 8 * stage;
+          if constexpr (kDw) {
+            // Both operands run along the rows of the batch.
+            const bool clear = t.k_len - k0 < 64;
+            const uint32_t own = clear ? clear_bar + 8 * stage : full_bar + 8 * stage;
+            if (clear) {
+              mbar_arrive_expect_tx(own, mine);
+            } else if (is_leader) {
+              mbar_arrive_expect_tx(own, both);
+              if (kCtaGroup == 2) mbar_arrive(own);
+            }
+            const int row = t.k_row + k0;
+            const int col = t.col_row + rank * half;
+            const int col_boxes = (half + 63) / 64;
+            auto load = [&](uint32_t dst, const CUtensorMap* map, int c0) {
+              if (kCtaGroup == 1 || clear) tma_load_2d(dst, map, own, c0, row);
+              else tma_load_2d_pair(dst, map, bar, c0, row);
+            };
+            load(sl, &tmap_l, lane_row);
+            load(sl + 8192, &tmap_l, lane_row + 64);
+            for (int b = 0; b < col_boxes; ++b) load(sc + b * 8192, &tmap_c, col + b * 64);
+          } else {
+            if (kCtaGroup == 1) mbar_arrive_expect_tx(bar, mine);
+            else if (is_leader) mbar_arrive_expect_tx(full_bar + 8 * stage, both);
+            auto load2 = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1) {
+              if (kCtaGroup == 1) tma_load_2d(dst, map, bar, c0, c1);
+              else tma_load_2d_pair(dst, map, bar, c0, c1);
+            };
+            auto load3 = [&](uint32_t dst, int c0, int c1) {
+              if (kCtaGroup == 1) tma_load_3d(dst, &tmap_l, bar, c0, c1, t.group);
+              else tma_load_3d_pair(dst, &tmap_l, bar, c0, c1, t.group);
+            };
+            if constexpr (Cfg::kOp == kGroupedDx) {
+              load3(sl, lane_row, k0);
+              load3(sl + 8192, lane_row + 64, k0);
+            } else {
+              load3(sl, kMx ? kb * 128 : k0, lane_row);
+            }
+            const int row = t.col_row + rank * half;
+            for (int b = first_box; b < first_box + boxes; ++b)
+              load2(sc + b * (Cfg::kBoxRows * 128), &tmap_c, kMx ? kb * 128 : k0,
+                    row + b * Cfg::kBoxRows);
+            if constexpr (kMx) {
+              // Two consecutive 512-byte tiles of scales (128 rows x 128 values of K each); the
+              // second one of a short last block is some other tile or zero fill and not used.
+              const uint32_t ss = sc + Cfg::kColBytes;
+              load2(ss, &tmap_sl, 0,
+                    (t.group * p.sf_row_blocks + lane_row / 128) * p.sf_k_blocks + 2 * kb);
+              for (int b = 0; b < Cfg::kScaleCols; ++b)
+                load2(ss + 1024 * (1 + b), &tmap_sc, 0,
+                      (t.col_row / 128 + b) * p.sf_k_blocks + 2 * kb);
+            }
+          }
+        }
+        __syncwarp();
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ======================= UMMA issuer =======================
+    if (is_leader) {
+      uint32_t stage = 0, phase = 0;
+      int count = 0;   // tiles with a contraction so far: their accumulators alternate
+      bool ok = true;
+      for (int tile = worker; ok && tile < num_tiles; tile += num_workers) {
+        const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
+        if (t.blocks == 0) continue;
+        const uint32_t acc = count & 1, acc_phase = (count >> 1) & 1;
+        ++count;
+        if (!__all_sync(0xffffffffu, mbar_wait<kCtaGroup == 2>(tmem_empty_bar + 8 * acc,
+                                                               acc_phase ^ 1, abort_flag))) {
+          if (lane == 0)
+            report_error(p.status, abort_flag, kDevTimeoutMmaTmem, tile, static_cast<int>(acc));
+          break;
+        }
+        tcgen05_fence_after();
+        const uint32_t tmem_d = tmem_base + acc * Cfg::kCols;
+        const uint32_t idesc =
+            kMx ? make_idesc_mxf4(Cfg::kLaneTile, static_cast<uint32_t>(t.mma_n))
+                : make_idesc_bf16(Cfg::kLaneTile, static_cast<uint32_t>(t.mma_n)) |
+                      (Cfg::kOp == kGroupedDx ? kIdescTransposeA : 0u) |
+                      (kDw ? kIdescTransposeA | kIdescTransposeB : 0u);
+        for (int kb = 0; kb < t.blocks; ++kb) {
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait<kDw && kCtaGroup == 2>(full_bar + 8 * stage, phase, abort_flag))) {
+            if (lane == 0)
+              report_error(p.status, abort_flag, kDevTimeoutMmaFull, tile, static_cast<int>(stage));
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const uint32_t sl = ring + stage * Cfg::kStageBytes;
+          const uint32_t sc = sl + Cfg::kLaneBytes;
+          const int steps = min(4, (t.k_len - kb * Cfg::kBlockK + Cfg::kStepK - 1) / Cfg::kStepK);
+          if (elect_one()) {
+            if constexpr (kMx) {
+              const uint32_t ss = sc + Cfg::kColBytes;
+              const uint32_t tsf = tmem_base + 2 * Cfg::kCols + stage * Cfg::kScaleTmemCols;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {   // 128 values of K each
+                tmem_copy_32x128b_x4<kCtaGroup>(tsf + h * 4, make_smem_desc_scales(ss + h * 512));
+#pragma unroll
+                for (int b = 0; b < Cfg::kScaleCols; ++b)
+                  tmem_copy_32x128b_x4<kCtaGroup>(
+                      tsf + 8 + (h * Cfg::kScaleCols + b) * 4,
+                      make_smem_desc_scales(ss + 1024 * (1 + b) + h * 512));
+              }
+              const uint64_t dl = make_smem_desc_sw128(sl), dc = make_smem_desc_sw128(sc);
+              for (int k = 0; k < steps; ++k) {
+                const uint32_t h = k >> 1;
+                umma_mxf4<kCtaGroup>(tmem_d, dl + 2 * k, dc + 2 * k,
+                                     idesc | idesc_scale_bytes((k & 1) * 2), tsf + h * 4,
+                                     tsf + 8 + h * Cfg::kScaleCols * 4, (kb > 0 || k > 0) ? 1u : 0u);
+              }
+            } else {
+              // A K-major operand moves 32 bytes along its swizzled rows per step of 16, an
+              // MN-major one two groups of eight rows.
+              constexpr uint64_t kLaneStep = (Cfg::kOp == kGroupedNt) ? 2 : 128;
+              constexpr uint64_t kColStepDesc = kDw ? 128 : 2;
+              const uint64_t dl = (Cfg::kOp == kGroupedNt) ? make_smem_desc_sw128(sl)
+                                                           : make_smem_desc_mn_sw128(sl, 8192);
+              const uint64_t dc = kDw ? make_smem_desc_mn_sw128(sc, 8192) : make_smem_desc_sw128(sc);
+              for (int k = 0; k < steps; ++k)
+                umma_bf16<kCtaGroup>(tmem_d, dl + kLaneStep * k, dc + kColStepDesc * k, idesc,
+                                     (kb > 0 || k > 0) ? 1u : 0u);
+            }
+            if (kCtaGroup == 2) umma_commit_both_ctas(empty_bar + 8 * stage);
+            else umma_commit<1>(empty_bar + 8 * stage);
+          }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        if (elect_one()) {
+          if (kCtaGroup == 2) umma_commit_both_ctas(tmem_full_bar + 8 * acc);
+          else umma_commit<1>(tmem_full_bar + 8 * acc);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 6) {
+    // ======================= epilogue =======================
+    const int quad = warp & 3;   // the warp's quarter of the tensor-memory lanes
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t stage_buf = epi_base + quad * 4096;
+    uint32_t buf = 0;
+    int count = 0;
+    for (int tile = worker; tile < num_tiles; tile += num_workers) {
+      const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
+      const uint32_t acc = count & 1, acc_phase = (count >> 1) & 1;
+      if (t.blocks > 0) {
+        ++count;
+        if (!__all_sync(0xffffffffu, mbar_wait(tmem_full_bar + 8 * acc, acc_phase, abort_flag))) {
+          if (lane == 0)
+            report_error(p.status, abort_flag, kDevTimeoutEpilogue, tile, static_cast<int>(acc));
+          break;
+        }
+        tcgen05_fence_after();
+      }
+      const int lane_first = t.lane0 + rank * Cfg::kLaneRows + quad * 32;   // of this warp
+      for (int c = t.lo & ~31; c < t.hi; c += 32) {
+        uint32_t r[32];
+        if (t.blocks > 0) {
+          tmem_ld_32x32b_x32(tmem_base + acc * Cfg::kCols + lane_base + c, r);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0u;
+        }
+        const uint32_t s = stage_buf + buf * 2048;
+        buf ^= 1;
+        if constexpr (kDw) {
+          // Lane = row of the result: 64 bytes of it, 16-byte units swizzled against conflicts.
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]),
+                                 __uint_as_float(r[8 * j + 2 * i + 1]));
+            st_shared_v4(s + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
+            uint32_t v[4];
+            ld_shared_v4(s + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4), v);
+            const int n = lane_first + row, col = t.col_row + c + unit * 8;
+            if (n < p.lanes && c + unit * 8 < t.hi) {
+              __nv_bfloat16* dst = p.out + t.group * p.out_stack + n * p.out_pitch + col;
+              if (p.vector_out && c + unit * 8 + 8 <= t.hi) {
+                *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+              } else {
+                const int left = min(t.hi - (c + unit * 8), 8);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (j < left)
+                    reinterpret_cast<unsigned short*>(dst)[j] =
+                        static_cast<unsigned short>(v[j >> 1] >> ((j & 1) * 16));
+              }
+            }
+          }
+        } else {
+          // Lane = column of the result: transposed through shared memory, 32 values of one row
+          // of the batch side by side.
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const uint32_t w = pack_bf16x2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+            st_shared_b16(s + j * 64 + lane * 2, static_cast<unsigned short>(w));
+            st_shared_b16(s + (j + 1) * 64 + lane * 2, static_cast<unsigned short>(w >> 16));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
+            uint32_t v[4];
+            ld_shared_v4(s + row * 64 + unit * 16, v);
+            const int col = lane_first + unit * 8;
+            if (c + row >= t.lo && c + row < t.hi && col < p.lanes) {
+              __nv_bfloat16* dst =
+                  p.out + static_cast<long long>(t.col_row + c + row) * p.out_pitch + col;
+              if (p.vector_out && col + 8 <= p.lanes) {
+                *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+              } else {
+                const int left = min(p.lanes - col, 8);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (j < left)
+                    reinterpret_cast<unsigned short*>(dst)[j] =
+                        static_cast<unsigned short>(v[j >> 1] >> ((j & 1) * 16));
+              }
+            }
+          }
+        }
+      }
+      if (t.blocks > 0) {
+        // The accumulator has been read: hand it back.
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kCtaGroup == 2) mbar_arrive_cluster(mapa_u32(tmem_empty_bar + 8 * acc, 0));
+          else mbar_arrive(tmem_empty_bar + 8 * acc);
+        }
+      }
+    }
+    if (!kDw && p.zero_rest) {
+      // Rows of no group: in front of the first and behind the last.
+      const int head = begin[0], tail = end[p.groups - 1];
+      const int rest = head + p.rows - tail;
+      for (int i = static_cast<int>(blockIdx.x) * 4 + quad; i < rest;
+           i += static_cast<int>(gridDim.x) * 4) {
+        const int row = i < head ? i : tail + i - head;
+        __nv_bfloat16* dst = p.out + static_cast<long long>(row) * p.out_pitch;
+        int c = static_cast<int>(lane) * 8;
+        if (p.vector_out)
+          for (; c + 8 <= p.lanes; c += 256)
+            *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
+        for (; c < p.lanes; c += 256)
+          for (int j = c; j < min(c + 8, p.lanes); ++j) dst[j] = __float2bfloat16_rn(0.f);
+      }
+    }
+  } else if (kDw) {
+    // ======================= rows of the next group =======================
+    uint32_t stage = 0, parities = 0;
+    bool ok = true;
+    for (int tile = worker; ok && tile < num_tiles; tile += num_workers) {
+      const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
+      if (t.blocks == 0) continue;
+      const int valid = t.k_len - (t.blocks - 1) * 64;   // rows of the last block
+      stage = (stage + t.blocks - 1) % kStages;
+      if (valid < 64) {
+        if (!__all_sync(0xffffffffu, mbar_wait(clear_bar + 8 * stage, (parities >> stage) & 1,
+                                               abort_flag))) {
+          if (lane == 0)
+            report_error(p.status, abort_flag, kDevTimeoutProducer, tile, static_cast<int>(stage));
+          ok = false;
+          break;
+        }
+        parities ^= 1u << stage;
+        // A box is 64 rows of 128 bytes; the swizzle moves bytes inside a row only.
+        const uint32_t sl = ring + stage * Cfg::kStageBytes;
+        const int boxes = 2 + (t.mma_n / kCtaGroup + 63) / 64;   // the lane operand's two in front
+        for (int b = 0; b < boxes; ++b)
+          for (uint32_t o = static_cast<uint32_t>(valid) * 128 + lane * 16; o < 8192; o += 512)
+            st_shared_v4(sl + b * 8192 + o, 0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (kCtaGroup == 2) mbar_arrive_release_cluster(mapa_u32(full_bar + 8 * stage, 0));
+          else mbar_arrive(full_bar + 8 * stage);
+        }
+      }
+      stage = (stage + 1) % kStages;
+    }
+  }
+  __syncwarp();
+
+  // ---------------------------------------------------------------- tear-down
+  tcgen05_fence_before();
+  if (kCtaGroup == 2) cluster_sync_all(); else __syncthreads();
+  if (*abort_flag != 0) {
+    // Let boxes still in flight land in this CTA's shared memory before it is released.
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
+  }
+  if (kCtaGroup == 2) cluster_sync_all(); else __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc<1>(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+}  // namespace neogemm

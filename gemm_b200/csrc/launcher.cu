@@ -24,6 +24,7 @@
 #include <vector>
 
 #include "gemm_sm100.cuh"
+#include "host.cuh"
 
 namespace neogemm {
 namespace {
@@ -174,7 +175,7 @@ bool g_encode_looked_up = false;
 
 struct Override {
   int cta_group = -1, block_n = -1, swap = -1, stream_k = -1, group_m = -1, max_ctas = -1;
-  int tuning[13] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};   // see neogemm_set_tuning
+  int tuning[14] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};   // see neogemm_set_tuning
 };
 thread_local Override t_override;
 thread_local int t_last_config[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -1021,6 +1022,31 @@ int ensure_stage(DeviceState* st, int which, size_t bytes) {
 }
 
 }  // namespace
+
+// ------------------------------------------------------------------------------------------
+// For the other translation units (host.cuh)
+// ------------------------------------------------------------------------------------------
+int acquire_device(DeviceView* out) {
+  std::lock_guard<std::mutex> lock(g_mu);
+  int rc;
+  DeviceState* st = device_state(&rc);
+  if (st == nullptr) return rc;
+  if (st->status_host[0] != 0) return NEOGEMM_ERR_DEVICE_TIMEOUT;
+  out->index = static_cast<int>(st - g_dev);
+  out->sm_count = st->sm_count;
+  out->status = st->status_dev;
+  out->encode = g_encode;
+  return NEOGEMM_OK;
+}
+
+int tuning_value(int key) { return t_override.tuning[key]; }
+
+void record_config(int cta_group, int columns, int stages, int swapped, int ctas, int tiles) {
+  const int config[8] = {cta_group, columns, stages, swapped, 0, ctas, tiles, 1};
+  std::memcpy(t_last_config, config, sizeof(config));
+  t_last_store_path = 0;
+}
+
 }  // namespace neogemm
 
 using namespace neogemm;
@@ -1280,7 +1306,7 @@ int neogemm_set_phase_timers(void* device_buffer, size_t bytes) {
 }
 
 int neogemm_set_tuning(int key, int value) {
-  if (key < 0 || key > 12 || (key == 6 && (value == 0 || value > 3)) || (key >= 8 && value > 1) || (key == 7 && value > 4) || (key == 5 && value > 3) || value > 1000000 || (key == 0 && value > 31) || (key == 3 && value > 1) ||
+  if (key < 0 || key > 13 || (key == 6 && (value == 0 || value > 3)) || (key >= 8 && value > 1) || (key == 7 && value > 4) || (key == 5 && value > 3) || value > 1000000 || (key == 0 && value > 31) || (key == 3 && value > 1) ||
       (key == 4 && value > 4))
     return NEOGEMM_ERR_BAD_ARG;
   t_override.tuning[key] = value;

@@ -106,6 +106,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
+// Arrive on a barrier of the cluster after ordinary stores to shared memory that the other CTA's
+// tensor pipe is going to read (the stores are also fenced towards the async proxy by the caller).
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
@@ -262,6 +269,27 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const CUtens
       : "memory");
 }
 
+// Three-dimensional boxes: c0 innermost, c2 the matrix of a stack.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const CUtensorMap* map, uint32_t bar,
+                                            int32_t c0, int32_t c1, int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst_smem, const CUtensorMap* map,
+                                                 uint32_t cluster_bar, int32_t c0, int32_t c1,
+                                                 int32_t c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(c0), "r"(c1),
+        "r"(c2)
+      : "memory");
+}
+
 // L2 eviction-priority policies for the hinted copy forms below.
 __device__ __forceinline__ uint64_t l2_policy_evict_last() {
   uint64_t pol;
@@ -391,6 +419,53 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t desc_a, uint
   }
 }
 
+// D[tmem] (+)= (A scaled) * (B scaled): E2M1 operands packed two to a byte, one E8M0 scale per 32
+// values of K for every row of A and of B (K = 64 per instruction, two scales a row), fp32
+// accumulate.  The scales sit in tensor memory: row r in lane r % 32 (repeated in all four lane
+// quadrants), column r / 32, one byte per block of 32; the instruction descriptor says which pair
+// of the word's four bytes this K step uses.
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b,
+                                          uint32_t idesc, uint32_t tmem_sfa, uint32_t tmem_sfb,
+                                          uint32_t accumulate) {
+  if constexpr (kCtaGroup == 1) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+        "}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb),
+          "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+        "}\n"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb),
+          "r"(accumulate)
+        : "memory");
+  }
+}
+
+// shared -> tensor memory: 32 rows of 16 bytes (512 contiguous bytes) into 32 lanes x 4 columns,
+// repeated in all four lane quadrants.  Issued by the thread that issues the MMAs that read it,
+// with which it is ordered.  With two CTAs each copies from its own shared memory at the same
+// offset.
+template <int kCtaGroup>
+__device__ __forceinline__ void tmem_copy_32x128b_x4(uint32_t taddr, uint64_t desc) {
+  if constexpr (kCtaGroup == 1) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+  } else {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+  }
+}
+
 // Arrive (count 1) on `bar` once every tcgen05 operation issued so far by this thread has
 // completed.  `bar` is a shared::cluster address: this CTA's own barrier (a shared::cta address is
 // valid there) or the peer's (from mapa_u32).  One barrier per commit; to signal both CTAs of a
@@ -472,6 +547,33 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t smem_addr) {
   d |= 1ull << 46;
   d |= 2ull << 61;
   return d;
+}
+
+// The same for an operand whose contraction index runs along the rows in memory (MN-major): a box
+// is 64 elements of M or N (128 bytes, swizzled) by `rows` rows of K.  The stride field holds the
+// distance between groups of 8 K rows (1024 B), the leading-dimension field that between boxes
+// of 64 M or N elements.
+__device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(uint32_t smem_addr, uint32_t box_bytes) {
+  return make_smem_desc_sw128(smem_addr) | (static_cast<uint64_t>(box_bytes >> 4) << 16);
+}
+constexpr uint32_t kIdescTransposeA = 1u << 15;   // A is MN-major
+constexpr uint32_t kIdescTransposeB = 1u << 16;   // B is MN-major
+
+// Descriptor of 512 contiguous bytes of scales, read as 32 rows of 16 bytes without swizzle:
+// groups of 8 rows are 128 bytes apart.
+__device__ __forceinline__ uint64_t make_smem_desc_scales(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128u >> 4) << 32) |
+         (1ull << 46);
+}
+
+// Instruction descriptor for kind::mxf4: E2M1 A and B (1 in bits 7-9 and 10-11), E8M0 scales
+// (bit 23), N>>3 in bits 17-22, M>>7 in bits 27-28; which bytes of the scale words a K step uses
+// goes into bits 29-30 (A) and 4-5 (B).
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(uint32_t mma_m, uint32_t mma_n) {
+  return (1u << 7) | (1u << 10) | ((mma_n >> 3) << 17) | (1u << 23) | ((mma_m >> 7) << 27);
+}
+__host__ __device__ constexpr uint32_t idesc_scale_bytes(uint32_t first_byte) {
+  return (first_byte << 4) | (first_byte << 29);
 }
 
 // Packs two fp32 into one bf16x2 word with round-to-nearest-even, the rounding of

@@ -12,7 +12,7 @@ torch is used here for device memory and streams only.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -180,6 +180,240 @@ def matmul_host(A_host: torch.Tensor, B_host: torch.Tensor, C_host: torch.Tensor
     return C_host
 
 
+# ----------------------------------------------------------------------------------------------
+# Products grouped by expert
+# ----------------------------------------------------------------------------------------------
+def _check_offsets(offsets: torch.Tensor, device: torch.device) -> int:
+    """Number of groups of an ``offsets`` vector."""
+    if not isinstance(offsets, torch.Tensor):
+        raise TypeError("offsets must be a torch.Tensor")
+    if offsets.device != device:
+        raise ValueError(f"offsets must be on {device}")
+    if offsets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"offsets must be int32 or int64, got {offsets.dtype}")
+    if offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
+        raise ValueError("offsets must be a contiguous vector of groups + 1 row indices")
+    return int(offsets.numel()) - 1
+
+
+def _check_stack(name: str, w: torch.Tensor, device: torch.device):
+    """(pitch, distance between matrices) of a [groups, N, K] operand with contiguous rows."""
+    if not isinstance(w, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if w.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    if w.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16, got {w.dtype}")
+    if w.dim() != 3:
+        raise ValueError(f"{name} must be [groups, N, K], got shape {tuple(w.shape)}")
+    if w.size(2) > 1 and w.stride(2) != 1:
+        raise ValueError(f"{name} must have unit stride along its last dimension")
+    pitch = int(w.stride(1)) if w.size(1) > 1 else max(int(w.size(2)), 1)
+    # The pitch of a single row is nobody's to read, but it has to be a legal one.
+    if w.size(1) <= 1:
+        pitch = -(-pitch // 8) * 8
+    return pitch, int(w.stride(0)) if w.size(0) > 1 else 0
+
+
+def _rows_pitch(name: str, t: torch.Tensor) -> int:
+    """Row pitch of an operand that is read; a single row gets the next legal one."""
+    pitch = _row_pitch(name, t)
+    return pitch if t.size(0) > 1 else -(-pitch // 8) * 8
+
+
+def _rows_out(out: Optional[torch.Tensor], T: int, width: int, device: torch.device):
+    if out is None:
+        return torch.empty((T, width), dtype=torch.bfloat16, device=device), 1
+    _require_cuda_bf16_matrix("out", out)
+    if tuple(out.shape) != (T, width) or out.device != device:
+        raise ValueError(f"out must be [{T},{width}] on {device}")
+    return out, 0
+
+
+def _grouped_rows(fn, name: str, rows: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+                  out: Optional[torch.Tensor], transposed: bool) -> torch.Tensor:
+    _require_cuda_bf16_matrix(name, rows)
+    pitch_w, stack_w = _check_stack("w", w, rows.device)
+    groups = _check_offsets(offsets, rows.device)
+    if int(w.size(0)) != groups:
+        raise ValueError(f"w has {int(w.size(0))} matrices but offsets delimit {groups} groups")
+    T, N, K = int(rows.size(0)), int(w.size(1)), int(w.size(2))
+    depth, width = (N, K) if transposed else (K, N)
+    if int(rows.size(1)) != depth:
+        raise ValueError(f"{name} is [{T},{int(rows.size(1))}] but w is [groups,{N},{K}]: expected "
+                         f"rows of {depth}")
+    out, zero_rest = _rows_out(out, T, width, rows.device)
+    with torch.cuda.device(rows.device):
+        rc = fn(rows.data_ptr(), w.data_ptr(), out.data_ptr(), offsets.data_ptr(),
+                1 if offsets.dtype == torch.int64 else 0, groups, T, N, K, _rows_pitch(name, rows),
+                pitch_w, stack_w, _row_pitch("out", out), zero_rest, _stream_ptr(rows.device))
+    check(rc)
+    return out
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] = x[t] @ w[e]^T for the rows t of group e, offsets[e] <= t < offsets[e+1].
+
+    ``x`` is bf16 [T, K] sorted by group, ``w`` bf16 [groups, N, K] (each matrix laid out like
+    ``linear``'s weight), ``offsets`` groups + 1 ascending row indices (int32 or int64) on the same
+    device; they are read on the GPU only.  Rows and matrices may be strided (contiguous along K,
+    pitches multiples of 8).  Groups may be empty; at most 1024 of them.  Without ``out`` the rows
+    of no group are zero; with ``out`` (bf16 [T, N], contiguous rows) they are left as they are."""
+    return _grouped_rows(lib.neogemm_grouped_nt, "x", x, w, offsets, out, False)
+
+
+def grouped_matmul_dx(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of :func:`grouped_matmul` by its rows: dx[t] = dy[t] @ w[e].  ``dy`` is bf16
+    [T, N]; everything else as there."""
+    return _grouped_rows(lib.neogemm_grouped_dx, "dy", dy, w, offsets, out, True)
+
+
+def grouped_matmul_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of :func:`grouped_matmul` by its matrices: dw[e] = sum over the group's rows of
+    dy[t]^T x[t], bf16 [groups, N, K]; zero for an empty group.  ``out`` must be contiguous."""
+    _require_cuda_bf16_matrix("dy", dy)
+    _require_cuda_bf16_matrix("x", x)
+    if x.device != dy.device:
+        raise ValueError("dy and x must be on the same device")
+    groups = _check_offsets(offsets, dy.device)
+    T, N, K = int(dy.size(0)), int(dy.size(1)), int(x.size(1))
+    if int(x.size(0)) != T:
+        raise ValueError(f"dy has {T} rows but x has {int(x.size(0))}")
+    if out is None:
+        out = torch.empty((groups, N, K), dtype=torch.bfloat16, device=dy.device)
+    elif (not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16
+          or out.device != dy.device or tuple(out.shape) != (groups, N, K)
+          or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous bfloat16 [{groups},{N},{K}] on {dy.device}")
+    with torch.cuda.device(dy.device):
+        rc = lib.neogemm_grouped_dw(dy.data_ptr(), x.data_ptr(), out.data_ptr(),
+                                    offsets.data_ptr(), 1 if offsets.dtype == torch.int64 else 0,
+                                    groups, T, N, K, _rows_pitch("dy", dy), _rows_pitch("x", x),
+                                    _stream_ptr(dy.device))
+    check(rc)
+    return out
+
+
+# ----------------------------------------------------------------------------------------------
+# Microscaled 4-bit floating point
+# ----------------------------------------------------------------------------------------------
+class MxFp4(NamedTuple):
+    """A matrix [rows, K] (or a stack of them) in MXFP4.
+
+    ``codes``: uint8 [..., rows, K/2], E2M1 values two to a byte, the even k in the low four bits.
+    ``scales``: uint8 [..., ceil(rows/128), ceil(K/128), 32, 4, 4]; the E8M0 scale of row r and block
+    b = k // 32 is at [r // 128, b // 4, r % 32, r % 128 // 32, b % 4].  Both contiguous."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _check_mxfp4(name: str, q: MxFp4, dims: tuple, device: Optional[torch.device] = None):
+    """(shape [.., rows, K], device) of an MXFP4 operand with as many dimensions as ``dims`` allows."""
+    if not isinstance(q, tuple) or len(q) != 2 or not all(isinstance(t, torch.Tensor) for t in q):
+        raise TypeError(f"{name} must be an MxFp4 (codes, scales)")
+    codes, scales = q
+    if not codes.is_cuda:
+        raise ValueError(f"{name} must live on a CUDA device (there is no CPU path)")
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError(f"{name}: codes and scales must be uint8")
+    if codes.dim() not in dims:
+        raise ValueError(f"{name}: codes must have {' or '.join(map(str, dims))} dimensions, got "
+                         f"shape {tuple(codes.shape)}")
+    if scales.device != codes.device or (device is not None and codes.device != device):
+        raise ValueError(f"{name}: all operands must be on the same device")
+    rows, K = int(codes.shape[-2]), 2 * int(codes.shape[-1])
+    want = (*codes.shape[:-2], -(-rows // 128), -(-K // 128), 32, 4, 4)
+    if tuple(scales.shape) != want:
+        raise ValueError(f"{name}: scales of codes {tuple(codes.shape)} must be {want}, got "
+                         f"{tuple(scales.shape)}")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{name}: codes and scales must be contiguous")
+    return (*map(int, codes.shape[:-2]), rows, K), codes.device
+
+
+def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
+    """bf16 or fp32 [rows, K] or [stack, rows, K] (contiguous along K, K a multiple of 32) to MXFP4:
+    per row and 32 values one scale 2^(floor(log2(largest magnitude)) - 2), values rounded to the
+    nearest code (ties to even) and saturated at 6 scales.  A block with an Inf or NaN becomes NaN."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    if not x.is_cuda:
+        raise ValueError("x must live on a CUDA device (there is no CPU path)")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"x must be bfloat16 or float32, got {x.dtype}")
+    if x.dim() not in (2, 3):
+        raise ValueError(f"x must be [rows, K] or [stack, rows, K], got shape {tuple(x.shape)}")
+    rows, K = int(x.size(-2)), int(x.size(-1))
+    stack = int(x.size(0)) if x.dim() == 3 else 1
+    if K % 32 != 0:
+        raise ValueError(f"K must be a multiple of 32, got {K}")
+    if K > 1 and x.stride(-1) != 1:
+        raise ValueError("x must have unit stride along its last dimension")
+    pitch = int(x.stride(-2)) if rows > 1 else K
+    codes = torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-2], -(-rows // 128), -(-K // 128), 32, 4, 4),
+                         dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        rc = lib.neogemm_mxfp4_quantize(x.data_ptr(), 1 if x.dtype == torch.float32 else 0,
+                                        codes.data_ptr(), scales.data_ptr(), stack, rows, K, pitch,
+                                        int(x.stride(0)) if x.dim() == 3 and stack > 1 else 0,
+                                        _stream_ptr(x.device))
+    check(rc)
+    return MxFp4(codes, scales)
+
+
+def dequantize_mxfp4(q: MxFp4) -> torch.Tensor:
+    """The values of an MXFP4 matrix (or stack) as bf16, which holds them exactly."""
+    shape, device = _check_mxfp4("q", q, (2, 3))
+    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    with torch.cuda.device(device):
+        rc = lib.neogemm_mxfp4_dequantize(q[0].data_ptr(), q[1].data_ptr(), out.data_ptr(),
+                                          shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1],
+                                          _stream_ptr(device))
+    check(rc)
+    return out
+
+
+def matmul_mxfp4(a: MxFp4, b: MxFp4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """C[M,N] = A[M,K] @ B[N,K]^T of two MXFP4 matrices, fp32 accumulation, bf16 result.  K must be
+    a multiple of 64.  ``out`` may be any bf16 [M,N] tensor with contiguous rows."""
+    (M, K), device = _check_mxfp4("a", a, (2,))
+    (N, Kb), _ = _check_mxfp4("b", b, (2,), device)
+    if Kb != K:
+        raise ValueError(f"a is [M,K]=[{M},{K}] but b is [N,K]=[{N},{Kb}]: K differs")
+    out, _ = _rows_out(out, M, N, device)
+    with torch.cuda.device(device):
+        rc = lib.neogemm_mxfp4_nt(a[0].data_ptr(), a[1].data_ptr(), b[0].data_ptr(),
+                                  b[1].data_ptr(), out.data_ptr(), M, N, K,
+                                  _row_pitch("out", out), _stream_ptr(device))
+    check(rc)
+    return out
+
+
+def grouped_matmul_mxfp4(x: MxFp4, w: MxFp4, offsets: torch.Tensor,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`grouped_matmul` with both operands in MXFP4: ``x`` [T, K], ``w`` [groups, N, K], K a
+    multiple of 64."""
+    (T, K), device = _check_mxfp4("x", x, (2,))
+    (matrices, N, Kw), _ = _check_mxfp4("w", w, (3,), device)
+    groups = _check_offsets(offsets, device)
+    if matrices != groups:
+        raise ValueError(f"w has {matrices} matrices but offsets delimit {groups} groups")
+    if Kw != K:
+        raise ValueError(f"x is [T,K]=[{T},{K}] but w is [groups,N,K]=[{groups},{N},{Kw}]: K differs")
+    out, zero_rest = _rows_out(out, T, N, device)
+    with torch.cuda.device(device):
+        rc = lib.neogemm_grouped_mxfp4_nt(x[0].data_ptr(), x[1].data_ptr(), w[0].data_ptr(),
+                                          w[1].data_ptr(), out.data_ptr(), offsets.data_ptr(),
+                                          1 if offsets.dtype == torch.int64 else 0, groups, T, N, K,
+                                          _row_pitch("out", out), zero_rest, _stream_ptr(device))
+    check(rc)
+    return out
+
+
 def workspace_bytes(M: int, N: int, K: int, col_major: bool = False) -> int:
     return int(lib.neogemm_workspace_bytes(M, N, K, 1 if col_major else 0))
 
@@ -217,7 +451,7 @@ TUNING_KEYS = {"l2_hints": 0, "epilogue_wait_hint_ns": 1, "ring_wait_hint_ns": 2
                "dynamic_pieces_per_tile": 4, "l2_promotion": 5, "wide_tile_prologue": 6,
                "two_ctas_per_sm": 7, "wave_pacing": 8,
                "k_direction_alternates": 9, "setup_overlap": 10,
-               "two_pass_split_k": 11, "narrow_tiles": 12}
+               "two_pass_split_k": 11, "narrow_tiles": 12, "grouped_wide_tiles": 13}
 
 
 def set_tuning(key: str, value: int = -1) -> None:
@@ -226,5 +460,7 @@ def set_tuning(key: str, value: int = -1) -> None:
 
 
 __all__ = ["neoGemmV1", "neogemm", "matmul", "matmul_fused", "linear", "matmul_host", "workspace_bytes",
+           "grouped_matmul", "grouped_matmul_dx", "grouped_matmul_dw", "MxFp4", "quantize_mxfp4",
+           "dequantize_mxfp4", "matmul_mxfp4", "grouped_matmul_mxfp4",
            "device_status", "clear_device_status", "last_config", "last_store_path", "set_override",
            "set_tuning", "NeoGemmError"]

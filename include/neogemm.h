@@ -154,6 +154,72 @@ int neogemm_noalloc_init(void);
 int neogemm_noalloc_status(int out[4], void* stream);
 int neogemm_noalloc_clear_status(void);
 
+/* ---- Products grouped by expert -----------------------------------------------------------------
+ *
+ * A batch of T rows is sorted by group (expert); group e owns the rows offsets[e] .. offsets[e+1]-1
+ * and has a matrix of its own, W[e].  `offsets` is device memory: groups + 1 ascending indices
+ * between 0 and T, int32 or (offsets_are_64) int64.  Nothing is read back to the host: the tiles
+ * are laid out on the GPU, so a captured graph replays with other group sizes.  Indices that
+ * descend or leave [0, T] are clamped (no access outside the operands) and recorded as a device
+ * error, code 6 with field 3 = 4 (see neogemm_device_status).
+ *
+ *   neogemm_grouped_nt   Y[t,n]    = sum_k X[t,k] W[e][n,k]       t in group e
+ *   neogemm_grouped_dx   dX[t,k]   = sum_n dY[t,n] W[e][n,k]      its gradient by the rows
+ *   neogemm_grouped_dw   dW[e][n,k] = sum_{t in e} dY[t,n] X[t,k] and by the matrices
+ *
+ * bf16 in and out, fp32 accumulation, one rounding.  Layouts (leading dimensions in elements):
+ *   X, dX [T,K] at x[t*ldx + k]; Y, dY [T,N] at y[t*ldy + n];
+ *   W [groups,N,K] at w[e*stack_w + n*ldw + k];  dW [groups,N,K] packed.
+ * Operands that are read have 16-byte aligned bases and leading dimensions (and stack_w) that are
+ * multiples of 8; results may have any leading dimension (16-byte stores need multiples of 8).
+ * T, N, K >= 0; an empty group is allowed (its dW is zero).  1 <= groups <= 1024 (0 groups: no-op).
+ * zero_rest != 0 writes zeros to the rows of Y or dX that belong to no group (in front of offsets[0],
+ * behind offsets[groups]); 0 leaves them as they are.  The sums of a row do not depend on the
+ * other rows, and no atomics are used: results are the same bits from call to call.
+ * No workspace; no counterpart in the reference. */
+int neogemm_grouped_nt(const void* X, const void* W, void* Y, const void* offsets,
+                       int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                       int64_t ldx, int64_t ldw, int64_t stack_w, int64_t ldy, int zero_rest,
+                       void* stream);
+int neogemm_grouped_dx(const void* dY, const void* W, void* dX, const void* offsets,
+                       int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                       int64_t lddy, int64_t ldw, int64_t stack_w, int64_t lddx, int zero_rest,
+                       void* stream);
+int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offsets,
+                       int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                       int64_t lddy, int64_t ldx, void* stream);
+
+/* ---- Microscaled 4-bit floating point (MXFP4) ----------------------------------------------------
+ *
+ * A matrix [rows, K] is held as
+ *   codes   [rows, K/2] bytes: E2M1 values (0 .5 1 1.5 2 3 4 6, sign in bit 3), two to a byte, the
+ *           even k in the low four bits;
+ *   scales  one E8M0 byte s (2^(s-127), 255 = NaN) per row and 32 consecutive k, in tiles of 128
+ *           rows x 128 values of K: byte [row/128][k/128][row%32][row%128/32][k/32%4] of an array
+ *           [ceil(rows/128), ceil(K/128), 32, 4, 4] - the order in which the tensor core takes them.
+ * A stack of matrices has one such pair after another.  Both are packed and 16-byte aligned.
+ *
+ * neogemm_mxfp4_quantize: the scale of a block is 2^(floor(log2(largest magnitude)) - 2), at least
+ *   2^-127; values are rounded to the nearest code, ties to even, and saturate at 6.  A block that
+ *   holds an Inf or a NaN gets the scale 255 and codes 0.  Padding bytes of `scales` are written
+ *   as 0.  X: bf16 (x_is_f32 = 0) or fp32, 16-byte aligned, element (i,r,k) at
+ *   x[i*stack_x + r*ldx + k], ldx and stack_x multiples of 8.  K % 32 == 0.
+ * neogemm_mxfp4_dequantize: the values as packed bf16 [stack, rows, K] (exact).  K % 32 == 0.
+ * neogemm_mxfp4_nt: C[m,n] = sum_k A[m,k] B[n,k], fp32 accumulation, bf16 result with row pitch
+ *   ldc.  K % 64 == 0.  Padding bytes of the scales have no influence.
+ * neogemm_grouped_mxfp4_nt: neogemm_grouped_nt with both operands in MXFP4. */
+int neogemm_mxfp4_quantize(const void* X, int x_is_f32, void* codes, void* scales, int64_t stack,
+                           int64_t rows, int64_t K, int64_t ldx, int64_t stack_x, void* stream);
+int neogemm_mxfp4_dequantize(const void* codes, const void* scales, void* Y, int64_t stack,
+                             int64_t rows, int64_t K, void* stream);
+int neogemm_mxfp4_nt(const void* A_codes, const void* A_scales, const void* B_codes,
+                     const void* B_scales, void* C, int64_t M, int64_t N, int64_t K, int64_t ldc,
+                     void* stream);
+int neogemm_grouped_mxfp4_nt(const void* X_codes, const void* X_scales, const void* W_codes,
+                             const void* W_scales, void* Y, const void* offsets,
+                             int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
+                             int64_t ldy, int zero_rest, void* stream);
+
 /* Upper bound on the workspace neogemm_bf16_nt() may need for this shape on the current device
  * (0 when the data-parallel schedule would be chosen).  No counterpart in the reference, which
  * has no split-K. */
@@ -175,7 +241,8 @@ int neogemm_bf16_nt_host(const void* A_host, const void* B_host, void* C_host,
 
 /* Device-side error record of the current device: out[0] = code (0 none; 1 producer wait expired,
  * 2 MMA operand wait, 3 MMA accumulator wait, 4 epilogue wait, 5 tensor-memory address,
- * 6 an index failed the kernel's own bounds check and the access was skipped, 7 a wait on the
+ * 6 an index failed the kernel's own bounds check and the access was skipped (out[3] = 4: group
+ * offsets, clamped), 7 a wait on the
  * run-time work queue expired),
  * out[1] = CTA index, out[2] = segment index, out[3] = ring stage or accumulator.  Meaningful once
  * the stream of the launch has been synchronised.  The reference only prints cudaGetLastError
@@ -251,6 +318,8 @@ int neogemm_set_override(int cta_group, int block_n, int swap, int stream_k, int
  *          only publishes fp32 partials and a reduction kernel launched right behind it sums
  *          them, applies the epilogue and stores C; 0: wide tiles are not cut at all and the
  *          last contributor of a cut narrow tile sums it alone (the earlier behaviour).
+ *   key 13: tiles of the grouped and MXFP4 products: -1 chosen from the average group, 0 narrow
+ *          (one CTA), 1 wide.
  *   key 12: 128 x 64 tiles for small problems (twice as many CTAs as 128 x 128 tiles): -1 when
  *          the 128 x 128 tiles would occupy at most half of the SMs, 0 never, 1 whenever the
  *          single-CTA 128 x 128 TMA-store kernel would be used.
