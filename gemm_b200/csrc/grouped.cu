@@ -17,68 +17,67 @@ constexpr int64_t kMaxExtent = 0x7fffffffll - 4096;   // room for tile coordinat
 
 struct KernelEntry {
   int op, cta_group, columns, stages;
+  bool stream;
+  int lane_step;   // lanes of a tile (streaming: of a unit)
+  int col_step;    // granularity of a tile's columns
+  int lane_box;        // rows of the lane operand's boxes
+  int ring_bytes, scale_bytes;   // shared memory: the ring, and the scales of a k-block
   const void* fn;
   int smem_bytes, threads;
 };
 
 template <class Cfg>
 KernelEntry make_entry() {
-  return KernelEntry{Cfg::kOp, Cfg::kCtaGroup, Cfg::kCols, Cfg::kStages,
+  constexpr bool kDw = Cfg::kOp == kGroupedDw;
+  return KernelEntry{Cfg::kOp, Cfg::kCtaGroup, Cfg::kCols, Cfg::kStages, Cfg::kStream,
+                     Cfg::kStream ? Cfg::kUnit : Cfg::kLaneTile,
+                     Cfg::kColStep,
+                     // MN-major operands come in boxes of 64 x 64
+                     kDw || Cfg::kOp == kGroupedDx ? 64 : 128,
+                     Cfg::kRingBytes, Cfg::kScaleBytes,
                      reinterpret_cast<const void*>(&grouped_kernel<Cfg>), Cfg::kSmemBytes,
                      Cfg::kThreads};
 }
 
 // [operation][0 narrow, 1 wide]
 const KernelEntry kKernels[4][2] = {
-    {make_entry<GroupedConfig<kGroupedNt, 1, 64, 8>>(), make_entry<GroupedConfig<kGroupedNt, 2, 256, 6>>()},
-    {make_entry<GroupedConfig<kGroupedDx, 1, 64, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 256, 6>>()},
+    {make_entry<GroupedConfig<kGroupedNt, 1, 128, 8>>(), make_entry<GroupedConfig<kGroupedNt, 2, 256, 6>>()},
+    {make_entry<GroupedConfig<kGroupedDx, 1, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 256, 6>>()},
     {make_entry<GroupedConfig<kGroupedDw, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 256, 6>>()},
-    {make_entry<GroupedConfig<kMxNt, 1, 128, 5>>(), make_entry<GroupedConfig<kMxNt, 1, 128, 5>>()},
+    {make_entry<GroupedConfig<kMxNt, 1, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 1, 128, 8>>()},
 };
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tensor map of `rank` dimensions, innermost first; strides (bytes) of dimensions 1 and up.
-int encode(const DeviceView& dev, CUtensorMap* map, CUtensorMapDataType type, int rank,
-           const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
-           bool swizzle) {
-  const cuuint32_t ones[3] = {1, 1, 1};
-  cuuint64_t d[3], s[2];
-  cuuint32_t b[3];
-  for (int i = 0; i < rank; ++i) {
-    d[i] = dims[i];
-    b[i] = box[i];
-    if (i > 0) s[i - 1] = strides[i - 1];
-    if (i > 0 && (strides[i - 1] >= (1ull << 40) || strides[i - 1] % 16 != 0)) return NEOGEMM_ERR_UNSUPPORTED;
-  }
+// Tensor map of a stack of matrices, innermost dimension first; pitches in bytes.  Every operand has
+// three dimensions, so that one copy instruction serves all of them.
+int encode(const DeviceView& dev, CUtensorMap* map, CUtensorMapDataType type, const void* base,
+           int64_t inner, int64_t rows, int64_t stack, int64_t pitch, int64_t stack_pitch,
+           uint32_t box_inner, uint32_t box_rows, bool swizzle) {
+  if (pitch % 16 != 0 || stack_pitch % 16 != 0 || pitch >= (1ll << 40) || stack_pitch >= (1ll << 40))
+    return NEOGEMM_ERR_UNSUPPORTED;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(stack)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(stack_pitch)};
+  const cuuint32_t box[3] = {box_inner, box_rows, 1}, ones[3] = {1, 1, 1};
   const CUresult r = dev.encode(
-      map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, b, ones,
+      map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
       CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? NEOGEMM_OK : NEOGEMM_ERR_DESCRIPTOR;
 }
 
-int encode_matrix(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t inner,
-                  int64_t rows, int64_t pitch, uint32_t box_rows) {
-  const uint64_t dims[2] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(rows)};
-  const uint64_t strides[1] = {static_cast<uint64_t>(pitch) * 2};
-  const uint32_t box[2] = {64, box_rows};
-  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, true);
-}
-
-int encode_stack(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t inner,
-                 int64_t rows, int64_t stack, int64_t pitch, int64_t stack_pitch, uint32_t box_rows) {
-  const uint64_t dims[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(rows),
-                            static_cast<uint64_t>(stack)};
-  const uint64_t strides[2] = {static_cast<uint64_t>(pitch) * 2,
-                               static_cast<uint64_t>(stack == 1 ? rows * pitch : stack_pitch) * 2};
-  const uint32_t box[3] = {64, box_rows, 1};
-  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, true);
+// bf16 matrices, boxes of 64 elements (a 128-byte swizzle row); pitches in elements.  A single
+// matrix's distance to the next is nobody's to use.
+int encode_bf16(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t inner,
+                int64_t rows, int64_t stack, int64_t pitch, int64_t stack_pitch, int64_t box_rows) {
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, inner, rows, stack, pitch * 2,
+                (stack == 1 ? pitch : stack_pitch) * 2, 64, static_cast<uint32_t>(box_rows), true);
 }
 
 int launch(const DeviceView& dev, const KernelEntry& k, int64_t tiles_at_most,
-           const CUtensorMap (&maps)[4], const GroupedParams& params, cudaStream_t stream) {
+           const CUtensorMap (&maps)[5], const GroupedParams& params, cudaStream_t stream) {
   static std::mutex mu;
   static bool attr_done[kMaxDevices][4][2] = {};
   const int which = &k == &kKernels[k.op][1] ? 1 : 0;
@@ -117,9 +116,9 @@ int launch(const DeviceView& dev, const KernelEntry& k, int64_t tiles_at_most,
   }
   cfg.attrs = attr;
   cfg.numAttrs = nattr;
-  void* args[5] = {const_cast<CUtensorMap*>(&maps[0]), const_cast<CUtensorMap*>(&maps[1]),
+  void* args[6] = {const_cast<CUtensorMap*>(&maps[0]), const_cast<CUtensorMap*>(&maps[1]),
                    const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]),
-                   const_cast<GroupedParams*>(&params)};
+                   const_cast<CUtensorMap*>(&maps[4]), const_cast<GroupedParams*>(&params)};
   if (cudaLaunchKernelExC(&cfg, k.fn, args) != cudaSuccess) {
     cudaGetLastError();
     return NEOGEMM_ERR_LAUNCH;
@@ -149,6 +148,36 @@ int zero_rows(void* out, int64_t pitch, int64_t rows, int64_t width, cudaStream_
     cudaGetLastError();
     return NEOGEMM_ERR_CUDA;
   }
+  return NEOGEMM_OK;
+}
+
+// Sizes that the rows' products share.  Streaming kernels keep as many columns per tile as a group
+// is likely to need (four times the average and some); a group of more rows reads its matrix once per
+// tile.
+int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, GroupedParams* p,
+              int64_t* tiles_at_most) {
+  int64_t cap = k.columns;
+  if (k.stream) {
+    // MXFP4 tiles take their rows from a frame of the whole batch.
+    const int64_t likely = k.op == kMxNt ? T : std::min(T, 4 * (T / groups) + 16);
+    cap = std::min(cap, ceil_div(likely, k.col_step) * k.col_step);
+  }
+  const int64_t lane_tiles = ceil_div(lanes, k.lane_step);
+  // Tiles that keep to a grid of rows may touch one more than the group's length says.
+  const int64_t tiles = lane_tiles * (2 * std::min(groups, T) + T / (k.op == kMxNt ? k.columns : cap));
+  if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
+  p->col_cap = static_cast<int>(cap);
+  p->col_box = cap <= 16 ? 16 : 32;
+  if (k.stream) {
+    // Slots of two full k-blocks where four of them fit: half the waits and copies of 256 bytes of
+    // a row in a row.  Behind the last slot an MMA reads up to one k-block's lanes.
+    const int block = 128 * 128 + p->col_box * static_cast<int>(ceil_div(cap, p->col_box)) * 128 + k.scale_bytes;
+    const int room = k.ring_bytes - 128 * 128;
+    p->slot_bytes = room / (2 * block) >= 4 ? 2 * block : block;
+    p->slots = std::min(k.stages, room / p->slot_bytes);
+  }
+  p->lane_tiles = static_cast<int>(lane_tiles);
+  *tiles_at_most = tiles;
   return NEOGEMM_OK;
 }
 
@@ -184,13 +213,6 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   if (rc != NEOGEMM_OK) return rc;
 
   const KernelEntry& k = kKernels[op][take_wide(T / groups) ? 1 : 0];
-  CUtensorMap maps[4];
-  std::memset(maps, 0, sizeof(maps));
-  if (depth > 0) {
-    rc = encode_stack(dev, &maps[0], W, K, N, groups, ldw, stack_w, op == kGroupedDx ? 64 : 128);
-    if (rc == NEOGEMM_OK) rc = encode_matrix(dev, &maps[1], R, depth, T, ldr, 32);
-    if (rc != NEOGEMM_OK) return rc;
-  }
   GroupedParams p;
   std::memset(&p, 0, sizeof(p));
   p.offsets = offsets;
@@ -199,10 +221,18 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   p.rows = static_cast<int>(T);
   p.lanes = static_cast<int>(lanes);
   p.depth = static_cast<int>(depth);
-  const int64_t lane_tiles = ceil_div(lanes, 128 * k.cta_group);
-  const int64_t tiles = lane_tiles * (std::min(groups, T) + T / k.columns);
-  if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
-  p.lane_tiles = static_cast<int>(lane_tiles);
+  int64_t tiles;
+  rc = fill_rows(k, groups, T, lanes, &p, &tiles);
+  if (rc != NEOGEMM_OK) return rc;
+  CUtensorMap maps[5];   // lanes, lanes by units, columns, scales of both
+  std::memset(maps, 0, sizeof(maps));
+  if (depth > 0) {
+    rc = encode_bf16(dev, &maps[0], W, K, N, groups, ldw, stack_w, k.lane_box);
+    if (rc == NEOGEMM_OK && k.stream)
+      rc = encode_bf16(dev, &maps[1], W, K, N, groups, ldw, stack_w, k.lane_step);
+    if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps[2], R, depth, T, 1, ldr, 0, p.col_box);
+    if (rc != NEOGEMM_OK) return rc;
+  }
   p.zero_rest = zero_rest;
   p.vector_out = ldo % 8 == 0 && aligned16(out);
   p.out = static_cast<__nv_bfloat16*>(out);
@@ -213,20 +243,13 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
 
 // Scale tiles as a matrix of 512-byte rows, read two at a time.
 int encode_scales(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t tiles) {
-  const uint64_t dims[2] = {128, static_cast<uint64_t>(tiles)};
-  const uint64_t strides[1] = {512};
-  const uint32_t box[2] = {128, 2};
-  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, base, dims, strides, box, false);
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, tiles, 1, 512, 512, 128, 2, false);
 }
 
 int encode_codes(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t K, int64_t rows,
-                 int64_t stack, uint32_t box_rows) {
-  const uint64_t bytes = static_cast<uint64_t>(K) / 2;
-  const uint64_t dims[3] = {bytes, static_cast<uint64_t>(rows), static_cast<uint64_t>(stack)};
-  const uint64_t strides[2] = {bytes, bytes * static_cast<uint64_t>(rows)};
-  const uint32_t box[3] = {128, box_rows, 1};
-  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, stack > 0 ? 3 : 2, base, dims, strides, box,
-                true);
+                 int64_t stack, int64_t box_rows) {
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, K / 2, rows, stack, K / 2,
+                stack == 1 ? K / 2 : K / 2 * rows, 128, static_cast<uint32_t>(box_rows), true);
 }
 
 int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void* Y,
@@ -249,15 +272,6 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
   const int64_t k_tiles = ceil_div(K, 128), w_tiles = ceil_div(N, 128), x_tiles = ceil_div(T, 128);
   if (groups * w_tiles * k_tiles > kMaxExtent || x_tiles * k_tiles > kMaxExtent)
     return NEOGEMM_ERR_UNSUPPORTED;
-  CUtensorMap maps[4];
-  std::memset(maps, 0, sizeof(maps));
-  if (K > 0) {
-    rc = encode_codes(dev, &maps[0], Wc, K, N, groups, 128);
-    if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps[1], Xc, K, T, 0, 32);
-    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[2], Ws, groups * w_tiles * k_tiles);
-    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[3], Xs, x_tiles * k_tiles);
-    if (rc != NEOGEMM_OK) return rc;
-  }
   GroupedParams p;
   std::memset(&p, 0, sizeof(p));
   p.offsets = offsets;
@@ -266,11 +280,20 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
   p.rows = static_cast<int>(T);
   p.lanes = static_cast<int>(N);
   p.depth = static_cast<int>(K);
-  const int64_t lane_tiles = ceil_div(N, 128 * k.cta_group);
-  // Tiles keep to the grid of the columns, so a group may touch one more than its length says.
-  const int64_t tiles = lane_tiles * (std::min(groups, T) + T / k.columns + 1);
-  if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
-  p.lane_tiles = static_cast<int>(lane_tiles);
+  int64_t tiles;
+  rc = fill_rows(k, groups, T, N, &p, &tiles);
+  if (rc != NEOGEMM_OK) return rc;
+  CUtensorMap maps[5];   // lanes, lanes by units, columns, scales of both
+  std::memset(maps, 0, sizeof(maps));
+  if (K > 0) {
+    rc = encode_codes(dev, &maps[0], Wc, K, N, groups, k.lane_box);
+    if (rc == NEOGEMM_OK && k.stream)
+      rc = encode_codes(dev, &maps[1], Wc, K, N, groups, k.lane_step);
+    if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps[2], Xc, K, T, 1, p.col_box);
+    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[3], Ws, groups * w_tiles * k_tiles);
+    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[4], Xs, x_tiles * k_tiles);
+    if (rc != NEOGEMM_OK) return rc;
+  }
   p.zero_rest = zero_rest;
   p.vector_out = ldy % 8 == 0 && aligned16(Y);
   p.out = static_cast<__nv_bfloat16*>(Y);
@@ -325,11 +348,11 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   const int forced = tuning_value(13);
   const bool wide = forced >= 0 ? forced != 0 : N >= 256 && K >= 256;
   const KernelEntry& k = kKernels[kGroupedDw][wide ? 1 : 0];
-  CUtensorMap maps[4];
+  CUtensorMap maps[5];   // lanes, lanes by units, columns, scales of both
   std::memset(maps, 0, sizeof(maps));
   if (T > 0) {
-    rc = encode_matrix(dev, &maps[0], dY, N, T, lddy, 64);
-    if (rc == NEOGEMM_OK) rc = encode_matrix(dev, &maps[1], X, K, T, ldx, 64);
+    rc = encode_bf16(dev, &maps[0], dY, N, T, 1, lddy, 0, 64);
+    if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps[2], X, K, T, 1, ldx, 0, 64);
     if (rc != NEOGEMM_OK) return rc;
   }
   GroupedParams p;
@@ -341,7 +364,7 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   p.lanes = static_cast<int>(N);
   p.cols = static_cast<int>(K);
   p.depth = static_cast<int>(T);
-  const int64_t lane_tiles = ceil_div(N, 128 * k.cta_group), col_tiles = ceil_div(K, k.columns);
+  const int64_t lane_tiles = ceil_div(N, k.lane_step), col_tiles = ceil_div(K, k.columns);
   const int64_t tiles = groups * lane_tiles * col_tiles;
   if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
   p.lane_tiles = static_cast<int>(lane_tiles);

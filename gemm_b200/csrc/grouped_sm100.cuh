@@ -47,7 +47,10 @@ struct GroupedParams {
   int lanes;                // extent of the axis on the tensor-memory lanes (N; K for dx)
   int cols;                 // kGroupedDw: extent of the column axis (K)
   int depth;                // contraction length (K; N for dx; for dW the rows of the batch)
-  int lane_tiles;           // tiles along `lanes`
+  int lane_tiles;           // tiles along `lanes` (streaming kernels: units of kUnit)
+  int col_cap;              // widest accumulator of a tile (a multiple of the column granularity)
+  int col_box;              // rows of the ragged operand's boxes
+  int slot_bytes, slots;    // streaming kernels: the ring
   int col_tiles;            // kGroupedDw: tiles along `cols`
   int zero_rest;            // write zeros to the rows of no group (0: leave them)
   int vector_out;           // 16-byte stores are possible (alignment of base and pitches)
@@ -59,34 +62,56 @@ struct GroupedParams {
   int* status;
 };
 
+// kCtaGroup == 2: tiles of 256 lanes x up to kCols columns on CTA pairs, for groups of many rows.
+//
+// kCtaGroup == 1 (but for dW): the streaming kernels, for groups of few rows, where the time is
+// that of reading the matrices once.  The lane axes of all groups are laid end to end in units of
+// kUnit rows and every CTA takes an equal run of units, cut into tiles of at most 128 lanes; so all
+// SMs read the same number of bytes whatever the number of chosen groups (with tiles of 128
+// lanes, 6 groups of 3584 rows are 168 tiles: two rounds on 148 SMs for 1.14 rounds of work).
+// A tile of fewer lanes still issues 128-lane MMAs - the tensor pipe idles here - and reads
+// whatever follows in shared memory; those accumulator lanes are never stored.  A load takes about
+// 3 us to land under load, so the rate of an SM is its bytes in flight over that time: a ring slot
+// takes as many k-blocks of the tile as fit, so that tiles of few lanes fill it too.
 template <int kOp_, int kCtaGroup_, int kCols_, int kStages_>
 struct GroupedConfig {
   static constexpr int kOp = kOp_;
   static constexpr int kCtaGroup = kCtaGroup_;
   static constexpr int kCols = kCols_;              // widest accumulator (UMMA N) of a tile
-  static constexpr int kStages = kStages_;
+  static constexpr int kStages = kStages_;          // ring slots (streaming: at most)
+  static constexpr bool kStream = kCtaGroup == 1 && kOp != kGroupedDw;
+  static constexpr int kUnit = (kOp == kGroupedDx) ? 64 : 32;
   static constexpr int kLaneRows = 128;             // lanes per CTA
   static constexpr int kLaneTile = kLaneRows * kCtaGroup;
   static constexpr int kHalfCols = kCols / kCtaGroup;   // column rows a CTA fetches at most
   static constexpr int kBlockK = (kOp == kMxNt) ? 256 : 64;   // values of K per 128-byte row
   static constexpr int kStepK = (kOp == kMxNt) ? 64 : 16;     // values of K per MMA
   static constexpr int kColStep = 16 * kCtaGroup;   // granularity of a tile's N
-  static constexpr int kBoxRows = 32;               // rows of a box of the ragged operand
   // Shared memory of one ring slot.
   static constexpr int kLaneBytes = kLaneRows * 128;
   static constexpr int kColBytes = kHalfCols * 128;
-  static constexpr int kScaleCols = (kCols + 127) / 128;      // 128-row scale blocks of the columns
+  // MXFP4: the instruction takes the scales of 128 rows from four columns of tensor memory that
+  // start at a multiple of four, so lanes and columns keep to frames of 128 rows (kCols for the
+  // columns), the blocks in which the scales are stored.  A tile uses a part of its frame: rows
+  // outside are not fetched and their lanes or columns are not stored.
+  static constexpr int kScaleCols = (kCols + 127) / 128;      // blocks of scales of the columns
   static constexpr int kScaleBytes = (kOp == kMxNt) ? 1024 * (1 + kScaleCols) : 0;
   static constexpr int kStageBytes = kLaneBytes + kColBytes + kScaleBytes;
   static constexpr int kEpiBytes = 4 * 2 * 2048;    // per epilogue warp two buffers of 32 x 32 bf16
   static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
   static constexpr int kBarrierBytes = (3 * kStages + 4) * 8 + 16;
-  static constexpr int kSmemBytes =
-      kStages * kStageBytes + kEpiBytes + kTableBytes + 12 + kBarrierBytes + 1024;
-  // Two accumulators, and behind them (MXFP4) the scales of every ring slot: per 128 values of K
-  // four columns per 128 rows.
+  static constexpr int kRestBytes = kEpiBytes + kTableBytes + 12 + kBarrierBytes + 1024;
+  // The epilogue's buffers lie in front of the ring: an MMA of a tile that starts inside its frame
+  // reads from the frame's start, up to 12 KB in front of its slot.
+  static constexpr int kRingBytes = kStream ? (232448 - kRestBytes) / 1024 * 1024 : kStages * kStageBytes;
+  static_assert(kOp != kMxNt || !kStream || kEpiBytes >= 96 * 128, "room in front of the ring");
+  static_assert(kEpiBytes % 1024 == 0, "the ring starts on the swizzle's alignment");
+  static constexpr int kSmemBytes = kRingBytes + kRestBytes;
+  // Two accumulators, and behind them (MXFP4) the scales of every k-block in the ring: per 128
+  // values of K four columns per 128 rows.
   static constexpr int kScaleTmemCols = (kOp == kMxNt) ? 8 * (1 + kScaleCols) : 0;
-  static constexpr int kTmemNeeded = 2 * kCols + kStages * kScaleTmemCols;
+  static constexpr int kScaleSets = (kOp != kMxNt) ? 0 : kStream ? (512 - 2 * kCols) / kScaleTmemCols : kStages;
+  static constexpr int kTmemNeeded = 2 * kCols + kScaleSets * kScaleTmemCols;
   static constexpr int kTmemCols = (kCtaGroup == 2) ? 512 : kTmemNeeded <= 128 ? 128
                                  : kTmemNeeded <= 256 ? 256 : 512;
   static constexpr int kThreads = (kOp == kGroupedDw) ? 224 : 192;
@@ -97,13 +122,16 @@ struct GroupedConfig {
   static_assert(kSmemBytes <= 232448, "exceeds 227 KB of shared memory per CTA");
   static_assert(kSmemBytes > 116224, "one CTA per SM: tensor memory is not shared");
   static_assert(kTmemNeeded <= 512, "tensor memory");
-  static_assert(kCols % 32 == 0 && kCols <= 256 && kHalfCols % kBoxRows == 0, "columns");
+  static_assert(kCols % 32 == 0 && kCols <= 256 && kHalfCols % 32 == 0, "columns");
+  static_assert(kRingBytes >= 2 * kStageBytes, "two full blocks");
 };
 
 // What a tile computes.  Every role derives it from the tile's number.
 struct GroupedTile {
   int group;
-  int lane0;      // first index on the lanes
+  int lane0;      // index on lane 0 of the tile
+  int lane_lo;    // first lane in use (streaming MXFP4: a multiple of kUnit; else 0)
+  int lane_rows;  // lanes in use per CTA (streaming: a multiple of kUnit)
   int col_row;    // row of the ragged operand (index of the column axis for dW) in column 0
   int lo, hi;     // columns that are this tile's to store
   int mma_n;      // columns computed: hi rounded up
@@ -123,93 +151,186 @@ __device__ __forceinline__ void report_error(int* status, volatile int* abort_fl
   }
 }
 
+// Tiles along the columns of a group.
 template <class Cfg>
-__device__ __forceinline__ int column_tiles(int begin, int end) {
-  if (Cfg::kOp == kMxNt)   // scale blocks are 128 rows: tiles keep to their grid
-    return end > begin ? (end - 1) / Cfg::kCols - begin / Cfg::kCols + 1 : 0;
-  return (end - begin + Cfg::kCols - 1) / Cfg::kCols;
+__device__ __forceinline__ int column_tiles(const GroupedParams& p, int begin, int end) {
+  if (end <= begin) return 0;
+  if (Cfg::kOp == kMxNt) return (end - 1) / Cfg::kCols - begin / Cfg::kCols + 1;
+  return (end - begin + p.col_cap - 1) / p.col_cap;
 }
 
+// The copy and matrix instructions take their operands from the warp's uniform registers: a value
+// that the compiler cannot prove uniform costs a transfer each time it is used.  One that came from
+// shared memory is made so once.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+__device__ __forceinline__ void make_uniform(GroupedTile& t) {
+  t.group = uniform(t.group);
+  t.lane0 = uniform(t.lane0);
+  t.lane_lo = uniform(t.lane_lo);
+  t.lane_rows = uniform(t.lane_rows);
+  t.col_row = uniform(t.col_row);
+  t.lo = uniform(t.lo);
+  t.hi = uniform(t.hi);
+  t.mma_n = uniform(t.mma_n);
+  t.k_row = uniform(t.k_row);
+  t.k_len = uniform(t.k_len);
+  t.blocks = uniform(t.blocks);
+}
+
+// The tiles of one worker, in order.  Every role walks its own copy.
 template <class Cfg>
-__device__ __forceinline__ GroupedTile find_tile(const GroupedParams& p, int tile, const int* begin,
-                                                 const int* end, const int* first_tile) {
-  GroupedTile t;
-  if (Cfg::kOp == kGroupedDw) {
-    const int per_group = p.lane_tiles * p.col_tiles;
-    t.group = tile / per_group;
-    const int local = tile - t.group * per_group;
-    const int lane_tile = local / p.col_tiles;
-    t.lane0 = lane_tile * Cfg::kLaneTile;
-    t.col_row = (local - lane_tile * p.col_tiles) * Cfg::kCols;
-    t.lo = 0;
-    t.hi = min(Cfg::kCols, p.cols - t.col_row);
-    t.k_row = begin[t.group];
-    t.k_len = end[t.group] - t.k_row;
-  } else {
-    // Last group whose first tile is not behind this one: groups without tiles share their
-    // first tile with the next group and lose the comparison.
-    int a = 0, b = p.groups - 1;
-    while (a < b) {
-      const int m = (a + b + 1) >> 1;
-      if (first_tile[m] <= tile) a = m; else b = m - 1;
-    }
-    t.group = a;
-    const int g0 = begin[a], g1 = end[a];
-    const int tiles = column_tiles<Cfg>(g0, g1);
-    const int local = tile - first_tile[a];
-    const int lane_tile = local / tiles;
-    const int c = local - lane_tile * tiles;
-    t.lane0 = lane_tile * Cfg::kLaneTile;
-    if (Cfg::kOp == kMxNt) {
-      t.col_row = (g0 / Cfg::kCols + c) * Cfg::kCols;
-      t.lo = max(g0 - t.col_row, 0);
-      t.hi = min(g1 - t.col_row, Cfg::kCols);
+struct GroupedTiles {
+  const int *begin, *end, *first;   // row ranges; first tile (streaming: first unit) of a group
+  int next, last, step;
+
+  __device__ __forceinline__ GroupedTiles(const GroupedParams& p, const int* begin_, const int* end_,
+                                          const int* first_, int worker, int workers)
+      : begin(begin_), end(end_), first(first_) {
+    if (Cfg::kStream) {
+      const long long units = first[p.groups];
+      next = static_cast<int>(units * worker / workers);
+      last = static_cast<int>(units * (worker + 1) / workers);
+      step = 0;
     } else {
-      // Equal shares, in steps of the MMA's column granularity.
-      const int share = ((g1 - g0 + tiles - 1) / tiles + Cfg::kColStep - 1) / Cfg::kColStep *
-                        Cfg::kColStep;
-      t.col_row = g0 + c * share;
-      t.lo = 0;
-      t.hi = max(min(share, g1 - t.col_row), 0);
+      next = worker;
+      last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : first[p.groups];
+      step = workers;
     }
-    t.k_row = 0;
-    t.k_len = p.depth;
   }
-  t.mma_n = max((t.hi + Cfg::kColStep - 1) / Cfg::kColStep, 1) * Cfg::kColStep;
-  t.blocks = (t.k_len + Cfg::kBlockK - 1) / Cfg::kBlockK;
-  return t;
-}
 
-// Boxes of the column operand that CTA `rank` fetches: rows [first, first + count) of boxes, in
-// units of kBoxRows rows from the start of its half.  Rows nobody stores are not fetched.
+  __device__ __forceinline__ bool take(const GroupedParams& p, GroupedTile& t) {
+    if (next >= last) return false;
+    if (Cfg::kOp == kGroupedDw) {
+      const int per_group = p.lane_tiles * p.col_tiles;
+      t.group = next / per_group;
+      const int local = next - t.group * per_group;
+      const int lane_tile = local / p.col_tiles;
+      t.lane0 = lane_tile * Cfg::kLaneTile;
+      t.lane_lo = 0;
+      t.lane_rows = Cfg::kLaneRows;
+      t.col_row = (local - lane_tile * p.col_tiles) * Cfg::kCols;
+      t.lo = 0;
+      t.hi = min(Cfg::kCols, p.cols - t.col_row);
+      t.k_row = begin[t.group];
+      t.k_len = end[t.group] - t.k_row;
+      next += step;
+    } else {
+      // Last group whose first tile is not behind this one: groups without tiles share their
+      // first tile with the next group and lose the comparison.
+      int a = 0, b = p.groups - 1;
+      while (a < b) {
+        const int m = (a + b + 1) >> 1;
+        if (first[m] <= next) a = m; else b = m - 1;
+      }
+      t.group = a;
+      const int g0 = begin[a], g1 = end[a];
+      const int tiles = column_tiles<Cfg>(p, g0, g1);
+      const int local = next - first[a];
+      int c;
+      if (Cfg::kStream) {
+        // A run of units along one lane axis, in equal tiles (MXFP4: by frames).
+        c = local / p.lane_tiles;
+        const int unit = local - c * p.lane_tiles;
+        const int run = min(last - next, p.lane_tiles - unit);
+        constexpr int kMost = Cfg::kLaneRows / Cfg::kUnit;
+        int units;
+        if (Cfg::kOp == kMxNt) {
+          t.lane_lo = unit % kMost * Cfg::kUnit;
+          units = min(run, kMost - unit % kMost);
+        } else {
+          const int cuts = (run + kMost - 1) / kMost;
+          t.lane_lo = 0;
+          units = (run + cuts - 1) / cuts;
+        }
+        t.lane0 = unit * Cfg::kUnit - t.lane_lo;
+        t.lane_rows = units * Cfg::kUnit;
+        next += units;
+      } else {
+        const int lane_tile = local / tiles;
+        c = local - lane_tile * tiles;
+        t.lane0 = lane_tile * Cfg::kLaneTile;
+        t.lane_lo = 0;
+        t.lane_rows = Cfg::kLaneRows;
+        next += step;
+      }
+      if (Cfg::kOp == kMxNt) {
+        t.col_row = (g0 / Cfg::kCols + c) * Cfg::kCols;
+        t.lo = max(g0 - t.col_row, 0);
+        t.hi = min(g1 - t.col_row, Cfg::kCols);
+      } else {
+        // Equal shares of the columns, in steps of the MMA's granularity.
+        const int share = ((g1 - g0 + tiles - 1) / tiles + Cfg::kColStep - 1) / Cfg::kColStep *
+                          Cfg::kColStep;
+        t.col_row = g0 + c * share;
+        t.lo = 0;
+        t.hi = max(min(share, g1 - t.col_row), 0);
+      }
+      t.k_row = 0;
+      t.k_len = p.depth;
+    }
+    t.mma_n = max((t.hi + Cfg::kColStep - 1) / Cfg::kColStep, 1) * Cfg::kColStep;
+    t.blocks = (t.k_len + Cfg::kBlockK - 1) / Cfg::kBlockK;
+    return true;
+  }
+};
+
+// Boxes of the column operand that CTA `rank` fetches, counted from the start of its half.  Rows
+// nobody stores are not fetched.
 template <class Cfg>
-__device__ __forceinline__ void column_boxes(const GroupedTile& t, int rank, int* first, int* count) {
+__device__ __forceinline__ void column_boxes(const GroupedParams& p, const GroupedTile& t, int rank,
+                                             int* first, int* count) {
   const int half = t.mma_n / Cfg::kCtaGroup;
   const int lo = max(t.lo - rank * half, 0), hi = min(t.hi - rank * half, half);
-  *first = lo / Cfg::kBoxRows;
-  *count = hi > lo ? (hi - 1) / Cfg::kBoxRows - *first + 1 : 0;
+  *first = lo / p.col_box;
+  *count = hi > lo ? (hi - 1) / p.col_box - *first + 1 : 0;
 }
+
+// Where the parts of a k-block lie from its start (lanes, columns, scales), and how many k-blocks a
+// ring slot takes.
+template <class Cfg>
+struct BlockLayout {
+  int first_box, boxes;   // of the columns (not for dW)
+  uint32_t lane_bytes, col_bytes, size;
+  int per_slot;
+
+  __device__ __forceinline__ BlockLayout(const GroupedParams& p, const GroupedTile& t, int rank)
+      : first_box(0), boxes(0), lane_bytes(Cfg::kLaneBytes), col_bytes(Cfg::kColBytes), per_slot(1) {
+    if (Cfg::kOp != kGroupedDw) column_boxes<Cfg>(p, t, rank, &first_box, &boxes);
+    if (Cfg::kStream) {   // what is in use; columns keep their places up to the last one
+      lane_bytes = static_cast<uint32_t>(t.lane_rows) * 128;
+      col_bytes = static_cast<uint32_t>((first_box + boxes) * p.col_box) * 128;
+    }
+    size = lane_bytes + col_bytes + Cfg::kScaleBytes;
+    if (Cfg::kStream) {
+      per_slot = p.slot_bytes / static_cast<int>(size);
+      if (Cfg::kOp == kMxNt) per_slot = min(per_slot, Cfg::kScaleSets / p.slots);
+    }
+  }
+};
 
 // Bytes CTA `rank` fetches per k-block.
 template <class Cfg>
-__device__ __forceinline__ uint32_t block_bytes(const GroupedTile& t, int rank) {
-  uint32_t bytes = Cfg::kLaneBytes + Cfg::kScaleBytes;
+__device__ __forceinline__ uint32_t block_bytes(const GroupedParams& p, const GroupedTile& t, int rank) {
+  uint32_t bytes = static_cast<uint32_t>(t.lane_rows) * 128 + Cfg::kScaleBytes;
   if (Cfg::kOp == kGroupedDw) {
     bytes += (t.mma_n / Cfg::kCtaGroup + 63) / 64 * 8192;
   } else {
     int first, count;
-    column_boxes<Cfg>(t, rank, &first, &count);
-    bytes += static_cast<uint32_t>(count) * (Cfg::kBoxRows * 128);
+    column_boxes<Cfg>(p, t, rank, &first, &count);
+    bytes += static_cast<uint32_t>(count * p.col_box) * 128;
   }
   return bytes;
 }
 
-// tmap_l: the operand on the lanes; tmap_c: the one on the columns; tmap_sl, tmap_sc: their scales
+// tmap_l: the operand on the lanes; tmap_u: the same in boxes of one unit (streaming kernels; a
+// tile of 128 lanes is fetched as one box: boxes of 16 rows, eight to a tile, took 1.4 times as long
+// on 32 groups of 3584 x 2048); tmap_c: the operand on the columns; tmap_sl, tmap_sc: their scales
 // (kMxNt).
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1)
-grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant__ CUtensorMap tmap_c,
-               const __grid_constant__ CUtensorMap tmap_sl,
+grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant__ CUtensorMap tmap_u,
+               const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ CUtensorMap tmap_sl,
                const __grid_constant__ CUtensorMap tmap_sc, const GroupedParams p) {
   using namespace ptx;
   constexpr int kCtaGroup = Cfg::kCtaGroup;
@@ -220,9 +341,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-  const uint32_t ring = smem_base;
-  const uint32_t epi_base = ring + kStages * Cfg::kStageBytes;
-  const uint32_t bar_base = epi_base + Cfg::kEpiBytes;
+  const uint32_t epi_base = smem_base;
+  const uint32_t ring = epi_base + Cfg::kEpiBytes;
+  const uint32_t bar_base = ring + Cfg::kRingBytes;
   const uint32_t full_bar = bar_base;                        // [kStages]
   const uint32_t empty_bar = full_bar + 8 * kStages;         // [kStages]
   const uint32_t clear_bar = empty_bar + 8 * kStages;        // [kStages] dW: last block has landed
@@ -259,6 +380,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
   }
   if (warp == 0 && lane == 0 && p.depth > 0) {   // without a contraction there are no maps
     prefetch_tensormap(&tmap_l);
+    if (Cfg::kStream && Cfg::kOp != kGroupedDx) prefetch_tensormap(&tmap_u);
     prefetch_tensormap(&tmap_c);
     if (kMx) {
       prefetch_tensormap(&tmap_sl);
@@ -307,7 +429,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     int sum = 0;
     for (int base = 0; base < p.groups; base += 32) {
       const int e = base + static_cast<int>(lane);
-      const int mine = e < p.groups ? column_tiles<Cfg>(begin[e], end[e]) * p.lane_tiles : 0;
+      const int mine = e < p.groups ? column_tiles<Cfg>(p, begin[e], end[e]) * p.lane_tiles : 0;
       int scan = mine;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -320,7 +442,11 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     if (lane == 0) first_tile[p.groups] = sum;
   }
   __syncthreads();
-  const int num_tiles = kDw ? p.groups * p.lane_tiles * p.col_tiles : first_tile[p.groups];
+  GroupedTiles<Cfg> tiles(p, begin, end, first_tile, worker, num_workers);
+  GroupedTile t;
+  int tile = 0;   // of this worker, for error records
+  const uint32_t slot_bytes = Cfg::kStream ? p.slot_bytes : Cfg::kStageBytes;
+  const uint32_t slots = Cfg::kStream ? p.slots : kStages;
 
   // ---------------------------------------------------------------- roles
   if (*abort_flag != 0) {
@@ -330,81 +456,79 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     uint32_t stage = 0, phase = 0;
     const uint32_t leader_full = (kCtaGroup == 2) ? mapa_u32(full_bar, 0) : full_bar;
     bool ok = true;
-    for (int tile = worker; ok && tile < num_tiles; tile += num_workers) {
-      const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
-      const uint32_t mine = block_bytes<Cfg>(t, rank);
-      const uint32_t both = mine + (kCtaGroup == 2 ? block_bytes<Cfg>(t, 1 - rank) : 0u);
-      int first_box = 0, boxes = 0;
-      if (!kDw) column_boxes<Cfg>(t, rank, &first_box, &boxes);
+    for (; ok && tiles.take(p, t); ++tile) {
+      make_uniform(t);
+      const uint32_t mine = block_bytes<Cfg>(p, t, rank);
+      const uint32_t both = mine + (kCtaGroup == 2 ? block_bytes<Cfg>(p, t, 1 - rank) : 0u);
+      const BlockLayout<Cfg> at(p, t, rank);
       const int half = t.mma_n / kCtaGroup;
-      const int lane_row = t.lane0 + rank * Cfg::kLaneRows;
-      for (int kb = 0; kb < t.blocks; ++kb) {
-        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, abort_flag))) {
+      const int lane_row = t.lane0 + rank * Cfg::kLaneRows + t.lane_lo;
+      const int col_row = t.col_row + rank * half;
+      const bool whole = !Cfg::kStream || t.lane_rows == Cfg::kLaneRows;
+      for (int kb0 = 0; kb0 < t.blocks; kb0 += at.per_slot) {
+        ok = __all_sync(0xffffffffu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, abort_flag));
+        if (!ok) {
           if (lane == 0)
             report_error(p.status, abort_flag, kDevTimeoutProducer, tile, static_cast<int>(stage));
-          ok = false;
           break;
         }
-        const uint32_t sl = ring + stage * Cfg::kStageBytes;
-        const uint32_t sc = sl + Cfg::kLaneBytes;
+        const int blocks = Cfg::kStream ? min(at.per_slot, t.blocks - kb0) : 1;
+        uint32_t sl = ring + stage * slot_bytes;
+        // dW: the last block of a group's rows is handed over by the warp that clears its tail.
+        const bool clear = kDw && t.k_len - kb0 * 64 < 64;
+        const uint32_t own = (clear ? clear_bar : full_bar) + 8 * stage;
+        const uint32_t bar = (kCtaGroup == 1 || clear) ? own : leader_full + 8 * stage;
+        auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+          if (kCtaGroup == 1 || clear) tma_load_3d(dst, map, bar, c0, c1, c2);
+          else tma_load_3d_pair(dst, map, bar, c0, c1, c2);
+        };
         if (elect_one()) {
-          const int k0 = kb * 64;   // first element of the block (byte pairs for MXFP4: 128 bytes)
-          const uint32_t bar = leader_full + 8 * stage;
-          if constexpr (kDw) {
-            // Both operands run along the rows of the batch.
-            const bool clear = t.k_len - k0 < 64;
-            const uint32_t own = clear ? clear_bar + 8 * stage : full_bar + 8 * stage;
-            if (clear) {
-              mbar_arrive_expect_tx(own, mine);
-            } else if (is_leader) {
-              mbar_arrive_expect_tx(own, both);
-              if (kCtaGroup == 2) mbar_arrive(own);
-            }
-            const int row = t.k_row + k0;
-            const int col = t.col_row + rank * half;
-            const int col_boxes = (half + 63) / 64;
-            auto load = [&](uint32_t dst, const CUtensorMap* map, int c0) {
-              if (kCtaGroup == 1 || clear) tma_load_2d(dst, map, own, c0, row);
-              else tma_load_2d_pair(dst, map, bar, c0, row);
-            };
-            load(sl, &tmap_l, lane_row);
-            load(sl + 8192, &tmap_l, lane_row + 64);
-            for (int b = 0; b < col_boxes; ++b) load(sc + b * 8192, &tmap_c, col + b * 64);
-          } else {
-            if (kCtaGroup == 1) mbar_arrive_expect_tx(bar, mine);
-            else if (is_leader) mbar_arrive_expect_tx(full_bar + 8 * stage, both);
-            auto load2 = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1) {
-              if (kCtaGroup == 1) tma_load_2d(dst, map, bar, c0, c1);
-              else tma_load_2d_pair(dst, map, bar, c0, c1);
-            };
-            auto load3 = [&](uint32_t dst, int c0, int c1) {
-              if (kCtaGroup == 1) tma_load_3d(dst, &tmap_l, bar, c0, c1, t.group);
-              else tma_load_3d_pair(dst, &tmap_l, bar, c0, c1, t.group);
-            };
-            if constexpr (Cfg::kOp == kGroupedDx) {
-              load3(sl, lane_row, k0);
-              load3(sl + 8192, lane_row + 64, k0);
+          if (kCtaGroup == 1 || clear) {
+            mbar_arrive_expect_tx(own, mine * blocks);
+          } else if (is_leader) {
+            mbar_arrive_expect_tx(own, both);
+            if (kDw) mbar_arrive(own);
+          }
+          for (int j = 0; j < blocks; ++j, sl += at.size) {
+            const int kb = kb0 + j;
+            const uint32_t sc = sl + at.lane_bytes;
+            const int k0 = kb * (kMx ? 128 : 64);   // first element (MXFP4: byte) of the block
+            if constexpr (kDw) {
+              load(sl, &tmap_l, lane_row, t.k_row + k0, 0);
+              load(sl + 8192, &tmap_l, lane_row + 64, t.k_row + k0, 0);
+#pragma unroll
+              for (int b = 0; b < Cfg::kHalfCols / 64; ++b)
+                if (b * 64 < half) load(sc + b * 8192, &tmap_c, col_row + b * 64, t.k_row + k0, 0);
             } else {
-              load3(sl, kMx ? kb * 128 : k0, lane_row);
-            }
-            const int row = t.col_row + rank * half;
-            for (int b = first_box; b < first_box + boxes; ++b)
-              load2(sc + b * (Cfg::kBoxRows * 128), &tmap_c, kMx ? kb * 128 : k0,
-                    row + b * Cfg::kBoxRows);
-            if constexpr (kMx) {
-              // Two consecutive 512-byte tiles of scales (128 rows x 128 values of K each); the
-              // second one of a short last block is some other tile or zero fill and not used.
-              const uint32_t ss = sc + Cfg::kColBytes;
-              load2(ss, &tmap_sl, 0,
-                    (t.group * p.sf_row_blocks + lane_row / 128) * p.sf_k_blocks + 2 * kb);
-              for (int b = 0; b < Cfg::kScaleCols; ++b)
-                load2(ss + 1024 * (1 + b), &tmap_sc, 0,
-                      (t.col_row / 128 + b) * p.sf_k_blocks + 2 * kb);
+              if constexpr (Cfg::kOp == kGroupedDx) {
+                load(sl, &tmap_l, lane_row, k0, t.group);
+                if (t.lane_rows > 64) load(sl + 8192, &tmap_l, lane_row + 64, k0, t.group);
+              } else if (whole) {
+                load(sl, &tmap_l, k0, lane_row, t.group);
+              } else {
+#pragma unroll
+                for (int u = 0; u < Cfg::kLaneRows - Cfg::kUnit; u += Cfg::kUnit)
+                  if (u < t.lane_rows) load(sl + u * 128, &tmap_u, k0, lane_row + u, t.group);
+              }
+#pragma unroll
+              for (int b = 0; b < Cfg::kHalfCols / 32; ++b)
+                if (b >= at.first_box && b < at.first_box + at.boxes)
+                  load(sc + b * (p.col_box * 128), &tmap_c, k0, col_row + b * p.col_box, 0);
+              if constexpr (kMx) {
+                // Two consecutive 512-byte tiles of scales (128 rows x 128 values of K each); the
+                // second one of a short last block is some other tile or zero fill and not used.
+                const uint32_t ss = sc + at.col_bytes;
+                load(ss, &tmap_sl, 0,
+                     (t.group * p.sf_row_blocks + lane_row / 128) * p.sf_k_blocks + 2 * kb, 0);
+#pragma unroll
+                for (int b = 0; b < Cfg::kScaleCols; ++b)
+                  load(ss + 1024 * (1 + b), &tmap_sc, 0, (t.col_row / 128 + b) * p.sf_k_blocks + 2 * kb, 0);
+              }
             }
           }
         }
         __syncwarp();
-        if (++stage == kStages) { stage = 0; phase ^= 1; }
+        if (++stage == slots) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -413,9 +537,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
       uint32_t stage = 0, phase = 0;
       int count = 0;   // tiles with a contraction so far: their accumulators alternate
       bool ok = true;
-      for (int tile = worker; ok && tile < num_tiles; tile += num_workers) {
-        const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
+      for (; ok && tiles.take(p, t); ++tile) {
         if (t.blocks == 0) continue;
+        make_uniform(t);
         const uint32_t acc = count & 1, acc_phase = (count >> 1) & 1;
         ++count;
         if (!__all_sync(0xffffffffu, mbar_wait<kCtaGroup == 2>(tmem_empty_bar + 8 * acc,
@@ -425,13 +549,14 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
           break;
         }
         tcgen05_fence_after();
+        const BlockLayout<Cfg> at(p, t, rank);
         const uint32_t tmem_d = tmem_base + acc * Cfg::kCols;
         const uint32_t idesc =
             kMx ? make_idesc_mxf4(Cfg::kLaneTile, static_cast<uint32_t>(t.mma_n))
                 : make_idesc_bf16(Cfg::kLaneTile, static_cast<uint32_t>(t.mma_n)) |
                       (Cfg::kOp == kGroupedDx ? kIdescTransposeA : 0u) |
                       (kDw ? kIdescTransposeA | kIdescTransposeB : 0u);
-        for (int kb = 0; kb < t.blocks; ++kb) {
+        for (int kb0 = 0; kb0 < t.blocks; kb0 += at.per_slot) {
           if (!__all_sync(0xffffffffu,
                           mbar_wait<kDw && kCtaGroup == 2>(full_bar + 8 * stage, phase, abort_flag))) {
             if (lane == 0)
@@ -440,46 +565,59 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
             break;
           }
           tcgen05_fence_after();
-          const uint32_t sl = ring + stage * Cfg::kStageBytes;
-          const uint32_t sc = sl + Cfg::kLaneBytes;
-          const int steps = min(4, (t.k_len - kb * Cfg::kBlockK + Cfg::kStepK - 1) / Cfg::kStepK);
+          const int blocks = Cfg::kStream ? min(at.per_slot, t.blocks - kb0) : 1;
+          uint32_t sl = ring + stage * slot_bytes;
           if (elect_one()) {
-            if constexpr (kMx) {
-              const uint32_t ss = sc + Cfg::kColBytes;
-              const uint32_t tsf = tmem_base + 2 * Cfg::kCols + stage * Cfg::kScaleTmemCols;
+            for (int j = 0; j < blocks; ++j, sl += at.size) {
+              const int kb = kb0 + j;
+              const uint32_t sc = sl + at.lane_bytes;
+              const int steps = min(4, (t.k_len - kb * Cfg::kBlockK + Cfg::kStepK - 1) / Cfg::kStepK);
+              if constexpr (kMx) {
+                // Scales of 128 values of K: four columns of tensor memory per block of 128 rows.
+                const uint32_t ss = sc + at.col_bytes;
+                const uint32_t set = Cfg::kStream ? stage * (Cfg::kScaleSets / slots) + j : stage;
+                const uint32_t tsl = tmem_base + 2 * Cfg::kCols + set * Cfg::kScaleTmemCols;
+                const uint32_t tsc = tsl + 8;
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {   // 128 values of K each
-                tmem_copy_32x128b_x4<kCtaGroup>(tsf + h * 4, make_smem_desc_scales(ss + h * 512));
+                for (int h = 0; h < 2; ++h) {
+                  tmem_copy_32x128b_x4<kCtaGroup>(tsl + h * 4, make_smem_desc_scales(ss + h * 512));
 #pragma unroll
-                for (int b = 0; b < Cfg::kScaleCols; ++b)
-                  tmem_copy_32x128b_x4<kCtaGroup>(
-                      tsf + 8 + (h * Cfg::kScaleCols + b) * 4,
-                      make_smem_desc_scales(ss + 1024 * (1 + b) + h * 512));
+                  for (int b = 0; b < Cfg::kScaleCols; ++b)
+                    tmem_copy_32x128b_x4<kCtaGroup>(
+                        tsc + (h * Cfg::kScaleCols + b) * 4,
+                        make_smem_desc_scales(ss + 1024 * (1 + b) + h * 512));
+                }
+                // Lane 0 of the frame lies in front of the tile's first fetched row.
+                const uint64_t dl = make_smem_desc_sw128(sl - t.lane_lo * 128);
+                const uint64_t dc = make_smem_desc_sw128(sc);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint32_t h = k >> 1;
+                  if (k < steps)
+                    umma_mxf4<kCtaGroup>(tmem_d, dl + 2 * k, dc + 2 * k,
+                                         idesc | idesc_scale_bytes((k & 1) * 2), tsl + h * 4,
+                                         tsc + h * Cfg::kScaleCols * 4, (kb > 0 || k > 0) ? 1u : 0u);
+                }
+              } else {
+                // A K-major operand moves 32 bytes along its swizzled rows per step of 16, an
+                // MN-major one two groups of eight rows.
+                constexpr uint64_t kLaneStep = (Cfg::kOp == kGroupedNt) ? 2 : 128;
+                constexpr uint64_t kColStepDesc = kDw ? 128 : 2;
+                const uint64_t dl = (Cfg::kOp == kGroupedNt) ? make_smem_desc_sw128(sl)
+                                                             : make_smem_desc_mn_sw128(sl, 8192);
+                const uint64_t dc = kDw ? make_smem_desc_mn_sw128(sc, 8192) : make_smem_desc_sw128(sc);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (k < steps)
+                    umma_bf16<kCtaGroup>(tmem_d, dl + kLaneStep * k, dc + kColStepDesc * k, idesc,
+                                         (kb > 0 || k > 0) ? 1u : 0u);
               }
-              const uint64_t dl = make_smem_desc_sw128(sl), dc = make_smem_desc_sw128(sc);
-              for (int k = 0; k < steps; ++k) {
-                const uint32_t h = k >> 1;
-                umma_mxf4<kCtaGroup>(tmem_d, dl + 2 * k, dc + 2 * k,
-                                     idesc | idesc_scale_bytes((k & 1) * 2), tsf + h * 4,
-                                     tsf + 8 + h * Cfg::kScaleCols * 4, (kb > 0 || k > 0) ? 1u : 0u);
-              }
-            } else {
-              // A K-major operand moves 32 bytes along its swizzled rows per step of 16, an
-              // MN-major one two groups of eight rows.
-              constexpr uint64_t kLaneStep = (Cfg::kOp == kGroupedNt) ? 2 : 128;
-              constexpr uint64_t kColStepDesc = kDw ? 128 : 2;
-              const uint64_t dl = (Cfg::kOp == kGroupedNt) ? make_smem_desc_sw128(sl)
-                                                           : make_smem_desc_mn_sw128(sl, 8192);
-              const uint64_t dc = kDw ? make_smem_desc_mn_sw128(sc, 8192) : make_smem_desc_sw128(sc);
-              for (int k = 0; k < steps; ++k)
-                umma_bf16<kCtaGroup>(tmem_d, dl + kLaneStep * k, dc + kColStepDesc * k, idesc,
-                                     (kb > 0 || k > 0) ? 1u : 0u);
             }
             if (kCtaGroup == 2) umma_commit_both_ctas(empty_bar + 8 * stage);
             else umma_commit<1>(empty_bar + 8 * stage);
           }
           __syncwarp();
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
+          if (++stage == slots) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
         if (elect_one()) {
@@ -496,8 +634,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     const uint32_t stage_buf = epi_base + quad * 4096;
     uint32_t buf = 0;
     int count = 0;
-    for (int tile = worker; tile < num_tiles; tile += num_workers) {
-      const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
+    for (; tiles.take(p, t); ++tile) {
       const uint32_t acc = count & 1, acc_phase = (count >> 1) & 1;
       if (t.blocks > 0) {
         ++count;
@@ -509,7 +646,9 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
         tcgen05_fence_after();
       }
       const int lane_first = t.lane0 + rank * Cfg::kLaneRows + quad * 32;   // of this warp
-      for (int c = t.lo & ~31; c < t.hi; c += 32) {
+      const int lane_end = min(p.lanes, t.lane0 + rank * Cfg::kLaneRows + t.lane_lo + t.lane_rows);
+      const bool in_use = lane_first < lane_end && quad * 32 + 32 > t.lane_lo;
+      for (int c = t.lo & ~31; c < t.hi && in_use; c += 32) {
         uint32_t r[32];
         if (t.blocks > 0) {
           tmem_ld_32x32b_x32(tmem_base + acc * Cfg::kCols + lane_base + c, r);
@@ -538,7 +677,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
             uint32_t v[4];
             ld_shared_v4(s + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4), v);
             const int n = lane_first + row, col = t.col_row + c + unit * 8;
-            if (n < p.lanes && c + unit * 8 < t.hi) {
+            if (n < lane_end && c + unit * 8 < t.hi) {
               __nv_bfloat16* dst = p.out + t.group * p.out_stack + n * p.out_pitch + col;
               if (p.vector_out && c + unit * 8 + 8 <= t.hi) {
                 *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -568,13 +707,13 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
             uint32_t v[4];
             ld_shared_v4(s + row * 64 + unit * 16, v);
             const int col = lane_first + unit * 8;
-            if (c + row >= t.lo && c + row < t.hi && col < p.lanes) {
+            if (c + row >= t.lo && c + row < t.hi && col < lane_end) {
               __nv_bfloat16* dst =
                   p.out + static_cast<long long>(t.col_row + c + row) * p.out_pitch + col;
-              if (p.vector_out && col + 8 <= p.lanes) {
+              if (p.vector_out && col + 8 <= lane_end) {
                 *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
               } else {
-                const int left = min(p.lanes - col, 8);
+                const int left = min(lane_end - col, 8);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                   if (j < left)
@@ -615,8 +754,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     // ======================= rows of the next group =======================
     uint32_t stage = 0, parities = 0;
     bool ok = true;
-    for (int tile = worker; ok && tile < num_tiles; tile += num_workers) {
-      const GroupedTile t = find_tile<Cfg>(p, tile, begin, end, first_tile);
+    for (; ok && tiles.take(p, t); ++tile) {
       if (t.blocks == 0) continue;
       const int valid = t.k_len - (t.blocks - 1) * 64;   // rows of the last block
       stage = (stage + t.blocks - 1) % kStages;
