@@ -54,13 +54,13 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // three dimensions, so that one copy instruction serves all of them.
 int encode(const DeviceView& dev, CUtensorMap* map, CUtensorMapDataType type, const void* base,
            int64_t inner, int64_t rows, int64_t stack, int64_t pitch, int64_t stack_pitch,
-           uint32_t box_inner, uint32_t box_rows, bool swizzle) {
+           uint32_t box_inner, uint32_t box_rows, bool swizzle, uint32_t box_stack = 1) {
   if (pitch % 16 != 0 || stack_pitch % 16 != 0 || pitch >= (1ll << 40) || stack_pitch >= (1ll << 40))
     return NEOGEMM_ERR_UNSUPPORTED;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(stack)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(stack_pitch)};
-  const cuuint32_t box[3] = {box_inner, box_rows, 1}, ones[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {box_inner, box_rows, box_stack}, ones[3] = {1, 1, 1};
   const CUresult r = dev.encode(
       map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
       CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
@@ -77,7 +77,7 @@ int encode_bf16(const DeviceView& dev, CUtensorMap* map, const void* base, int64
 }
 
 int launch(const DeviceView& dev, const KernelEntry& k, int64_t tiles_at_most,
-           const CUtensorMap (&maps)[5], const GroupedParams& params, cudaStream_t stream) {
+           const GroupedMaps& maps, const GroupedParams& params, cudaStream_t stream) {
   static std::mutex mu;
   static bool attr_done[kMaxDevices][4][2] = {};
   const int which = &k == &kKernels[k.op][1] ? 1 : 0;
@@ -116,9 +116,7 @@ int launch(const DeviceView& dev, const KernelEntry& k, int64_t tiles_at_most,
   }
   cfg.attrs = attr;
   cfg.numAttrs = nattr;
-  void* args[6] = {const_cast<CUtensorMap*>(&maps[0]), const_cast<CUtensorMap*>(&maps[1]),
-                   const_cast<CUtensorMap*>(&maps[2]), const_cast<CUtensorMap*>(&maps[3]),
-                   const_cast<CUtensorMap*>(&maps[4]), const_cast<GroupedParams*>(&params)};
+  void* args[2] = {const_cast<GroupedMaps*>(&maps), const_cast<GroupedParams*>(&params)};
   if (cudaLaunchKernelExC(&cfg, k.fn, args) != cudaSuccess) {
     cudaGetLastError();
     return NEOGEMM_ERR_LAUNCH;
@@ -166,18 +164,21 @@ int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, Gr
   // Tiles that keep to a grid of rows may touch one more than the group's length says.
   const int64_t tiles = lane_tiles * (2 * std::min(groups, T) + T / (k.op == kMxNt ? k.columns : cap));
   if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
+  *tiles_at_most = tiles;
+  p->lane_tiles = static_cast<int>(lane_tiles);
   p->col_cap = static_cast<int>(cap);
-  p->col_box = cap <= 16 ? 16 : 32;
+  // A CTA fetches its columns as one box: a small one where that covers them (tails of groups).
+  p->col_box = static_cast<int>(ceil_div(cap / k.cta_group, 16) * 16);
+  p->small_box = std::min(p->col_box, 32);
+  if (p->col_box > 32) p->col_box = static_cast<int>(ceil_div(p->col_box, 32) * 32);
   if (k.stream) {
-    // Slots of two full k-blocks where four of them fit: half the waits and copies of 256 bytes of
-    // a row in a row.  Behind the last slot an MMA reads up to one k-block's lanes.
-    const int block = 128 * 128 + p->col_box * static_cast<int>(ceil_div(cap, p->col_box)) * 128 + k.scale_bytes;
+    // Slots of two full k-blocks where four of them fit: half the waits.  Behind the last slot an
+    // MMA reads up to one k-block's lanes.
+    const int block = 128 * 128 + p->col_box * 128 + k.scale_bytes;
     const int room = k.ring_bytes - 128 * 128;
     p->slot_bytes = room / (2 * block) >= 4 ? 2 * block : block;
     p->slots = std::min(k.stages, room / p->slot_bytes);
   }
-  p->lane_tiles = static_cast<int>(lane_tiles);
-  *tiles_at_most = tiles;
   return NEOGEMM_OK;
 }
 
@@ -224,13 +225,17 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   int64_t tiles;
   rc = fill_rows(k, groups, T, lanes, &p, &tiles);
   if (rc != NEOGEMM_OK) return rc;
-  CUtensorMap maps[5];   // lanes, lanes by units, columns, scales of both
-  std::memset(maps, 0, sizeof(maps));
+  GroupedMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
   if (depth > 0) {
-    rc = encode_bf16(dev, &maps[0], W, K, N, groups, ldw, stack_w, k.lane_box);
-    if (rc == NEOGEMM_OK && k.stream)
-      rc = encode_bf16(dev, &maps[1], W, K, N, groups, ldw, stack_w, k.lane_step);
-    if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps[2], R, depth, T, 1, ldr, 0, p.col_box);
+    rc = encode_bf16(dev, &maps.lanes, W, K, N, groups, ldw, stack_w, k.lane_box);
+    if (rc == NEOGEMM_OK && k.stream && op == kGroupedNt) {
+      rc = encode_bf16(dev, &maps.two_units, W, K, N, groups, ldw, stack_w, 2 * k.lane_step);
+      if (rc == NEOGEMM_OK)
+        rc = encode_bf16(dev, &maps.unit, W, K, N, groups, ldw, stack_w, k.lane_step);
+    }
+    if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps.cols, R, depth, T, 1, ldr, 0, p.col_box);
+    if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps.small_cols, R, depth, T, 1, ldr, 0, p.small_box);
     if (rc != NEOGEMM_OK) return rc;
   }
   p.zero_rest = zero_rest;
@@ -241,9 +246,11 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   return launch(dev, k, tiles, maps, p, stream);
 }
 
-// Scale tiles as a matrix of 512-byte rows, read two at a time.
-int encode_scales(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t tiles) {
-  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, tiles, 1, 512, 512, 128, 2, false);
+// Scale tiles as a matrix of 512-byte rows, read two at a time, of one or more blocks of rows.
+int encode_scales(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t tiles,
+                  int64_t row_blocks, int box_blocks) {
+  return encode(dev, map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, tiles, row_blocks, 512,
+                512 * tiles, 128, 2, false, static_cast<uint32_t>(box_blocks));
 }
 
 int encode_codes(const DeviceView& dev, CUtensorMap* map, const void* base, int64_t K, int64_t rows,
@@ -283,15 +290,19 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
   int64_t tiles;
   rc = fill_rows(k, groups, T, N, &p, &tiles);
   if (rc != NEOGEMM_OK) return rc;
-  CUtensorMap maps[5];   // lanes, lanes by units, columns, scales of both
-  std::memset(maps, 0, sizeof(maps));
+  GroupedMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
   if (K > 0) {
-    rc = encode_codes(dev, &maps[0], Wc, K, N, groups, k.lane_box);
-    if (rc == NEOGEMM_OK && k.stream)
-      rc = encode_codes(dev, &maps[1], Wc, K, N, groups, k.lane_step);
-    if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps[2], Xc, K, T, 1, p.col_box);
-    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[3], Ws, groups * w_tiles * k_tiles);
-    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps[4], Xs, x_tiles * k_tiles);
+    rc = encode_codes(dev, &maps.lanes, Wc, K, N, groups, k.lane_box);
+    if (rc == NEOGEMM_OK && k.stream) {
+      rc = encode_codes(dev, &maps.two_units, Wc, K, N, groups, 2 * k.lane_step);
+      if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps.unit, Wc, K, N, groups, k.lane_step);
+    }
+    if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps.cols, Xc, K, T, 1, p.col_box);
+    if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps.small_cols, Xc, K, T, 1, p.small_box);
+    if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps.lane_scales, Ws, groups * w_tiles * k_tiles, 1, 1);
+    if (rc == NEOGEMM_OK)
+      rc = encode_scales(dev, &maps.col_scales, Xs, k_tiles, x_tiles, (k.columns + 127) / 128);
     if (rc != NEOGEMM_OK) return rc;
   }
   p.zero_rest = zero_rest;
@@ -348,11 +359,11 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   const int forced = tuning_value(13);
   const bool wide = forced >= 0 ? forced != 0 : N >= 256 && K >= 256;
   const KernelEntry& k = kKernels[kGroupedDw][wide ? 1 : 0];
-  CUtensorMap maps[5];   // lanes, lanes by units, columns, scales of both
-  std::memset(maps, 0, sizeof(maps));
+  GroupedMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
   if (T > 0) {
-    rc = encode_bf16(dev, &maps[0], dY, N, T, 1, lddy, 0, 64);
-    if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps[2], X, K, T, 1, ldx, 0, 64);
+    rc = encode_bf16(dev, &maps.lanes, dY, N, T, 1, lddy, 0, 64);
+    if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps.cols, X, K, T, 1, ldx, 0, 64);
     if (rc != NEOGEMM_OK) return rc;
   }
   GroupedParams p;

@@ -49,7 +49,8 @@ struct GroupedParams {
   int depth;                // contraction length (K; N for dx; for dW the rows of the batch)
   int lane_tiles;           // tiles along `lanes` (streaming kernels: units of kUnit)
   int col_cap;              // widest accumulator of a tile (a multiple of the column granularity)
-  int col_box;              // rows of the ragged operand's boxes
+  int col_box;              // rows of the ragged operand's large boxes (a CTA's share of col_cap)
+  int small_box;            // and of its small ones
   int slot_bytes, slots;    // streaming kernels: the ring
   int col_tiles;            // kGroupedDw: tiles along `cols`
   int zero_rest;            // write zeros to the rows of no group (0: leave them)
@@ -229,20 +230,18 @@ struct GroupedTiles {
       const int local = next - first[a];
       int c;
       if (Cfg::kStream) {
-        // A run of units along one lane axis, in equal tiles (MXFP4: by frames).
+        // A run of units along one lane axis, in tiles of 4, 2 or 1 units (one box each).
         c = local / p.lane_tiles;
         const int unit = local - c * p.lane_tiles;
         const int run = min(last - next, p.lane_tiles - unit);
         constexpr int kMost = Cfg::kLaneRows / Cfg::kUnit;
-        int units;
-        if (Cfg::kOp == kMxNt) {
+        int units = run;
+        t.lane_lo = 0;
+        if (Cfg::kOp == kMxNt) {   // inside its frame
           t.lane_lo = unit % kMost * Cfg::kUnit;
           units = min(run, kMost - unit % kMost);
-        } else {
-          const int cuts = (run + kMost - 1) / kMost;
-          t.lane_lo = 0;
-          units = (run + cuts - 1) / cuts;
         }
+        units = units >= kMost ? kMost : units >= 2 ? 2 : 1;
         t.lane0 = unit * Cfg::kUnit - t.lane_lo;
         t.lane_rows = units * Cfg::kUnit;
         next += units;
@@ -275,31 +274,36 @@ struct GroupedTiles {
   }
 };
 
-// Boxes of the column operand that CTA `rank` fetches, counted from the start of its half.  Rows
-// nobody stores are not fetched.
-template <class Cfg>
-__device__ __forceinline__ void column_boxes(const GroupedParams& p, const GroupedTile& t, int rank,
-                                             int* first, int* count) {
-  const int half = t.mma_n / Cfg::kCtaGroup;
-  const int lo = max(t.lo - rank * half, 0), hi = min(t.hi - rank * half, half);
-  *first = lo / p.col_box;
-  *count = hi > lo ? (hi - 1) / p.col_box - *first + 1 : 0;
-}
-
-// Where the parts of a k-block lie from its start (lanes, columns, scales), and how many k-blocks a
-// ring slot takes.
+// A k-block of a tile: where its parts lie from its start (lanes, columns, scales), which rows of the
+// ragged operand it fetches, and how many k-blocks a ring slot takes.
 template <class Cfg>
 struct BlockLayout {
-  int first_box, boxes;   // of the columns (not for dW)
+  bool small;             // the columns in use lie in one small box; otherwise a large one from column 0
+  int first_col;          // column of the box's first row
   uint32_t lane_bytes, col_bytes, size;
+  uint32_t fetched;       // bytes that arrive
   int per_slot;
 
-  __device__ __forceinline__ BlockLayout(const GroupedParams& p, const GroupedTile& t, int rank)
-      : first_box(0), boxes(0), lane_bytes(Cfg::kLaneBytes), col_bytes(Cfg::kColBytes), per_slot(1) {
-    if (Cfg::kOp != kGroupedDw) column_boxes<Cfg>(p, t, rank, &first_box, &boxes);
-    if (Cfg::kStream) {   // what is in use; columns keep their places up to the last one
-      lane_bytes = static_cast<uint32_t>(t.lane_rows) * 128;
-      col_bytes = static_cast<uint32_t>((first_box + boxes) * p.col_box) * 128;
+  __device__ __forceinline__ BlockLayout(const GroupedParams& p, const GroupedTile& t, int rank) {
+    lane_bytes = Cfg::kLaneBytes;
+    col_bytes = Cfg::kColBytes;
+    small = false;
+    first_col = 0;
+    per_slot = 1;
+    if (Cfg::kOp == kGroupedDw) {
+      fetched = Cfg::kLaneBytes + (t.mma_n / Cfg::kCtaGroup + 63) / 64 * 8192;
+    } else {
+      const int half = t.mma_n / Cfg::kCtaGroup;
+      const int lo = max(t.lo - rank * half, 0), hi = max(min(t.hi - rank * half, half), 1);
+      first_col = lo / p.small_box * p.small_box;
+      small = hi - first_col <= p.small_box;
+      if (!small) first_col = 0;
+      if (Cfg::kStream) {
+        lane_bytes = static_cast<uint32_t>(t.lane_rows) * 128;
+        col_bytes = static_cast<uint32_t>(small ? first_col + p.small_box : p.col_box) * 128;
+      }
+      fetched = lane_bytes + static_cast<uint32_t>(small ? p.small_box : p.col_box) * 128 +
+                Cfg::kScaleBytes;
     }
     size = lane_bytes + col_bytes + Cfg::kScaleBytes;
     if (Cfg::kStream) {
@@ -307,31 +311,27 @@ struct BlockLayout {
       if (Cfg::kOp == kMxNt) per_slot = min(per_slot, Cfg::kScaleSets / p.slots);
     }
   }
+
+  __device__ __forceinline__ void make_uniform() {
+    small = uniform(small) != 0;
+    first_col = uniform(first_col);
+    lane_bytes = uniform(lane_bytes);
+    col_bytes = uniform(col_bytes);
+    size = uniform(size);
+    fetched = uniform(fetched);
+    per_slot = uniform(per_slot);
+  }
 };
 
-// Bytes CTA `rank` fetches per k-block.
-template <class Cfg>
-__device__ __forceinline__ uint32_t block_bytes(const GroupedParams& p, const GroupedTile& t, int rank) {
-  uint32_t bytes = static_cast<uint32_t>(t.lane_rows) * 128 + Cfg::kScaleBytes;
-  if (Cfg::kOp == kGroupedDw) {
-    bytes += (t.mma_n / Cfg::kCtaGroup + 63) / 64 * 8192;
-  } else {
-    int first, count;
-    column_boxes<Cfg>(p, t, rank, &first, &count);
-    bytes += static_cast<uint32_t>(count * p.col_box) * 128;
-  }
-  return bytes;
-}
+// Tensor maps of the operands, by box: lanes by 128, two units and one unit of rows (MN-major lanes:
+// 64 x 64), columns by col_box and small_box rows, scales (MXFP4) of the lanes and of the columns.
+struct GroupedMaps {
+  CUtensorMap lanes, two_units, unit, cols, small_cols, lane_scales, col_scales;
+};
 
-// tmap_l: the operand on the lanes; tmap_u: the same in boxes of one unit (streaming kernels; a
-// tile of 128 lanes is fetched as one box: boxes of 16 rows, eight to a tile, took 1.4 times as long
-// on 32 groups of 3584 x 2048); tmap_c: the operand on the columns; tmap_sl, tmap_sc: their scales
-// (kMxNt).
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::kThreads, 1)
-grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant__ CUtensorMap tmap_u,
-               const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ CUtensorMap tmap_sl,
-               const __grid_constant__ CUtensorMap tmap_sc, const GroupedParams p) {
+grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) {
   using namespace ptx;
   constexpr int kCtaGroup = Cfg::kCtaGroup;
   constexpr int kStages = Cfg::kStages;
@@ -358,7 +358,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
-  const int rank = (kCtaGroup == 2) ? static_cast<int>(cluster_ctarank()) : 0;
+  const int rank = (kCtaGroup == 2) ? uniform(static_cast<int>(cluster_ctarank())) : 0;
   const bool is_leader = rank == 0;
   const int worker = static_cast<int>(blockIdx.x) / kCtaGroup;
   const int num_workers = static_cast<int>(gridDim.x) / kCtaGroup;
@@ -379,12 +379,16 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0 && p.depth > 0) {   // without a contraction there are no maps
-    prefetch_tensormap(&tmap_l);
-    if (Cfg::kStream && Cfg::kOp != kGroupedDx) prefetch_tensormap(&tmap_u);
-    prefetch_tensormap(&tmap_c);
+    prefetch_tensormap(&maps.lanes);
+    prefetch_tensormap(&maps.cols);
+    if (Cfg::kStream && Cfg::kUnit < 64) {
+      prefetch_tensormap(&maps.two_units);
+      prefetch_tensormap(&maps.unit);
+    }
+    if (!kDw) prefetch_tensormap(&maps.small_cols);
     if (kMx) {
-      prefetch_tensormap(&tmap_sl);
-      prefetch_tensormap(&tmap_sc);
+      prefetch_tensormap(&maps.lane_scales);
+      prefetch_tensormap(&maps.col_scales);
     }
   }
   if (warp == 1) {
@@ -458,13 +462,25 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     bool ok = true;
     for (; ok && tiles.take(p, t); ++tile) {
       make_uniform(t);
-      const uint32_t mine = block_bytes<Cfg>(p, t, rank);
-      const uint32_t both = mine + (kCtaGroup == 2 ? block_bytes<Cfg>(p, t, 1 - rank) : 0u);
-      const BlockLayout<Cfg> at(p, t, rank);
+      BlockLayout<Cfg> at(p, t, rank);
+      uint32_t expected = at.fetched;   // by the leader of a pair: for both CTAs
+      if (kCtaGroup == 2) expected += BlockLayout<Cfg>(p, t, 1 - rank).fetched;
+      expected = uniform(expected);
+      at.make_uniform();
       const int half = t.mma_n / kCtaGroup;
       const int lane_row = t.lane0 + rank * Cfg::kLaneRows + t.lane_lo;
-      const int col_row = t.col_row + rank * half;
-      const bool whole = !Cfg::kStream || t.lane_rows == Cfg::kLaneRows;
+      const int col_row = t.col_row + rank * half + at.first_col;
+      const CUtensorMap* map_l = &maps.lanes;
+      if (Cfg::kStream && Cfg::kUnit < 64 && t.lane_rows < Cfg::kLaneRows)
+        map_l = t.lane_rows == Cfg::kUnit ? &maps.unit : &maps.two_units;
+      const CUtensorMap* map_c = at.small ? &maps.small_cols : &maps.cols;
+      const uint32_t to_cols = at.lane_bytes + at.first_col * 128;
+      const uint32_t to_scales = at.lane_bytes + at.col_bytes;
+      int scale_row = 0, col_scale_row = 0;
+      if (kMx) {
+        scale_row = (t.group * p.sf_row_blocks + lane_row / 128) * p.sf_k_blocks;
+        col_scale_row = t.col_row / 128;
+      }
       for (int kb0 = 0; kb0 < t.blocks; kb0 += at.per_slot) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, abort_flag));
         if (!ok) {
@@ -478,56 +494,53 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
         const bool clear = kDw && t.k_len - kb0 * 64 < 64;
         const uint32_t own = (clear ? clear_bar : full_bar) + 8 * stage;
         const uint32_t bar = (kCtaGroup == 1 || clear) ? own : leader_full + 8 * stage;
-        auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
-          if (kCtaGroup == 1 || clear) tma_load_3d(dst, map, bar, c0, c1, c2);
-          else tma_load_3d_pair(dst, map, bar, c0, c1, c2);
-        };
         if (elect_one()) {
           if (kCtaGroup == 1 || clear) {
-            mbar_arrive_expect_tx(own, mine * blocks);
+            mbar_arrive_expect_tx(own, at.fetched * blocks);
           } else if (is_leader) {
-            mbar_arrive_expect_tx(own, both);
+            mbar_arrive_expect_tx(own, expected);
             if (kDw) mbar_arrive(own);
-          }
-          for (int j = 0; j < blocks; ++j, sl += at.size) {
-            const int kb = kb0 + j;
-            const uint32_t sc = sl + at.lane_bytes;
-            const int k0 = kb * (kMx ? 128 : 64);   // first element (MXFP4: byte) of the block
-            if constexpr (kDw) {
-              load(sl, &tmap_l, lane_row, t.k_row + k0, 0);
-              load(sl + 8192, &tmap_l, lane_row + 64, t.k_row + k0, 0);
-#pragma unroll
-              for (int b = 0; b < Cfg::kHalfCols / 64; ++b)
-                if (b * 64 < half) load(sc + b * 8192, &tmap_c, col_row + b * 64, t.k_row + k0, 0);
-            } else {
-              if constexpr (Cfg::kOp == kGroupedDx) {
-                load(sl, &tmap_l, lane_row, k0, t.group);
-                if (t.lane_rows > 64) load(sl + 8192, &tmap_l, lane_row + 64, k0, t.group);
-              } else if (whole) {
-                load(sl, &tmap_l, k0, lane_row, t.group);
-              } else {
-#pragma unroll
-                for (int u = 0; u < Cfg::kLaneRows - Cfg::kUnit; u += Cfg::kUnit)
-                  if (u < t.lane_rows) load(sl + u * 128, &tmap_u, k0, lane_row + u, t.group);
-              }
-#pragma unroll
-              for (int b = 0; b < Cfg::kHalfCols / 32; ++b)
-                if (b >= at.first_box && b < at.first_box + at.boxes)
-                  load(sc + b * (p.col_box * 128), &tmap_c, k0, col_row + b * p.col_box, 0);
-              if constexpr (kMx) {
-                // Two consecutive 512-byte tiles of scales (128 rows x 128 values of K each); the
-                // second one of a short last block is some other tile or zero fill and not used.
-                const uint32_t ss = sc + at.col_bytes;
-                load(ss, &tmap_sl, 0,
-                     (t.group * p.sf_row_blocks + lane_row / 128) * p.sf_k_blocks + 2 * kb, 0);
-#pragma unroll
-                for (int b = 0; b < Cfg::kScaleCols; ++b)
-                  load(ss + 1024 * (1 + b), &tmap_sc, 0, (t.col_row / 128 + b) * p.sf_k_blocks + 2 * kb, 0);
-              }
-            }
           }
         }
         __syncwarp();
+        // Everything a copy needs is worked out outside the elected lane's branch, where the warp's
+        // uniform registers hold it: 17 cycles a copy, against about 95 inside.
+        for (int j = 0; j < blocks; ++j, sl += at.size) {
+          const int kb = kb0 + j;
+          const uint32_t sc = sl + to_cols, ss = sl + to_scales;
+          const int k0 = kb * (kMx ? 128 : 64);   // first element (MXFP4: byte) of the block
+          const int row = t.k_row + k0;
+          const int scales_l = scale_row + 2 * kb;
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2) {
+            if (kCtaGroup == 1 || clear) tma_load_3d(dst, map, bar, c0, c1, c2);
+            else tma_load_3d_pair(dst, map, bar, c0, c1, c2);
+          };
+          if (elect_one()) {
+            if constexpr (kDw) {
+              load(sl, &maps.lanes, lane_row, row, 0);
+              load(sl + 8192, &maps.lanes, lane_row + 64, row, 0);
+#pragma unroll
+              for (int b = 0; b < Cfg::kHalfCols / 64; ++b)
+                if (b * 64 < half) load(sc + b * 8192, &maps.cols, col_row + b * 64, row, 0);
+            } else {
+              if constexpr (Cfg::kOp == kGroupedDx) {
+                load(sl, &maps.lanes, lane_row, k0, t.group);
+                if (!Cfg::kStream || t.lane_rows > 64)
+                  load(sl + 8192, &maps.lanes, lane_row + 64, k0, t.group);
+              } else {
+                load(sl, map_l, k0, lane_row, t.group);
+              }
+              load(sc, map_c, k0, col_row, 0);
+              if constexpr (kMx) {
+                // Two consecutive 512-byte tiles of scales (128 rows x 128 values of K each) per
+                // block of rows; past the end of K they are other tiles or zero fill, and not used.
+                load(ss, &maps.lane_scales, 0, scales_l, 0);
+                load(ss + 1024, &maps.col_scales, 0, 2 * kb, col_scale_row);
+              }
+            }
+          }
+          __syncwarp();
+        }
         if (++stage == slots) { stage = 0; phase ^= 1; }
       }
     }
@@ -536,6 +549,7 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
     if (is_leader) {
       uint32_t stage = 0, phase = 0;
       int count = 0;   // tiles with a contraction so far: their accumulators alternate
+      const uint32_t sets_per_slot = Cfg::kScaleSets / slots;
       bool ok = true;
       for (; ok && tiles.take(p, t); ++tile) {
         if (t.blocks == 0) continue;
@@ -549,7 +563,8 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
           break;
         }
         tcgen05_fence_after();
-        const BlockLayout<Cfg> at(p, t, rank);
+        BlockLayout<Cfg> at(p, t, rank);
+        at.make_uniform();
         const uint32_t tmem_d = tmem_base + acc * Cfg::kCols;
         const uint32_t idesc =
             kMx ? make_idesc_mxf4(Cfg::kLaneTile, static_cast<uint32_t>(t.mma_n))
@@ -567,52 +582,53 @@ grouped_kernel(const __grid_constant__ CUtensorMap tmap_l, const __grid_constant
           tcgen05_fence_after();
           const int blocks = Cfg::kStream ? min(at.per_slot, t.blocks - kb0) : 1;
           uint32_t sl = ring + stage * slot_bytes;
-          if (elect_one()) {
-            for (int j = 0; j < blocks; ++j, sl += at.size) {
-              const int kb = kb0 + j;
-              const uint32_t sc = sl + at.lane_bytes;
-              const int steps = min(4, (t.k_len - kb * Cfg::kBlockK + Cfg::kStepK - 1) / Cfg::kStepK);
-              if constexpr (kMx) {
-                // Scales of 128 values of K: four columns of tensor memory per block of 128 rows.
-                const uint32_t ss = sc + at.col_bytes;
-                const uint32_t set = Cfg::kStream ? stage * (Cfg::kScaleSets / slots) + j : stage;
-                const uint32_t tsl = tmem_base + 2 * Cfg::kCols + set * Cfg::kScaleTmemCols;
-                const uint32_t tsc = tsl + 8;
+          for (int j = 0; j < blocks; ++j, sl += at.size) {
+            const int kb = kb0 + j;
+            const uint32_t sc = sl + at.lane_bytes;
+            // A K-major operand moves 32 bytes along its swizzled rows per step, an MN-major one two
+            // groups of eight rows.
+            constexpr uint64_t kLaneStep = (kDw || Cfg::kOp == kGroupedDx) ? 128 : 2;
+            constexpr uint64_t kColStepDesc = kDw ? 128 : 2;
+            // MXFP4: lane 0 of the frame lies in front of the tile's first fetched row.
+            const uint64_t dl = (kLaneStep == 128) ? make_smem_desc_mn_sw128(sl, 8192)
+                                                   : make_smem_desc_sw128(sl - t.lane_lo * 128);
+            const uint64_t dc = kDw ? make_smem_desc_mn_sw128(sc, 8192) : make_smem_desc_sw128(sc);
+            const int left = t.k_len - kb * Cfg::kBlockK;
+            const uint32_t first = kb > 0 ? 1u : 0u;
+            if constexpr (kMx) {
+              // Scales of 128 values of K: four columns of tensor memory per block of 128 rows.
+              const uint32_t set = Cfg::kStream ? stage * sets_per_slot + j : stage;
+              const uint32_t tsl = tmem_base + 2 * Cfg::kCols + set * Cfg::kScaleTmemCols;
+              const uint32_t tsc = tsl + 8;
+              const uint64_t ds = make_smem_desc_scales(sc + at.col_bytes);
+              if (elect_one()) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                  tmem_copy_32x128b_x4<kCtaGroup>(tsl + h * 4, make_smem_desc_scales(ss + h * 512));
+                  tmem_copy_32x128b_x4<kCtaGroup>(tsl + h * 4, ds + h * 32);
 #pragma unroll
                   for (int b = 0; b < Cfg::kScaleCols; ++b)
-                    tmem_copy_32x128b_x4<kCtaGroup>(
-                        tsc + (h * Cfg::kScaleCols + b) * 4,
-                        make_smem_desc_scales(ss + 1024 * (1 + b) + h * 512));
+                    tmem_copy_32x128b_x4<kCtaGroup>(tsc + (h * Cfg::kScaleCols + b) * 4,
+                                                    ds + 64 * (1 + b) + h * 32);
                 }
-                // Lane 0 of the frame lies in front of the tile's first fetched row.
-                const uint64_t dl = make_smem_desc_sw128(sl - t.lane_lo * 128);
-                const uint64_t dc = make_smem_desc_sw128(sc);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const uint32_t h = k >> 1;
-                  if (k < steps)
-                    umma_mxf4<kCtaGroup>(tmem_d, dl + 2 * k, dc + 2 * k,
-                                         idesc | idesc_scale_bytes((k & 1) * 2), tsl + h * 4,
-                                         tsc + h * Cfg::kScaleCols * 4, (kb > 0 || k > 0) ? 1u : 0u);
-                }
-              } else {
-                // A K-major operand moves 32 bytes along its swizzled rows per step of 16, an
-                // MN-major one two groups of eight rows.
-                constexpr uint64_t kLaneStep = (Cfg::kOp == kGroupedNt) ? 2 : 128;
-                constexpr uint64_t kColStepDesc = kDw ? 128 : 2;
-                const uint64_t dl = (Cfg::kOp == kGroupedNt) ? make_smem_desc_sw128(sl)
-                                                             : make_smem_desc_mn_sw128(sl, 8192);
-                const uint64_t dc = kDw ? make_smem_desc_mn_sw128(sc, 8192) : make_smem_desc_sw128(sc);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  if (k < steps)
+                  if (k * Cfg::kStepK < left)
+                    umma_mxf4<kCtaGroup>(tmem_d, dl + 2 * k, dc + 2 * k,
+                                         idesc | idesc_scale_bytes((k & 1) * 2), tsl + (k >> 1) * 4,
+                                         tsc + (k >> 1) * Cfg::kScaleCols * 4, k > 0 ? 1u : first);
+              }
+            } else {
+              if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (k * Cfg::kStepK < left)
                     umma_bf16<kCtaGroup>(tmem_d, dl + kLaneStep * k, dc + kColStepDesc * k, idesc,
-                                         (kb > 0 || k > 0) ? 1u : 0u);
+                                         k > 0 ? 1u : first);
               }
             }
+            __syncwarp();
+          }
+          if (elect_one()) {
             if (kCtaGroup == 2) umma_commit_both_ctas(empty_bar + 8 * stage);
             else umma_commit<1>(empty_bar + 8 * stage);
           }
