@@ -184,15 +184,14 @@ template <class Cfg>
 struct GroupedTiles {
   const int *begin, *end, *first;   // row ranges; first tile (streaming: first unit) of a group
   int next, last, step;
+  int worker, workers, units, round, height;   // streaming: all units; this round's start and tiles
 
   __device__ __forceinline__ GroupedTiles(const GroupedParams& p, const int* begin_, const int* end_,
-                                          const int* first_, int worker, int workers)
-      : begin(begin_), end(end_), first(first_) {
+                                          const int* first_, int worker_, int workers_)
+      : begin(begin_), end(end_), first(first_), worker(worker_), workers(workers_) {
     if (Cfg::kStream) {
-      const long long units = first[p.groups];
-      next = static_cast<int>(units * worker / workers);
-      last = static_cast<int>(units * (worker + 1) / workers);
-      step = 0;
+      units = first[p.groups];
+      round = height = next = last = 0;
     } else {
       next = worker;
       last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : first[p.groups];
@@ -201,6 +200,15 @@ struct GroupedTiles {
   }
 
   __device__ __forceinline__ bool take(const GroupedParams& p, GroupedTile& t) {
+    if (Cfg::kStream && next >= last) {
+      // The next round: every worker takes as many units, side by side.
+      round += height * workers;
+      const int left = units - round;
+      constexpr int kMost = Cfg::kLaneRows / Cfg::kUnit;
+      height = left >= kMost * workers ? kMost : left >= 2 * workers ? 2 : 1;
+      next = round + worker * height;
+      last = min(next + height, units);
+    }
     if (next >= last) return false;
     if (Cfg::kOp == kGroupedDw) {
       const int per_group = p.lane_tiles * p.col_tiles;
@@ -230,21 +238,21 @@ struct GroupedTiles {
       const int local = next - first[a];
       int c;
       if (Cfg::kStream) {
-        // A run of units along one lane axis, in tiles of 4, 2 or 1 units (one box each).
+        // Units along one lane axis, in tiles of 4, 2 or 1 of them (one box each).
         c = local / p.lane_tiles;
         const int unit = local - c * p.lane_tiles;
         const int run = min(last - next, p.lane_tiles - unit);
         constexpr int kMost = Cfg::kLaneRows / Cfg::kUnit;
-        int units = run;
+        int take = run;
         t.lane_lo = 0;
         if (Cfg::kOp == kMxNt) {   // inside its frame
           t.lane_lo = unit % kMost * Cfg::kUnit;
-          units = min(run, kMost - unit % kMost);
+          take = min(run, kMost - unit % kMost);
         }
-        units = units >= kMost ? kMost : units >= 2 ? 2 : 1;
+        take = take >= kMost ? kMost : take >= 2 ? 2 : 1;
         t.lane0 = unit * Cfg::kUnit - t.lane_lo;
-        t.lane_rows = units * Cfg::kUnit;
-        next += units;
+        t.lane_rows = take * Cfg::kUnit;
+        next += take;
       } else {
         const int lane_tile = local / tiles;
         c = local - lane_tile * tiles;
@@ -610,20 +618,31 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
                     tmem_copy_32x128b_x4<kCtaGroup>(tsc + (h * Cfg::kScaleCols + b) * 4,
                                                     ds + 64 * (1 + b) + h * 32);
                 }
+                // (A test per step between the instructions doubles the time of issuing them.)
+                auto step = [&](int k) {
+                  umma_mxf4<kCtaGroup>(tmem_d, dl + 2 * k, dc + 2 * k,
+                                       idesc | idesc_scale_bytes((k & 1) * 2), tsl + (k >> 1) * 4,
+                                       tsc + (k >> 1) * Cfg::kScaleCols * 4, k > 0 ? 1u : first);
+                };
+                if (left >= Cfg::kBlockK) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (k * Cfg::kStepK < left)
-                    umma_mxf4<kCtaGroup>(tmem_d, dl + 2 * k, dc + 2 * k,
-                                         idesc | idesc_scale_bytes((k & 1) * 2), tsl + (k >> 1) * 4,
-                                         tsc + (k >> 1) * Cfg::kScaleCols * 4, k > 0 ? 1u : first);
+                  for (int k = 0; k < 4; ++k) step(k);
+                } else {
+                  for (int k = 0; k * Cfg::kStepK < left; ++k) step(k);
+                }
               }
             } else {
               if (elect_one()) {
+                auto step = [&](int k) {
+                  umma_bf16<kCtaGroup>(tmem_d, dl + kLaneStep * k, dc + kColStepDesc * k, idesc,
+                                       k > 0 ? 1u : first);
+                };
+                if (left >= Cfg::kBlockK) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (k * Cfg::kStepK < left)
-                    umma_bf16<kCtaGroup>(tmem_d, dl + kLaneStep * k, dc + kColStepDesc * k, idesc,
-                                         k > 0 ? 1u : first);
+                  for (int k = 0; k < 4; ++k) step(k);
+                } else {
+                  for (int k = 0; k * Cfg::kStepK < left; ++k) step(k);
+                }
               }
             }
             __syncwarp();
