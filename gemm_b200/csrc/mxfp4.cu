@@ -1,9 +1,10 @@
 // Conversion between bf16 / fp32 and MXFP4 (format and contracts: include/neogemm.h).
 //
-// Both directions move each value once and are bound by HBM.  A lane owns 8 consecutive values (16
-// bytes of bf16), four lanes a block of 32; a warp covers 256 values of K in four rows that are 32
-// apart, because those are the rows whose scales are neighbours in the format: lane 0 of the first
-// and of the second 128 values each write their 16 bytes of scales as one word vector.
+// Both directions move each value once, which HBM bounds as long as the instructions per value are few
+// (straightforward code, about 15 per value, was bound by issue slots at 60 % of the bandwidth): bf16
+// stays packed in pairs through maximum and scaling, codes become bf16 by byte permutes of two
+// eight-entry tables.  A lane owns 8 consecutive values (16 bytes of bf16) and four lanes a block of
+// 32; a warp covers up to 1024 consecutive values of a row.
 #include "../../include/neogemm.h"
 
 #include <cuda_bf16.h>
@@ -17,8 +18,10 @@
 namespace neogemm {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRowsPerItem = 4;     // rows r, r + 32, r + 64, r + 96 of a block of 128
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kParts = 4;             // 256 values each
+constexpr int kSpan = 256 * kParts;   // values of a row that a warp covers
 
 struct ConvertParams {
   const void* x;
@@ -26,27 +29,24 @@ struct ConvertParams {
   unsigned char* scales;
   __nv_bfloat16* y;
   long long stack, rows, K, ldx, stack_x;
-  long long row_blocks, k_tiles, k_items;   // 128-row blocks, 128-value tiles, 256-value items
-  long long items;
+  long long row_blocks, k_tiles;   // 128-row blocks, 128-value tiles
+  unsigned spans;                  // warps per row
 };
 
-struct Item {
-  long long matrix, row_block, k0, row;     // row: r % 32 of the item's rows
-};
-
-__device__ __forceinline__ Item item_of(const ConvertParams& p, long long i) {
-  Item it;
-  it.k0 = (i % p.k_items) * 256;
-  i /= p.k_items;
-  it.row = i % 32;
-  i /= 32;
-  it.row_block = i % p.row_blocks;
-  it.matrix = i / p.row_blocks;
-  return it;
+// A warp's place: (row of the padded matrix, span of K); false past the end.
+__device__ __forceinline__ bool place(const ConvertParams& p, long long* row, long long* k) {
+  const unsigned warp = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const unsigned r = warp / p.spans;
+  *row = r;
+  *k = static_cast<long long>(warp - r * p.spans) * kSpan + (threadIdx.x & 31) * 8;
+  return r < p.row_blocks * 128;
 }
 
-__device__ __forceinline__ long long scale_tile(const ConvertParams& p, const Item& it) {
-  return ((it.matrix * p.row_blocks + it.row_block) * p.k_tiles + it.k0 / 128) * 512 + it.row * 16;
+// Byte of this lane's scale in the first 256 values of its span; 1024 bytes further per 256 values.
+__device__ __forceinline__ long long scale_at(const ConvertParams& p, long long matrix, long long row,
+                                              long long k0) {
+  return ((matrix * p.row_blocks + row / 128) * p.k_tiles + k0 / 128) * 512 + (row & 31) * 16 +
+         ((row >> 5) & 3) * 4 + ((threadIdx.x >> 2) & 3);
 }
 
 // Two fp32 to E2M1, nearest even, saturating: `lo` in the low four bits of the byte.
@@ -60,120 +60,131 @@ __device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi) {
   return out;
 }
 
+// Exponent of the largest magnitude (biased) to the block's biased scale exponent.
+__device__ __forceinline__ uint32_t scale_of(uint32_t e) { return e == 255 ? 255u : e > 2 ? e - 2 : 0u; }
+
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads) mxfp4_quantize_kernel(const ConvertParams p) {
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  const int lane = threadIdx.x & 31;
-  const long long warps = static_cast<long long>(gridDim.x) * (kThreads / 32);
-  for (long long i = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-       i < p.items; i += warps) {
-    const Item it = item_of(p, i);
-    const long long k = it.k0 + lane * 8;
-    const bool in_k = k < p.K;       // K is a multiple of 32: a block is inside or outside
-    float v[kRowsPerItem][8];
+  long long row, k0;
+  if (!place(p, &row, &k0)) return;
+  const bool in_rows = row < p.rows;
+  // Padding: the scales of rows past the last, and of blocks between K and the next 128.
+  const long long k_scales = p.k_tiles * 128;
+  for (long long m = blockIdx.y; m < p.stack; m += gridDim.y) {
+    const long long src = m * p.stack_x + row * p.ldx + k0;
+    uint32_t* codes = reinterpret_cast<uint32_t*>(p.codes + ((m * p.rows + row) * p.K + k0) / 2);
+    unsigned char* scales = p.scales + scale_at(p, m, row, k0);
+    const uint4* x = kF32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p.x) + src)
+                          : reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + src);
+    uint4 a[kParts], b[kParts];   // raw bits; b only for fp32
 #pragma unroll
-    for (int q = 0; q < kRowsPerItem; ++q) {
-      const long long row = it.row_block * 128 + q * 32 + it.row;
-      const bool in = in_k && row < p.rows;
-      const long long at = it.matrix * p.stack_x + row * p.ldx + k;
+    for (int q = 0; q < kParts; ++q) {
+      a[q] = b[q] = make_uint4(0, 0, 0, 0);
+      if (in_rows && k0 + q * 256 < p.K) {   // K is a multiple of 32: blocks are whole
+        a[q] = __ldcs(x + q * (kF32 ? 64 : 32));
+        if (kF32) b[q] = __ldcs(x + q * 64 + 1);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      const long long k = k0 + q * 256;
+      const bool in = in_rows && k < p.K;
+      float v[8];
+      uint32_t s;
+      // Magnitudes as bits are ordered like the values, with Inf and NaN on top.
       if (kF32) {
-        float4 a = make_float4(0, 0, 0, 0), b = a;
-        if (in) {
-          const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + at);
-          a = src[0];
-          b = src[1];
-        }
-        v[q][0] = a.x; v[q][1] = a.y; v[q][2] = a.z; v[q][3] = a.w;
-        v[q][4] = b.x; v[q][5] = b.y; v[q][6] = b.z; v[q][7] = b.w;
+        const uint32_t w[8] = {a[q].x, a[q].y, a[q].z, a[q].w, b[q].x, b[q].y, b[q].z, b[q].w};
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, w[j] & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        s = scale_of(top >> 23);
+        const float up = __uint_as_float((254 - min(s, 252u)) << 23);   // 2^(127 - s), a normal number
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]) * up;
       } else {
-        uint4 a = make_uint4(0, 0, 0, 0);
-        if (in) a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + at);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        uint32_t w[4] = {a[q].x, a[q].y, a[q].z, a[q].w};
+        uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                                __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = max(top >> 16, top & 0xffffu);
+        s = scale_of(top >> 7);
+        // A power of two: exact, but for values far below the smallest code's half.
+        const uint32_t up = (254 - min(s, 252u)) * 0x00800080u;
+        __nv_bfloat162 up2;
+        memcpy(&up2, &up, 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[q][2 * j] = __uint_as_float(w[j] << 16);
-          v[q][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+          __nv_bfloat162 t;
+          memcpy(&t, &w[j], 4);
+          t = __hmul2(t, up2);
+          memcpy(&w[j], &t, 4);
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
         }
       }
+      uint32_t code = e2m1_pair(v[0], v[1]) | e2m1_pair(v[2], v[3]) << 8 | e2m1_pair(v[4], v[5]) << 16 |
+                      e2m1_pair(v[6], v[7]) << 24;
+      if (s == 255) code = 0;
+      if (in) codes[q * 32] = code;
+      if ((threadIdx.x & 3) == 0 && k < k_scales)
+        scales[q * 1024] = static_cast<unsigned char>(in ? s : 0u);
     }
-    uint32_t words[kRowsPerItem];   // the four scales of this lane's 128 values, row by row
-#pragma unroll
-    for (int q = 0; q < kRowsPerItem; ++q) {
-      const long long row = it.row_block * 128 + q * 32 + it.row;
-      const bool in = in_k && row < p.rows;
-      // Largest magnitude as bits: ordered like the values, with Inf and NaN on top.
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[q][j]) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t e = top >> 23;
-      const bool bad = e == 255;
-      const uint32_t s = e > 2 ? e - 2 : 0;            // biased exponent of the block's scale
-      const float up = __uint_as_float((254 - s) << 23);   // 2^(127 - s): a normal number
-      uint32_t code = 0;
-      if (!bad) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          code |= e2m1_pair(v[q][2 * j] * up, v[q][2 * j + 1] * up) << (8 * j);
-      }
-      if (in)
-        reinterpret_cast<uint32_t*>(p.codes)[((it.matrix * p.rows + row) * p.K + k) >> 3] = code;
-      // The block's four lanes agree; gather four blocks' bytes into a word.
-      uint32_t byte = in ? (bad ? 255u : s) : 0u;
-      uint32_t word = byte << (8 * ((lane >> 2) & 3));
-      word |= __shfl_xor_sync(0xffffffffu, word, 4);
-      word |= __shfl_xor_sync(0xffffffffu, word, 8);
-      words[q] = word;
-    }
-    if ((lane & 15) == 0 && (it.k0 + lane * 8) / 128 < p.k_tiles)
-      *reinterpret_cast<uint4*>(p.scales + scale_tile(p, it) + (lane >> 4) * 512) =
-          make_uint4(words[0], words[1], words[2], words[3]);
   }
 }
 
-// An E2M1 code as fp32: exponent and mantissa sit three bits wide; code 1 is the subnormal 0.5.
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-  const uint32_t m = code & 7;
-  const uint32_t bits = m == 0 ? 0u : m == 1 ? 0x3f000000u : (m << 22) + 0x3f000000u;
-  return __uint_as_float(bits | ((code & 8) << 28));
-}
+// Four codes in the low 16 bits of `m` (magnitudes, sign bits clear) to the bytes of their bf16.
+__device__ __forceinline__ uint32_t high_bytes(uint32_t m) { return __byte_perm(0x3f3f3f00u, 0x40404040u, m); }
+__device__ __forceinline__ uint32_t low_bytes(uint32_t m) { return __byte_perm(0xc0800000u, 0xc0804000u, m); }
 
 __global__ void __launch_bounds__(kThreads) mxfp4_dequantize_kernel(const ConvertParams p) {
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
-  const int lane = threadIdx.x & 31;
-  const long long warps = static_cast<long long>(gridDim.x) * (kThreads / 32);
-  for (long long i = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-       i < p.items; i += warps) {
-    const Item it = item_of(p, i);
-    const long long k = it.k0 + lane * 8;
-    if (k >= p.K) continue;
-    const uint4 sw = *reinterpret_cast<const uint4*>(p.scales + scale_tile(p, it) + (lane >> 4) * 512);
-    const uint32_t words[kRowsPerItem] = {sw.x, sw.y, sw.z, sw.w};
-    uint32_t code[kRowsPerItem];
+  long long row, k0;
+  if (!place(p, &row, &k0) || row >= p.rows) return;
+  for (long long m = blockIdx.y; m < p.stack; m += gridDim.y) {
+    const long long first = (m * p.rows + row) * p.K + k0;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.codes + first / 2);
+    const unsigned char* scales = p.scales + scale_at(p, m, row, k0);
+    uint4* out = reinterpret_cast<uint4*>(p.y + first);
+    uint32_t code[kParts], scale[kParts];
 #pragma unroll
-    for (int q = 0; q < kRowsPerItem; ++q) {
-      const long long row = it.row_block * 128 + q * 32 + it.row;
-      code[q] = row < p.rows
-          ? reinterpret_cast<const uint32_t*>(p.codes)[((it.matrix * p.rows + row) * p.K + k) >> 3]
-          : 0u;
+    for (int q = 0; q < kParts; ++q) {
+      code[q] = scale[q] = 0;
+      if (k0 + q * 256 < p.K) {
+        code[q] = __ldcs(codes + q * 32);
+        scale[q] = scales[q * 1024];
+      }
     }
 #pragma unroll
-    for (int q = 0; q < kRowsPerItem; ++q) {
-      const long long row = it.row_block * 128 + q * 32 + it.row;
-      if (row >= p.rows) continue;
-      const uint32_t s = (words[q] >> (8 * ((lane >> 2) & 3))) & 255u;
-      // 2^(s - 127); the smallest is half of the smallest normal number.
-      const float scale = __uint_as_float(s == 255 ? 0x7fc00000u : s == 0 ? 0x00400000u : s << 23);
-      uint32_t out[4];
+    for (int q = 0; q < kParts; ++q) {
+      // 2^(s - 127) in bf16, twice; the smallest is half of the smallest normal number.
+      const uint32_t s = scale[q];
+      const uint32_t bits = s == 255 ? 0x7fc07fc0u : s == 0 ? 0x00400040u : s * 0x00800080u;
+      __nv_bfloat162 factor;
+      memcpy(&factor, &bits, 4);
+      const uint32_t mag = code[q] & 0x77777777u, even = code[q] << 4;
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        out[j] = ptx::pack_bf16x2(e2m1_value(code[q] >> (8 * j)) * scale,
-                                  e2m1_value(code[q] >> (8 * j + 4)) * scale);
-      *reinterpret_cast<uint4*>(p.y + (it.matrix * p.rows + row) * p.K + k) =
-          make_uint4(out[0], out[1], out[2], out[3]);
+      for (int h = 0; h < 2; ++h) {
+        // Sign bits of four codes to the top bits of four bytes: codes 0 and 2 from `even`.
+        const uint32_t sign = __byte_perm(even, code[q], h ? 0x7362 : 0x5140) & 0x80808080u;
+        const uint32_t hi = high_bytes(mag >> (16 * h)) | sign, lo = low_bytes(mag >> (16 * h));
+        w[2 * h] = __byte_perm(lo, hi, 0x5140);
+        w[2 * h + 1] = __byte_perm(lo, hi, 0x7362);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __nv_bfloat162 t;
+        memcpy(&t, &w[j], 4);
+        t = __hmul2(t, factor);
+        memcpy(&w[j], &t, 4);
+      }
+      if (k0 + q * 256 < p.K) out[q * 32] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -186,17 +197,16 @@ void fill(ConvertParams& p, int64_t stack, int64_t rows, int64_t K) {
   p.K = K;
   p.row_blocks = (rows + 127) / 128;
   p.k_tiles = (K + 127) / 128;
-  p.k_items = (K + 255) / 256;
-  p.items = stack * p.row_blocks * 32 * p.k_items;
+  p.spans = static_cast<unsigned>((K + kSpan - 1) / kSpan);
 }
 
-int launch(const DeviceView& dev, const void* fn, ConvertParams& p, cudaStream_t stream) {
-  // Eight blocks of 256 threads fill an SM.
-  const long long blocks = std::min<long long>((p.items + kThreads / 32 - 1) / (kThreads / 32),
-                                               8ll * dev.sm_count);
+int launch(const void* fn, ConvertParams& p, cudaStream_t stream) {
+  const long long warps = p.row_blocks * 128 * p.spans;
+  if (warps > 0xffffffffll - kWarps) return NEOGEMM_ERR_UNSUPPORTED;
+  const long long x = (warps + kWarps - 1) / kWarps, y = std::min<long long>(p.stack, 65535);
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y), 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -215,10 +225,10 @@ int launch(const DeviceView& dev, const void* fn, ConvertParams& p, cudaStream_t
 int check(int64_t stack, int64_t rows, int64_t K, const void* codes, const void* scales) {
   if (stack < 0 || rows < 0 || K < 0) return NEOGEMM_ERR_BAD_ARG;
   if (K % 32 != 0) return NEOGEMM_ERR_UNSUPPORTED;
-  // Extents far past any memory would overflow the products below.
+  // Extents far past any memory would overflow the products above.
   if (stack > (1ll << 31) || rows > (1ll << 31) || K > (1ll << 31)) return NEOGEMM_ERR_UNSUPPORTED;
   if (stack == 0 || rows == 0 || K == 0) return NEOGEMM_OK;
-  if (stack * rows > (1ll << 45) / K) return NEOGEMM_ERR_UNSUPPORTED;
+  if (stack > (1ll << 45) / rows || stack * rows > (1ll << 45) / K) return NEOGEMM_ERR_UNSUPPORTED;
   if (codes == nullptr || scales == nullptr) return NEOGEMM_ERR_BAD_ARG;
   if (!aligned16(codes) || !aligned16(scales)) return NEOGEMM_ERR_UNSUPPORTED;
   return NEOGEMM_OK;
@@ -237,7 +247,9 @@ int neogemm_mxfp4_quantize(const void* X, int x_is_f32, void* codes, void* scale
   if (rc != NEOGEMM_OK) return rc;
   if (stack == 0 || rows == 0 || K == 0) return NEOGEMM_OK;
   if (X == nullptr || ldx < K || stack_x < 0) return NEOGEMM_ERR_BAD_ARG;
-  if (!aligned16(X) || ldx % 8 != 0 || (stack > 1 && stack_x % 8 != 0)) return NEOGEMM_ERR_UNSUPPORTED;
+  const int64_t step = x_is_f32 ? 4 : 8;   // elements in 16 bytes
+  if (!aligned16(X) || (rows > 1 && ldx % step != 0) || (stack > 1 && stack_x % step != 0))
+    return NEOGEMM_ERR_UNSUPPORTED;
   DeviceView dev;
   rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
@@ -251,7 +263,7 @@ int neogemm_mxfp4_quantize(const void* X, int x_is_f32, void* codes, void* scale
   p.stack_x = stack_x;
   const void* fn = x_is_f32 ? reinterpret_cast<const void*>(&mxfp4_quantize_kernel<true>)
                             : reinterpret_cast<const void*>(&mxfp4_quantize_kernel<false>);
-  return launch(dev, fn, p, static_cast<cudaStream_t>(stream));
+  return launch(fn, p, static_cast<cudaStream_t>(stream));
 }
 
 int neogemm_mxfp4_dequantize(const void* codes, const void* scales, void* Y, int64_t stack,
@@ -270,7 +282,7 @@ int neogemm_mxfp4_dequantize(const void* codes, const void* scales, void* Y, int
   p.codes = static_cast<unsigned char*>(const_cast<void*>(codes));
   p.scales = static_cast<unsigned char*>(const_cast<void*>(scales));
   p.y = static_cast<__nv_bfloat16*>(Y);
-  return launch(dev, reinterpret_cast<const void*>(&mxfp4_dequantize_kernel), p,
+  return launch(reinterpret_cast<const void*>(&mxfp4_dequantize_kernel), p,
                 static_cast<cudaStream_t>(stream));
 }
 
