@@ -44,7 +44,7 @@ const KernelEntry kKernels[4][2] = {
     {make_entry<GroupedConfig<kGroupedNt, 1, 128, 8>>(), make_entry<GroupedConfig<kGroupedNt, 2, 256, 6>>()},
     {make_entry<GroupedConfig<kGroupedDx, 1, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 256, 6>>()},
     {make_entry<GroupedConfig<kGroupedDw, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 256, 6>>()},
-    {make_entry<GroupedConfig<kMxNt, 1, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 1, 128, 8>>()},
+    {make_entry<GroupedConfig<kMxNt, 1, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 2, 256, 5>>()},
 };
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -19,7 +19,7 @@
 // remnant.  dW has no ragged output; there the group's rows are the contraction.
 //
 //   warp 0      TMA producer      warp 1      UMMA issuer (leader CTA of a pair)
-//   warps 2-5   epilogue: tcgen05.ld -> bf16 -> shared-memory transpose -> 16-byte row stores,
+//   warps 2-5   (2-9) epilogue: tcgen05.ld -> bf16 -> shared-memory transpose -> 16-byte row stores,
 //               overlapped with the next tile through a second accumulator
 //   warp 6      kGroupedDw only: clears the rows of a tile's last k-block that belong to the next
 //               group (both operands: a zero times a neighbour's Inf would still be NaN)
@@ -92,13 +92,20 @@ struct GroupedConfig {
   static constexpr int kLaneBytes = kLaneRows * 128;
   static constexpr int kColBytes = kHalfCols * 128;
   // MXFP4: the instruction takes the scales of 128 rows from four columns of tensor memory that
-  // start at a multiple of four, so lanes and columns keep to frames of 128 rows (kCols for the
-  // columns), the blocks in which the scales are stored.  A tile uses a part of its frame: rows
-  // outside are not fetched and their lanes or columns are not stored.
+  // start at a multiple of four, so lanes and columns start at multiples of 128 rows, the blocks in
+  // which the scales are stored.  A tile uses a part of its frame: rows outside are not fetched and
+  // their lanes or columns are not stored.
   static constexpr int kScaleCols = (kCols + 127) / 128;      // blocks of scales of the columns
   static constexpr int kScaleBytes = (kOp == kMxNt) ? 1024 * (1 + kScaleCols) : 0;
   static constexpr int kStageBytes = kLaneBytes + kColBytes + kScaleBytes;
-  static constexpr int kEpiBytes = 4 * 2 * 2048;    // per epilogue warp two buffers of 32 x 32 bf16
+  // Two accumulators, so that a tile's epilogue overlaps the next tile's products.  The MXFP4 pair
+  // takes one of 256 columns instead (the scales need the rest of tensor memory): narrower tiles are
+  // bound by shared memory - 256 x 128 reads and fills 192 bytes per cycle of the 128 there are - and
+  // its eight epilogue warps pull the accumulator into registers, packed, before they store anything.
+  static constexpr int kAccs = (kOp == kMxNt && kCtaGroup == 2) ? 1 : 2;
+  static constexpr int kEpiWarps = (kAccs == 1) ? 8 : 4;
+  static constexpr int kEpiCols = kCols * 4 / kEpiWarps;   // columns that a warp stores at most
+  static constexpr int kEpiBytes = kEpiWarps * 2 * 2048;   // per warp two buffers of 32 x 32 bf16
   static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
   static constexpr int kBarrierBytes = (3 * kStages + 4) * 8 + 16;
   static constexpr int kRestBytes = kEpiBytes + kTableBytes + 12 + kBarrierBytes + 1024;
@@ -108,14 +115,14 @@ struct GroupedConfig {
   static_assert(kOp != kMxNt || !kStream || kEpiBytes >= 96 * 128, "room in front of the ring");
   static_assert(kEpiBytes % 1024 == 0, "the ring starts on the swizzle's alignment");
   static constexpr int kSmemBytes = kRingBytes + kRestBytes;
-  // Two accumulators, and behind them (MXFP4) the scales of every k-block in the ring: per 128
+  // The accumulators, and behind them (MXFP4) the scales of every k-block in the ring: per 128
   // values of K four columns per 128 rows.
   static constexpr int kScaleTmemCols = (kOp == kMxNt) ? 8 * (1 + kScaleCols) : 0;
-  static constexpr int kScaleSets = (kOp != kMxNt) ? 0 : kStream ? (512 - 2 * kCols) / kScaleTmemCols : kStages;
-  static constexpr int kTmemNeeded = 2 * kCols + kScaleSets * kScaleTmemCols;
+  static constexpr int kScaleSets = (kOp != kMxNt) ? 0 : kStream ? (512 - kAccs * kCols) / kScaleTmemCols : kStages;
+  static constexpr int kTmemNeeded = kAccs * kCols + kScaleSets * kScaleTmemCols;
   static constexpr int kTmemCols = (kCtaGroup == 2) ? 512 : kTmemNeeded <= 128 ? 128
                                  : kTmemNeeded <= 256 ? 256 : 512;
-  static constexpr int kThreads = (kOp == kGroupedDw) ? 224 : 192;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps + ((kOp == kGroupedDw) ? 32 : 0);
   // Arrivals that complete a ring slot's phase besides its bytes: the slot's producer, and for
   // dW one per CTA (the last block of a tile is handed over by the warps that cleared its rows).
   static constexpr int kFullArrivals = (kOp == kGroupedDw) ? kCtaGroup : 1;
@@ -156,7 +163,7 @@ __device__ __forceinline__ void report_error(int* status, volatile int* abort_fl
 template <class Cfg>
 __device__ __forceinline__ int column_tiles(const GroupedParams& p, int begin, int end) {
   if (end <= begin) return 0;
-  if (Cfg::kOp == kMxNt) return (end - 1) / Cfg::kCols - begin / Cfg::kCols + 1;
+  if (Cfg::kOp == kMxNt) return (end - begin / 128 * 128 + Cfg::kCols - 1) / Cfg::kCols;
   return (end - begin + p.col_cap - 1) / p.col_cap;
 }
 
@@ -262,7 +269,7 @@ struct GroupedTiles {
         next += step;
       }
       if (Cfg::kOp == kMxNt) {
-        t.col_row = (g0 / Cfg::kCols + c) * Cfg::kCols;
+        t.col_row = g0 / 128 * 128 + c * Cfg::kCols;
         t.lo = max(g0 - t.col_row, 0);
         t.hi = min(g1 - t.col_row, Cfg::kCols);
       } else {
@@ -382,7 +389,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tmem_full_bar + 8 * a, 1);
-      mbar_init(tmem_empty_bar + 8 * a, 4 * kCtaGroup);
+      mbar_init(tmem_empty_bar + 8 * a, Cfg::kEpiWarps * kCtaGroup);
     }
     fence_barrier_init();
   }
@@ -562,7 +569,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       for (; ok && tiles.take(p, t); ++tile) {
         if (t.blocks == 0) continue;
         make_uniform(t);
-        const uint32_t acc = count & 1, acc_phase = (count >> 1) & 1;
+        const uint32_t acc = count % Cfg::kAccs, acc_phase = (count / Cfg::kAccs) & 1;
         ++count;
         if (!__all_sync(0xffffffffu, mbar_wait<kCtaGroup == 2>(tmem_empty_bar + 8 * acc,
                                                                acc_phase ^ 1, abort_flag))) {
@@ -606,7 +613,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             if constexpr (kMx) {
               // Scales of 128 values of K: four columns of tensor memory per block of 128 rows.
               const uint32_t set = Cfg::kStream ? stage * sets_per_slot + j : stage;
-              const uint32_t tsl = tmem_base + 2 * Cfg::kCols + set * Cfg::kScaleTmemCols;
+              const uint32_t tsl = tmem_base + Cfg::kAccs * Cfg::kCols + set * Cfg::kScaleTmemCols;
               const uint32_t tsc = tsl + 8;
               const uint64_t ds = make_smem_desc_scales(sc + at.col_bytes);
               if (elect_one()) {
@@ -662,15 +669,16 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         __syncwarp();
       }
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + Cfg::kEpiWarps) {
     // ======================= epilogue =======================
     const int quad = warp & 3;   // the warp's quarter of the tensor-memory lanes
+    const int first_col = (warp - 2) / 4 * Cfg::kEpiCols;   // and its share of the columns
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t stage_buf = epi_base + quad * 4096;
+    const uint32_t stage_buf = epi_base + (warp - 2) * 4096;
     uint32_t buf = 0;
     int count = 0;
     for (; tiles.take(p, t); ++tile) {
-      const uint32_t acc = count & 1, acc_phase = (count >> 1) & 1;
+      const uint32_t acc = count % Cfg::kAccs, acc_phase = (count / Cfg::kAccs) & 1;
       if (t.blocks > 0) {
         ++count;
         if (!__all_sync(0xffffffffu, mbar_wait(tmem_full_bar + 8 * acc, acc_phase, abort_flag))) {
@@ -682,99 +690,106 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       }
       const int lane_first = t.lane0 + rank * Cfg::kLaneRows + quad * 32;   // of this warp
       const int lane_end = min(p.lanes, t.lane0 + rank * Cfg::kLaneRows + t.lane_lo + t.lane_rows);
-      const bool in_use = lane_first < lane_end && quad * 32 + 32 > t.lane_lo;
-      for (int c = t.lo & ~31; c < t.hi && in_use; c += 32) {
-        uint32_t r[32];
+      const bool lanes_in_use = lane_first < lane_end && quad * 32 + 32 > t.lane_lo;
+      // 32 columns of this warp's lanes, rounded to bf16 and packed in pairs.
+      auto pull = [&](int c, uint32_t (&w)[16]) {
         if (t.blocks > 0) {
+          uint32_t r[32];
           tmem_ld_32x32b_x32(tmem_base + acc * Cfg::kCols + lane_base + c, r);
           tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            w[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = 0u;
+          for (int j = 0; j < 16; ++j) w[j] = 0u;
         }
-        const uint32_t s = stage_buf + buf * 2048;
-        buf ^= 1;
-        if constexpr (kDw) {
-          // Lane = row of the result: 64 bytes of it, 16-byte units swizzled against conflicts.
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]),
-                                 __uint_as_float(r[8 * j + 2 * i + 1]));
-            st_shared_v4(s + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
-            uint32_t v[4];
-            ld_shared_v4(s + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4), v);
-            const int n = lane_first + row, col = t.col_row + c + unit * 8;
-            if (n < lane_end && c + unit * 8 < t.hi) {
-              __nv_bfloat16* dst = p.out + t.group * p.out_stack + n * p.out_pitch + col;
-              if (p.vector_out && c + unit * 8 + 8 <= t.hi) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
-              } else {
-                const int left = min(t.hi - (c + unit * 8), 8);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (j < left)
-                    reinterpret_cast<unsigned short*>(dst)[j] =
-                        static_cast<unsigned short>(v[j >> 1] >> ((j & 1) * 16));
-              }
-            }
-          }
-        } else {
-          // Lane = column of the result: transposed through shared memory, 32 values of one row
-          // of the batch side by side.
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const uint32_t w = pack_bf16x2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-            st_shared_b16(s + j * 64 + lane * 2, static_cast<unsigned short>(w));
-            st_shared_b16(s + (j + 1) * 64 + lane * 2, static_cast<unsigned short>(w >> 16));
-          }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
-            uint32_t v[4];
-            ld_shared_v4(s + row * 64 + unit * 16, v);
-            const int col = lane_first + unit * 8;
-            if (c + row >= t.lo && c + row < t.hi && col < lane_end) {
-              __nv_bfloat16* dst =
-                  p.out + static_cast<long long>(t.col_row + c + row) * p.out_pitch + col;
-              if (p.vector_out && col + 8 <= lane_end) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
-              } else {
-                const int left = min(lane_end - col, 8);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (j < left)
-                    reinterpret_cast<unsigned short*>(dst)[j] =
-                        static_cast<unsigned short>(v[j >> 1] >> ((j & 1) * 16));
-              }
-            }
-          }
-        }
-      }
-      if (t.blocks > 0) {
-        // The accumulator has been read: hand it back.
+      };
+      auto hand_back = [&] {
+        if (t.blocks == 0) return;
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) {
           if (kCtaGroup == 2) mbar_arrive_cluster(mapa_u32(tmem_empty_bar + 8 * acc, 0));
           else mbar_arrive(tmem_empty_bar + 8 * acc);
         }
+      };
+      auto store = [&](int c, const uint32_t (&w)[16]) {
+        const uint32_t s = stage_buf + buf * 2048;
+        buf ^= 1;
+        // 16 bytes of the result at `dst`, of which `left` values exist.
+        auto put = [&](__nv_bfloat16* dst, const uint32_t (&v)[4], int left) {
+          if (p.vector_out && left >= 8) {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j < left)
+                reinterpret_cast<unsigned short*>(dst)[j] =
+                    static_cast<unsigned short>(v[j >> 1] >> ((j & 1) * 16));
+          }
+        };
+        if constexpr (kDw) {
+          // Lane = row of the result: 64 bytes of it, 16-byte units swizzled against conflicts.
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            st_shared_v4(s + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[4 * j], w[4 * j + 1],
+                         w[4 * j + 2], w[4 * j + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
+            uint32_t v[4];
+            ld_shared_v4(s + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4), v);
+            const int n = lane_first + row, col = c + unit * 8;
+            if (n < lane_end && col < t.hi)
+              put(p.out + t.group * p.out_stack + n * p.out_pitch + t.col_row + col, v, t.hi - col);
+          }
+        } else {
+          // Lane = column of the result: transposed through shared memory, 32 values of one row
+          // of the batch side by side.
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            st_shared_b16(s + 2 * j * 64 + lane * 2, static_cast<unsigned short>(w[j]));
+            st_shared_b16(s + (2 * j + 1) * 64 + lane * 2, static_cast<unsigned short>(w[j] >> 16));
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = c + i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
+            uint32_t v[4];
+            ld_shared_v4(s + (row - c) * 64 + unit * 16, v);
+            const int col = lane_first + unit * 8;
+            if (row >= t.lo && row < t.hi && col < lane_end)
+              put(p.out + static_cast<long long>(t.col_row + row) * p.out_pitch + col, v, lane_end - col);
+          }
+        }
+      };
+      auto in_use = [&](int c) { return lanes_in_use && c < t.hi && c + 32 > t.lo; };
+      if constexpr (Cfg::kAccs == 1) {
+        uint32_t w[Cfg::kEpiCols / 32][16];
+#pragma unroll
+        for (int i = 0; i < Cfg::kEpiCols / 32; ++i)
+          if (in_use(first_col + i * 32)) pull(first_col + i * 32, w[i]);
+        hand_back();
+#pragma unroll
+        for (int i = 0; i < Cfg::kEpiCols / 32; ++i)
+          if (in_use(first_col + i * 32)) store(first_col + i * 32, w[i]);
+      } else {
+        for (int c = t.lo & ~31; in_use(c); c += 32) {
+          uint32_t w[16];
+          pull(c, w);
+          store(c, w);
+        }
+        hand_back();
       }
     }
     if (!kDw && p.zero_rest) {
       // Rows of no group: in front of the first and behind the last.
       const int head = begin[0], tail = end[p.groups - 1];
       const int rest = head + p.rows - tail;
-      for (int i = static_cast<int>(blockIdx.x) * 4 + quad; i < rest;
-           i += static_cast<int>(gridDim.x) * 4) {
+      for (int i = static_cast<int>(blockIdx.x) * Cfg::kEpiWarps + warp - 2; i < rest;
+           i += static_cast<int>(gridDim.x) * Cfg::kEpiWarps) {
         const int row = i < head ? i : tail + i - head;
         __nv_bfloat16* dst = p.out + static_cast<long long>(row) * p.out_pitch;
         int c = static_cast<int>(lane) * 8;
