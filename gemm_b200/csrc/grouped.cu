@@ -16,35 +16,36 @@ constexpr int kMaxDevices = 64;
 constexpr int64_t kMaxExtent = 0x7fffffffll - 4096;   // room for tile coordinates past the end
 
 struct KernelEntry {
-  int op, cta_group, columns, stages;
-  bool stream;
-  int lane_step;   // lanes of a tile (streaming: of a unit)
+  int op, cta_group, split, columns, stages;
+  int lane_step;   // lanes of a tile
   int col_step;    // granularity of a tile's columns
-  int lane_box;        // rows of the lane operand's boxes
+  int lane_box;    // rows of the lane operand's boxes
   int ring_bytes, scale_bytes;   // shared memory: the ring, and the scales of a k-block
+  int scale_sets;  // MXFP4: k-blocks whose scales tensor memory holds
   const void* fn;
   int smem_bytes, threads;
 };
 
 template <class Cfg>
 KernelEntry make_entry() {
-  constexpr bool kDw = Cfg::kOp == kGroupedDw;
-  return KernelEntry{Cfg::kOp, Cfg::kCtaGroup, Cfg::kCols, Cfg::kStages, Cfg::kStream,
-                     Cfg::kStream ? Cfg::kUnit : Cfg::kLaneTile,
-                     Cfg::kColStep,
-                     // MN-major operands come in boxes of 64 x 64
-                     kDw || Cfg::kOp == kGroupedDx ? 64 : 128,
-                     Cfg::kRingBytes, Cfg::kScaleBytes,
-                     reinterpret_cast<const void*>(&grouped_kernel<Cfg>), Cfg::kSmemBytes,
-                     Cfg::kThreads};
+  constexpr bool kMnMajor = Cfg::kOp == kGroupedDw || Cfg::kOp == kGroupedDx;   // boxes of 64 x 64
+  return KernelEntry{Cfg::kOp, Cfg::kCtaGroup, Cfg::kSplit, Cfg::kCols, Cfg::kStages, Cfg::kLaneTile,
+                     Cfg::kColStep, kMnMajor ? 64 : 128, Cfg::kRingBytes, Cfg::kScaleBytes,
+                     Cfg::kScaleSets, reinterpret_cast<const void*>(&grouped_kernel<Cfg>),
+                     Cfg::kSmemBytes, Cfg::kThreads};
 }
 
-// [operation][0 narrow, 1 wide]
-const KernelEntry kKernels[4][2] = {
-    {make_entry<GroupedConfig<kGroupedNt, 1, 128, 8>>(), make_entry<GroupedConfig<kGroupedNt, 2, 256, 6>>()},
-    {make_entry<GroupedConfig<kGroupedDx, 1, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 256, 6>>()},
-    {make_entry<GroupedConfig<kGroupedDw, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 256, 6>>()},
-    {make_entry<GroupedConfig<kMxNt, 1, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 2, 256, 5>>()},
+// [operation][variant]
+enum Variant : int { kNarrow = 0, kWide = 1, kMiddle = 2, kVariants = 3 };
+const KernelEntry kKernels[4][kVariants] = {
+    {make_entry<GroupedConfig<kGroupedNt, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kGroupedNt, 2, 1, 256, 6>>(),
+     make_entry<GroupedConfig<kGroupedNt, 1, 2, 128, 8>>()},
+    {make_entry<GroupedConfig<kGroupedDx, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 1, 256, 6>>(),
+     make_entry<GroupedConfig<kGroupedDx, 1, 2, 128, 8>>()},
+    {make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 1, 256, 6>>(),
+     make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 6>>()},
+    {make_entry<GroupedConfig<kMxNt, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 2, 1, 256, 5>>(),
+     make_entry<GroupedConfig<kMxNt, 1, 2, 128, 8>>()},
 };
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -78,43 +79,61 @@ int encode_bf16(const DeviceView& dev, CUtensorMap* map, const void* base, int64
 
 int launch(const DeviceView& dev, const KernelEntry& k, int64_t tiles_at_most,
            const GroupedMaps& maps, const GroupedParams& params, cudaStream_t stream) {
-  static std::mutex mu;
-  static bool attr_done[kMaxDevices][4][2] = {};
-  const int which = &k == &kKernels[k.op][1] ? 1 : 0;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    bool& done = attr_done[dev.index][k.op][which];
-    if (!done && cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      k.smem_bytes) != cudaSuccess) {
-      cudaGetLastError();
-      return NEOGEMM_ERR_LAUNCH;
-    }
-    done = true;
-  }
-  const int64_t workers = std::max<int64_t>(
-      1, std::min<int64_t>(dev.sm_count / k.cta_group, tiles_at_most));
+  const int cluster = k.cta_group * k.split;
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(workers * k.cta_group), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(k.threads), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(k.smem_bytes);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int nattr = 0;
-  if (k.cta_group == 2) {
+  if (cluster > 1) {
     attr[nattr].id = cudaLaunchAttributeClusterDimension;
-    attr[nattr].val.clusterDim.x = 2;
+    attr[nattr].val.clusterDim.x = static_cast<unsigned>(cluster);
     attr[nattr].val.clusterDim.y = 1;
     attr[nattr].val.clusterDim.z = 1;
     ++nattr;
   }
+  cfg.attrs = attr;
+  cfg.numAttrs = nattr;
+
+  // Clusters that the device holds at a time: the launch is one such wave, with a fixed list of
+  // tiles for each.
+  static std::mutex mu;
+  static int resident[kMaxDevices][4][kVariants] = {};
+  const int variant = static_cast<int>(&k - kKernels[k.op]);
+  int workers;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    int& known = resident[dev.index][k.op][variant];
+    if (known == 0) {
+      if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem_bytes) !=
+          cudaSuccess) {
+        cudaGetLastError();
+        return NEOGEMM_ERR_LAUNCH;
+      }
+      int most = dev.sm_count / cluster;
+      if (cluster > 1) {
+        cfg.gridDim = dim3(static_cast<unsigned>(most * cluster), 1, 1);
+        int fit = 0;
+        if (cudaOccupancyMaxActiveClusters(&fit, k.fn, &cfg) != cudaSuccess || fit < 1) {
+          cudaGetLastError();
+          return NEOGEMM_ERR_LAUNCH;
+        }
+        most = std::min(most, fit);
+      }
+      known = most;
+    }
+    workers = known;
+  }
+  workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(workers, tiles_at_most)));
+  cfg.gridDim = dim3(static_cast<unsigned>(workers * cluster), 1, 1);
   if (tuning_value(10) != 0) {
     // The kernel's set-up overlaps the tail of the stream's previous kernel (see launcher.cu).
     attr[nattr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[nattr].val.programmaticStreamSerializationAllowed = 1;
     ++nattr;
   }
-  cfg.attrs = attr;
   cfg.numAttrs = nattr;
   void* args[2] = {const_cast<GroupedMaps*>(&maps), const_cast<GroupedParams*>(&params)};
   if (cudaLaunchKernelExC(&cfg, k.fn, args) != cudaSuccess) {
@@ -155,13 +174,13 @@ int zero_rows(void* out, int64_t pitch, int64_t rows, int64_t width, cudaStream_
 int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, GroupedParams* p,
               int64_t* tiles_at_most) {
   int64_t cap = k.columns;
-  if (k.stream) {
+  if (k.split > 1) {
     // MXFP4 tiles take their rows from a frame of the whole batch.
     const int64_t likely = k.op == kMxNt ? T : std::min(T, 4 * (T / groups) + 16);
     cap = std::min(cap, ceil_div(likely, k.col_step) * k.col_step);
   }
   const int64_t lane_tiles = ceil_div(lanes, k.lane_step);
-  // Tiles that keep to a grid of rows may touch one more than the group's length says.
+  // MXFP4 tiles that start in front of their group may touch one more than its length says.
   const int64_t tiles = lane_tiles * (2 * std::min(groups, T) + T / (k.op == kMxNt ? k.columns : cap));
   if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
   *tiles_at_most = tiles;
@@ -171,23 +190,25 @@ int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, Gr
   p->col_box = static_cast<int>(ceil_div(cap / k.cta_group, 16) * 16);
   p->small_box = std::min(p->col_box, 32);
   if (p->col_box > 32) p->col_box = static_cast<int>(ceil_div(p->col_box, 32) * 32);
-  if (k.stream) {
-    // Slots of two full k-blocks where four of them fit: half the waits.  Behind the last slot an
-    // MMA reads up to one k-block's lanes.
+  if (k.split > 1) {
+    // Slots of two k-blocks where four of them fit: half the waits.
     const int block = 128 * 128 + p->col_box * 128 + k.scale_bytes;
-    const int room = k.ring_bytes - 128 * 128;
-    p->slot_bytes = room / (2 * block) >= 4 ? 2 * block : block;
-    p->slots = std::min(k.stages, room / p->slot_bytes);
+    p->per_slot = k.ring_bytes / (2 * block) >= 4 ? 2 : 1;
+    p->slots = std::min(k.stages, k.ring_bytes / (p->per_slot * block));
   }
   return NEOGEMM_OK;
 }
 
-// Average rows per group from which the wide tiles (a CTA pair, 256 x 256) are taken.
+// Variant for an average of `rows` rows per group: CTA pairs with 256 x 256 tiles from kWideRows on;
+// below, the contraction is split over two CTAs, or over four where the columns of a tile are few and
+// their partial sums quickly exchanged.
 constexpr int64_t kWideRows = 96;
+constexpr int64_t kMiddleRows = 8;
 
-bool take_wide(int64_t average_rows) {
+int variant_of(int64_t rows) {
   const int forced = tuning_value(13);
-  return forced >= 0 ? forced != 0 : average_rows >= kWideRows;
+  if (forced >= 0) return forced;
+  return rows >= kWideRows ? kWide : rows >= kMiddleRows ? kMiddle : kNarrow;
 }
 
 // Y or dX: rows of the batch in, rows out.
@@ -213,7 +234,7 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  const KernelEntry& k = kKernels[op][take_wide(T / groups) ? 1 : 0];
+  const KernelEntry& k = kKernels[op][variant_of(T / groups)];
   GroupedParams p;
   std::memset(&p, 0, sizeof(p));
   p.offsets = offsets;
@@ -229,11 +250,6 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   std::memset(&maps, 0, sizeof(maps));
   if (depth > 0) {
     rc = encode_bf16(dev, &maps.lanes, W, K, N, groups, ldw, stack_w, k.lane_box);
-    if (rc == NEOGEMM_OK && k.stream && op == kGroupedNt) {
-      rc = encode_bf16(dev, &maps.two_units, W, K, N, groups, ldw, stack_w, 2 * k.lane_step);
-      if (rc == NEOGEMM_OK)
-        rc = encode_bf16(dev, &maps.unit, W, K, N, groups, ldw, stack_w, k.lane_step);
-    }
     if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps.cols, R, depth, T, 1, ldr, 0, p.col_box);
     if (rc == NEOGEMM_OK) rc = encode_bf16(dev, &maps.small_cols, R, depth, T, 1, ldr, 0, p.small_box);
     if (rc != NEOGEMM_OK) return rc;
@@ -275,7 +291,7 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
   int rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  const KernelEntry& k = kKernels[kMxNt][take_wide(T / groups) ? 1 : 0];
+  const KernelEntry& k = kKernels[kMxNt][variant_of(T / groups)];
   const int64_t k_tiles = ceil_div(K, 128), w_tiles = ceil_div(N, 128), x_tiles = ceil_div(T, 128);
   if (groups * w_tiles * k_tiles > kMaxExtent || x_tiles * k_tiles > kMaxExtent)
     return NEOGEMM_ERR_UNSUPPORTED;
@@ -294,10 +310,6 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
   std::memset(&maps, 0, sizeof(maps));
   if (K > 0) {
     rc = encode_codes(dev, &maps.lanes, Wc, K, N, groups, k.lane_box);
-    if (rc == NEOGEMM_OK && k.stream) {
-      rc = encode_codes(dev, &maps.two_units, Wc, K, N, groups, 2 * k.lane_step);
-      if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps.unit, Wc, K, N, groups, k.lane_step);
-    }
     if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps.cols, Xc, K, T, 1, p.col_box);
     if (rc == NEOGEMM_OK) rc = encode_codes(dev, &maps.small_cols, Xc, K, T, 1, p.small_box);
     if (rc == NEOGEMM_OK) rc = encode_scales(dev, &maps.lane_scales, Ws, groups * w_tiles * k_tiles, 1, 1);
@@ -357,8 +369,8 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
 
   // The pair's tiles are 256 x 256 of a group's matrix whatever its rows.
   const int forced = tuning_value(13);
-  const bool wide = forced >= 0 ? forced != 0 : N >= 256 && K >= 256;
-  const KernelEntry& k = kKernels[kGroupedDw][wide ? 1 : 0];
+  const bool wide = forced >= 0 ? forced == kWide : N >= 256 && K >= 256;
+  const KernelEntry& k = kKernels[kGroupedDw][wide ? kWide : kNarrow];
   GroupedMaps maps;
   std::memset(&maps, 0, sizeof(maps));
   if (T > 0) {

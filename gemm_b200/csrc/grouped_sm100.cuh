@@ -47,11 +47,11 @@ struct GroupedParams {
   int lanes;                // extent of the axis on the tensor-memory lanes (N; K for dx)
   int cols;                 // kGroupedDw: extent of the column axis (K)
   int depth;                // contraction length (K; N for dx; for dW the rows of the batch)
-  int lane_tiles;           // tiles along `lanes` (streaming kernels: units of kUnit)
+  int lane_tiles;           // tiles along `lanes`
   int col_cap;              // widest accumulator of a tile (a multiple of the column granularity)
   int col_box;              // rows of the ragged operand's large boxes (a CTA's share of col_cap)
   int small_box;            // and of its small ones
-  int slot_bytes, slots;    // streaming kernels: the ring
+  int slots, per_slot;      // streaming kernels: ring slots, and the k-blocks that each takes
   int col_tiles;            // kGroupedDw: tiles along `cols`
   int zero_rest;            // write zeros to the rows of no group (0: leave them)
   int vector_out;           // 16-byte stores are possible (alignment of base and pitches)
@@ -65,23 +65,24 @@ struct GroupedParams {
 
 // kCtaGroup == 2: tiles of 256 lanes x up to kCols columns on CTA pairs, for groups of many rows.
 //
-// kCtaGroup == 1 (but for dW): the streaming kernels, for groups of few rows, where the time is
-// that of reading the matrices once.  The lane axes of all groups are laid end to end in units of
-// kUnit rows and every CTA takes an equal run of units, cut into tiles of at most 128 lanes; so all
-// SMs read the same number of bytes whatever the number of chosen groups (with tiles of 128
-// lanes, 6 groups of 3584 rows are 168 tiles: two rounds on 148 SMs for 1.14 rounds of work).
-// A tile of fewer lanes still issues 128-lane MMAs - the tensor pipe idles here - and reads
-// whatever follows in shared memory; those accumulator lanes are never stored.  A load takes about
-// 3 us to land under load, so the rate of an SM is its bytes in flight over that time: a ring slot
-// takes as many k-blocks of the tile as fit, so that tiles of few lanes fill it too.
-template <int kOp_, int kCtaGroup_, int kCols_, int kStages_>
+// kSplit > 1: the streaming kernels, for groups of few rows, where the time is that of reading the
+// matrices once.  A cluster of kSplit CTAs shares a tile of 128 lanes: each takes an equal part of
+// the contraction, and at the end each collects the partial sums of 128 / kSplit lanes from the
+// others through distributed shared memory and adds them in rank order.  So the SMs' shares differ
+// by a fraction of a tile however many tiles there are (6 groups of 3584 rows are 168 tiles: in
+// whole tiles, two rounds on 148 SMs for 1.14 rounds of work).  Two ways of evening out the lanes
+// instead were slower: tiles of fewer lanes take as many k-blocks, each with its fixed cost, and
+// contiguous runs per SM scatter the addresses that are read at a time (32 groups of 3584 x 2048:
+// 102 us against 86).
+template <int kOp_, int kCtaGroup_, int kSplit_, int kCols_, int kStages_>
 struct GroupedConfig {
   static constexpr int kOp = kOp_;
   static constexpr int kCtaGroup = kCtaGroup_;
   static constexpr int kCols = kCols_;              // widest accumulator (UMMA N) of a tile
   static constexpr int kStages = kStages_;          // ring slots (streaming: at most)
-  static constexpr bool kStream = kCtaGroup == 1 && kOp != kGroupedDw;
-  static constexpr int kUnit = (kOp == kGroupedDx) ? 64 : 32;
+  static constexpr int kSplit = kSplit_;            // CTAs that share a tile's contraction
+  static constexpr bool kStream = kSplit > 1;
+  static constexpr int kCluster = kCtaGroup * kSplit;
   static constexpr int kLaneRows = 128;             // lanes per CTA
   static constexpr int kLaneTile = kLaneRows * kCtaGroup;
   static constexpr int kHalfCols = kCols / kCtaGroup;   // column rows a CTA fetches at most
@@ -93,8 +94,7 @@ struct GroupedConfig {
   static constexpr int kColBytes = kHalfCols * 128;
   // MXFP4: the instruction takes the scales of 128 rows from four columns of tensor memory that
   // start at a multiple of four, so lanes and columns start at multiples of 128 rows, the blocks in
-  // which the scales are stored.  A tile uses a part of its frame: rows outside are not fetched and
-  // their lanes or columns are not stored.
+  // which the scales are stored.  A group's first tile may use a part of its columns only.
   static constexpr int kScaleCols = (kCols + 127) / 128;      // blocks of scales of the columns
   static constexpr int kScaleBytes = (kOp == kMxNt) ? 1024 * (1 + kScaleCols) : 0;
   static constexpr int kStageBytes = kLaneBytes + kColBytes + kScaleBytes;
@@ -105,14 +105,16 @@ struct GroupedConfig {
   static constexpr int kAccs = (kOp == kMxNt && kCtaGroup == 2) ? 1 : 2;
   static constexpr int kEpiWarps = (kAccs == 1) ? 8 : 4;
   static constexpr int kEpiCols = kCols * 4 / kEpiWarps;   // columns that a warp stores at most
-  static constexpr int kEpiBytes = kEpiWarps * 2 * 2048;   // per warp two buffers of 32 x 32 bf16
+  // Per warp two buffers of 32 x 32 bf16; streaming: two buffers for the partial sums of 128 lanes
+  // x 16 columns in fp32 (from kSplit CTAs 128 / kSplit lanes each).
+  static constexpr int kPartCols = 16;
+  static constexpr int kPartBytes = 128 * kPartCols * 4;
+  static constexpr int kEpiBytes = kEpiWarps * 2 * 2048;
+  static_assert(!kStream || kEpiBytes >= 2 * kPartBytes, "partial sums");
   static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
-  static constexpr int kBarrierBytes = (3 * kStages + 4) * 8 + 16;
+  static constexpr int kBarrierBytes = (3 * kStages + 4 + 2 + 2 * kSplit) * 8 + 16;
   static constexpr int kRestBytes = kEpiBytes + kTableBytes + 12 + kBarrierBytes + 1024;
-  // The epilogue's buffers lie in front of the ring: an MMA of a tile that starts inside its frame
-  // reads from the frame's start, up to 12 KB in front of its slot.
   static constexpr int kRingBytes = kStream ? (232448 - kRestBytes) / 1024 * 1024 : kStages * kStageBytes;
-  static_assert(kOp != kMxNt || !kStream || kEpiBytes >= 96 * 128, "room in front of the ring");
   static_assert(kEpiBytes % 1024 == 0, "the ring starts on the swizzle's alignment");
   static constexpr int kSmemBytes = kRingBytes + kRestBytes;
   // The accumulators, and behind them (MXFP4) the scales of every k-block in the ring: per 128
@@ -138,14 +140,13 @@ struct GroupedConfig {
 struct GroupedTile {
   int group;
   int lane0;      // index on lane 0 of the tile
-  int lane_lo;    // first lane in use (streaming MXFP4: a multiple of kUnit; else 0)
-  int lane_rows;  // lanes in use per CTA (streaming: a multiple of kUnit)
   int col_row;    // row of the ragged operand (index of the column axis for dW) in column 0
   int lo, hi;     // columns that are this tile's to store
   int mma_n;      // columns computed: hi rounded up
   int k_row;      // kGroupedDw: first row of the contraction
   int k_len;      // contraction length
-  int blocks;     // k-blocks (0: the result is zero)
+  int first_kb;   // this CTA's k-blocks
+  int blocks;     // (0: its sum is zero)
 };
 
 __device__ __forceinline__ void report_error(int* status, volatile int* abort_flag, int code,
@@ -175,47 +176,34 @@ __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, 
 __device__ __forceinline__ void make_uniform(GroupedTile& t) {
   t.group = uniform(t.group);
   t.lane0 = uniform(t.lane0);
-  t.lane_lo = uniform(t.lane_lo);
-  t.lane_rows = uniform(t.lane_rows);
   t.col_row = uniform(t.col_row);
   t.lo = uniform(t.lo);
   t.hi = uniform(t.hi);
   t.mma_n = uniform(t.mma_n);
   t.k_row = uniform(t.k_row);
   t.k_len = uniform(t.k_len);
+  t.first_kb = uniform(t.first_kb);
   t.blocks = uniform(t.blocks);
 }
 
-// The tiles of one worker, in order.  Every role walks its own copy.
+// The tiles of one worker (a CTA, a pair, or a cluster that splits the contraction), in order.
+// Every role walks its own copy.
 template <class Cfg>
 struct GroupedTiles {
-  const int *begin, *end, *first;   // row ranges; first tile (streaming: first unit) of a group
+  const int *begin, *end, *first;   // row ranges, and the first tile of every group
   int next, last, step;
-  int worker, workers, units, round, height;   // streaming: all units; this round's start and tiles
+  int split_rank;
+  int group, g0, g1, tiles, share;  // the group of the last tile: its rows and its columns' tiles
+  int group_last;                   // first tile of the next group
 
   __device__ __forceinline__ GroupedTiles(const GroupedParams& p, const int* begin_, const int* end_,
-                                          const int* first_, int worker_, int workers_)
-      : begin(begin_), end(end_), first(first_), worker(worker_), workers(workers_) {
-    if (Cfg::kStream) {
-      units = first[p.groups];
-      round = height = next = last = 0;
-    } else {
-      next = worker;
-      last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : first[p.groups];
-      step = workers;
-    }
+                                          const int* first_, int worker, int workers, int split_rank_)
+      : begin(begin_), end(end_), first(first_), next(worker), step(workers), split_rank(split_rank_),
+        group_last(0) {
+    last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : first[p.groups];
   }
 
   __device__ __forceinline__ bool take(const GroupedParams& p, GroupedTile& t) {
-    if (Cfg::kStream && next >= last) {
-      // The next round: every worker takes as many units, side by side.
-      round += height * workers;
-      const int left = units - round;
-      constexpr int kMost = Cfg::kLaneRows / Cfg::kUnit;
-      height = left >= kMost * workers ? kMost : left >= 2 * workers ? 2 : 1;
-      next = round + worker * height;
-      last = min(next + height, units);
-    }
     if (next >= last) return false;
     if (Cfg::kOp == kGroupedDw) {
       const int per_group = p.lane_tiles * p.col_tiles;
@@ -223,125 +211,84 @@ struct GroupedTiles {
       const int local = next - t.group * per_group;
       const int lane_tile = local / p.col_tiles;
       t.lane0 = lane_tile * Cfg::kLaneTile;
-      t.lane_lo = 0;
-      t.lane_rows = Cfg::kLaneRows;
       t.col_row = (local - lane_tile * p.col_tiles) * Cfg::kCols;
       t.lo = 0;
       t.hi = min(Cfg::kCols, p.cols - t.col_row);
       t.k_row = begin[t.group];
       t.k_len = end[t.group] - t.k_row;
-      next += step;
     } else {
-      // Last group whose first tile is not behind this one: groups without tiles share their
-      // first tile with the next group and lose the comparison.
-      int a = 0, b = p.groups - 1;
-      while (a < b) {
-        const int m = (a + b + 1) >> 1;
-        if (first[m] <= next) a = m; else b = m - 1;
-      }
-      t.group = a;
-      const int g0 = begin[a], g1 = end[a];
-      const int tiles = column_tiles<Cfg>(p, g0, g1);
-      const int local = next - first[a];
-      int c;
-      if (Cfg::kStream) {
-        // Units along one lane axis, in tiles of 4, 2 or 1 of them (one box each).
-        c = local / p.lane_tiles;
-        const int unit = local - c * p.lane_tiles;
-        const int run = min(last - next, p.lane_tiles - unit);
-        constexpr int kMost = Cfg::kLaneRows / Cfg::kUnit;
-        int take = run;
-        t.lane_lo = 0;
-        if (Cfg::kOp == kMxNt) {   // inside its frame
-          t.lane_lo = unit % kMost * Cfg::kUnit;
-          take = min(run, kMost - unit % kMost);
+      if (next >= group_last) {
+        // Last group whose first tile is not behind this one: groups without tiles share their
+        // first tile with the next group and lose the comparison.
+        int a = 0, b = p.groups - 1;
+        while (a < b) {
+          const int m = (a + b + 1) >> 1;
+          if (first[m] <= next) a = m; else b = m - 1;
         }
-        take = take >= kMost ? kMost : take >= 2 ? 2 : 1;
-        t.lane0 = unit * Cfg::kUnit - t.lane_lo;
-        t.lane_rows = take * Cfg::kUnit;
-        next += take;
-      } else {
-        const int lane_tile = local / tiles;
-        c = local - lane_tile * tiles;
-        t.lane0 = lane_tile * Cfg::kLaneTile;
-        t.lane_lo = 0;
-        t.lane_rows = Cfg::kLaneRows;
-        next += step;
-      }
-      if (Cfg::kOp == kMxNt) {
-        t.col_row = g0 / 128 * 128 + c * Cfg::kCols;
-        t.lo = max(g0 - t.col_row, 0);
-        t.hi = min(g1 - t.col_row, Cfg::kCols);
-      } else {
+        group = a;
+        g0 = begin[a];
+        g1 = end[a];
+        group_last = first[a + 1];
+        tiles = column_tiles<Cfg>(p, g0, g1);
         // Equal shares of the columns, in steps of the MMA's granularity.
-        const int share = ((g1 - g0 + tiles - 1) / tiles + Cfg::kColStep - 1) / Cfg::kColStep *
-                          Cfg::kColStep;
-        t.col_row = g0 + c * share;
-        t.lo = 0;
-        t.hi = max(min(share, g1 - t.col_row), 0);
+        share = Cfg::kCols;
+        if (Cfg::kOp != kMxNt)
+          share = ((g1 - g0 + tiles - 1) / tiles + Cfg::kColStep - 1) / Cfg::kColStep * Cfg::kColStep;
       }
+      t.group = group;
+      const int local = next - first[group];
+      // Streaming: tiles that are read at a time lie side by side.
+      int c, lane_tile;
+      if (Cfg::kStream) {
+        c = local / p.lane_tiles;
+        lane_tile = local - c * p.lane_tiles;
+      } else {
+        lane_tile = local / tiles;
+        c = local - lane_tile * tiles;
+      }
+      t.lane0 = lane_tile * Cfg::kLaneTile;
+      t.col_row = (Cfg::kOp == kMxNt ? g0 / 128 * 128 : g0) + c * share;
+      t.lo = max(g0 - t.col_row, 0);
+      t.hi = max(min(g1 - t.col_row, share), 0);
       t.k_row = 0;
       t.k_len = p.depth;
     }
+    next += step;
     t.mma_n = max((t.hi + Cfg::kColStep - 1) / Cfg::kColStep, 1) * Cfg::kColStep;
-    t.blocks = (t.k_len + Cfg::kBlockK - 1) / Cfg::kBlockK;
+    const int blocks = (t.k_len + Cfg::kBlockK - 1) / Cfg::kBlockK;
+    t.first_kb = blocks * split_rank / Cfg::kSplit;
+    t.blocks = blocks * (split_rank + 1) / Cfg::kSplit - t.first_kb;
     return true;
   }
 };
 
-// A k-block of a tile: where its parts lie from its start (lanes, columns, scales), which rows of the
-// ragged operand it fetches, and how many k-blocks a ring slot takes.
+// What a k-block of a tile fetches of the ragged operand, and the block's size.
 template <class Cfg>
 struct BlockLayout {
   bool small;             // the columns in use lie in one small box; otherwise a large one from column 0
   int first_col;          // column of the box's first row
-  uint32_t lane_bytes, col_bytes, size;
-  uint32_t fetched;       // bytes that arrive
-  int per_slot;
+  uint32_t fetched;       // bytes of the whole block
 
   __device__ __forceinline__ BlockLayout(const GroupedParams& p, const GroupedTile& t, int rank) {
-    lane_bytes = Cfg::kLaneBytes;
-    col_bytes = Cfg::kColBytes;
     small = false;
     first_col = 0;
-    per_slot = 1;
     if (Cfg::kOp == kGroupedDw) {
       fetched = Cfg::kLaneBytes + (t.mma_n / Cfg::kCtaGroup + 63) / 64 * 8192;
     } else {
       const int half = t.mma_n / Cfg::kCtaGroup;
       const int lo = max(t.lo - rank * half, 0), hi = max(min(t.hi - rank * half, half), 1);
-      first_col = lo / p.small_box * p.small_box;
+      first_col = lo & ~(p.small_box - 1);
       small = hi - first_col <= p.small_box;
       if (!small) first_col = 0;
-      if (Cfg::kStream) {
-        lane_bytes = static_cast<uint32_t>(t.lane_rows) * 128;
-        col_bytes = static_cast<uint32_t>(small ? first_col + p.small_box : p.col_box) * 128;
-      }
-      fetched = lane_bytes + static_cast<uint32_t>(small ? p.small_box : p.col_box) * 128 +
-                Cfg::kScaleBytes;
+      fetched = Cfg::kLaneBytes + (small ? p.small_box : p.col_box) * 128 + Cfg::kScaleBytes;
     }
-    size = lane_bytes + col_bytes + Cfg::kScaleBytes;
-    if (Cfg::kStream) {
-      per_slot = p.slot_bytes / static_cast<int>(size);
-      if (Cfg::kOp == kMxNt) per_slot = min(per_slot, Cfg::kScaleSets / p.slots);
-    }
-  }
-
-  __device__ __forceinline__ void make_uniform() {
-    small = uniform(small) != 0;
-    first_col = uniform(first_col);
-    lane_bytes = uniform(lane_bytes);
-    col_bytes = uniform(col_bytes);
-    size = uniform(size);
-    fetched = uniform(fetched);
-    per_slot = uniform(per_slot);
   }
 };
 
-// Tensor maps of the operands, by box: lanes by 128, two units and one unit of rows (MN-major lanes:
-// 64 x 64), columns by col_box and small_box rows, scales (MXFP4) of the lanes and of the columns.
+// Tensor maps of the operands, by box: lanes (128 rows, MN-major lanes 64 x 64), columns (col_box and
+// small_box rows), scales (MXFP4) of the lanes and of the columns.
 struct GroupedMaps {
-  CUtensorMap lanes, two_units, unit, cols, small_cols, lane_scales, col_scales;
+  CUtensorMap lanes, cols, small_cols, lane_scales, col_scales;
 };
 
 template <class Cfg>
@@ -364,7 +311,9 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   const uint32_t clear_bar = empty_bar + 8 * kStages;        // [kStages] dW: last block has landed
   const uint32_t tmem_full_bar = clear_bar + 8 * kStages;    // [2]
   const uint32_t tmem_empty_bar = tmem_full_bar + 16;        // [2]
-  uint8_t* tail_gen = smem_gen + (tmem_empty_bar + 16 - smem_base);
+  const uint32_t part_full_bar = tmem_empty_bar + 16;        // [2] partial sums have arrived
+  const uint32_t part_free_bar = part_full_bar + 16;         // [kSplit][2] CTA d's buffer is free
+  uint8_t* tail_gen = smem_gen + (part_free_bar + 16 * Cfg::kSplit - smem_base);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail_gen);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_gen + 4);
   int* begin = reinterpret_cast<int*>(tail_gen + 16);        // [kMaxGroups]
@@ -373,10 +322,12 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
-  const int rank = (kCtaGroup == 2) ? uniform(static_cast<int>(cluster_ctarank())) : 0;
+  const int cluster_rank = (Cfg::kCluster > 1) ? uniform(static_cast<int>(cluster_ctarank())) : 0;
+  const int rank = (kCtaGroup == 2) ? cluster_rank : 0;          // in a pair
+  const int split_rank = (Cfg::kSplit > 1) ? cluster_rank : 0;   // along the contraction
   const bool is_leader = rank == 0;
-  const int worker = static_cast<int>(blockIdx.x) / kCtaGroup;
-  const int num_workers = static_cast<int>(gridDim.x) / kCtaGroup;
+  const int worker = static_cast<int>(blockIdx.x) / Cfg::kCluster;
+  const int num_workers = static_cast<int>(gridDim.x) / Cfg::kCluster;
 
   // ---------------------------------------------------------------- set-up
   if (threadIdx.x == 0) {
@@ -390,16 +341,14 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     for (int a = 0; a < 2; ++a) {
       mbar_init(tmem_full_bar + 8 * a, 1);
       mbar_init(tmem_empty_bar + 8 * a, Cfg::kEpiWarps * kCtaGroup);
+      mbar_init(part_full_bar + 8 * a, 4);   // four warps send to a CTA, whatever kSplit is
+      for (int d = 0; d < Cfg::kSplit; ++d) mbar_init(part_free_bar + 16 * d + 8 * a, 4);
     }
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0 && p.depth > 0) {   // without a contraction there are no maps
     prefetch_tensormap(&maps.lanes);
     prefetch_tensormap(&maps.cols);
-    if (Cfg::kStream && Cfg::kUnit < 64) {
-      prefetch_tensormap(&maps.two_units);
-      prefetch_tensormap(&maps.unit);
-    }
     if (!kDw) prefetch_tensormap(&maps.small_cols);
     if (kMx) {
       prefetch_tensormap(&maps.lane_scales);
@@ -439,7 +388,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     end[e] = static_cast<int>(f);
   }
   tcgen05_fence_before();
-  if (kCtaGroup == 2) cluster_sync_all(); else __syncthreads();
+  if (Cfg::kCluster > 1) cluster_sync_all(); else __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   if (kCtaGroup == 2 && tmem_base != 0 && threadIdx.x == 0)
@@ -461,10 +410,14 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     if (lane == 0) first_tile[p.groups] = sum;
   }
   __syncthreads();
-  GroupedTiles<Cfg> tiles(p, begin, end, first_tile, worker, num_workers);
+  GroupedTiles<Cfg> tiles(p, begin, end, first_tile, worker, num_workers, split_rank);
   GroupedTile t;
   int tile = 0;   // of this worker, for error records
-  const uint32_t slot_bytes = Cfg::kStream ? p.slot_bytes : Cfg::kStageBytes;
+  // Ring slots.  Streaming: sized for the widest tile of the launch, of one or two k-blocks.
+  const uint32_t col_bytes = Cfg::kStream ? p.col_box * 128 : Cfg::kColBytes;
+  const uint32_t block_bytes = Cfg::kLaneBytes + col_bytes + Cfg::kScaleBytes;
+  const int per_slot = Cfg::kStream ? p.per_slot : 1;
+  const uint32_t slot_bytes = block_bytes * per_slot;
   const uint32_t slots = Cfg::kStream ? p.slots : kStages;
 
   // ---------------------------------------------------------------- roles
@@ -477,33 +430,32 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     bool ok = true;
     for (; ok && tiles.take(p, t); ++tile) {
       make_uniform(t);
-      BlockLayout<Cfg> at(p, t, rank);
+      const BlockLayout<Cfg> at(p, t, rank);
+      const uint32_t fetched = uniform(at.fetched);
       uint32_t expected = at.fetched;   // by the leader of a pair: for both CTAs
       if (kCtaGroup == 2) expected += BlockLayout<Cfg>(p, t, 1 - rank).fetched;
       expected = uniform(expected);
-      at.make_uniform();
+      const bool small = uniform(at.small) != 0;
+      const int first_col = uniform(at.first_col);
       const int half = t.mma_n / kCtaGroup;
-      const int lane_row = t.lane0 + rank * Cfg::kLaneRows + t.lane_lo;
-      const int col_row = t.col_row + rank * half + at.first_col;
-      const CUtensorMap* map_l = &maps.lanes;
-      if (Cfg::kStream && Cfg::kUnit < 64 && t.lane_rows < Cfg::kLaneRows)
-        map_l = t.lane_rows == Cfg::kUnit ? &maps.unit : &maps.two_units;
-      const CUtensorMap* map_c = at.small ? &maps.small_cols : &maps.cols;
-      const uint32_t to_cols = at.lane_bytes + at.first_col * 128;
-      const uint32_t to_scales = at.lane_bytes + at.col_bytes;
+      const int lane_row = t.lane0 + rank * Cfg::kLaneRows;
+      const int col_row = t.col_row + rank * half + first_col;
+      const CUtensorMap* map_c = small ? &maps.small_cols : &maps.cols;
+      const uint32_t to_cols = Cfg::kLaneBytes + first_col * 128;
+      const uint32_t to_scales = Cfg::kLaneBytes + col_bytes;
       int scale_row = 0, col_scale_row = 0;
       if (kMx) {
         scale_row = (t.group * p.sf_row_blocks + lane_row / 128) * p.sf_k_blocks;
         col_scale_row = t.col_row / 128;
       }
-      for (int kb0 = 0; kb0 < t.blocks; kb0 += at.per_slot) {
+      for (int kb0 = 0; kb0 < t.blocks; kb0 += per_slot) {
         ok = __all_sync(0xffffffffu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, abort_flag));
         if (!ok) {
           if (lane == 0)
             report_error(p.status, abort_flag, kDevTimeoutProducer, tile, static_cast<int>(stage));
           break;
         }
-        const int blocks = Cfg::kStream ? min(at.per_slot, t.blocks - kb0) : 1;
+        const int blocks = Cfg::kStream ? min(per_slot, t.blocks - kb0) : 1;
         uint32_t sl = ring + stage * slot_bytes;
         // dW: the last block of a group's rows is handed over by the warp that clears its tail.
         const bool clear = kDw && t.k_len - kb0 * 64 < 64;
@@ -511,7 +463,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         const uint32_t bar = (kCtaGroup == 1 || clear) ? own : leader_full + 8 * stage;
         if (elect_one()) {
           if (kCtaGroup == 1 || clear) {
-            mbar_arrive_expect_tx(own, at.fetched * blocks);
+            mbar_arrive_expect_tx(own, fetched * blocks);
           } else if (is_leader) {
             mbar_arrive_expect_tx(own, expected);
             if (kDw) mbar_arrive(own);
@@ -520,8 +472,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         __syncwarp();
         // Everything a copy needs is worked out outside the elected lane's branch, where the warp's
         // uniform registers hold it: 17 cycles a copy, against about 95 inside.
-        for (int j = 0; j < blocks; ++j, sl += at.size) {
-          const int kb = kb0 + j;
+        for (int j = 0; j < blocks; ++j, sl += block_bytes) {
+          const int kb = t.first_kb + kb0 + j;
           const uint32_t sc = sl + to_cols, ss = sl + to_scales;
           const int k0 = kb * (kMx ? 128 : 64);   // first element (MXFP4: byte) of the block
           const int row = t.k_row + k0;
@@ -540,10 +492,9 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             } else {
               if constexpr (Cfg::kOp == kGroupedDx) {
                 load(sl, &maps.lanes, lane_row, k0, t.group);
-                if (!Cfg::kStream || t.lane_rows > 64)
-                  load(sl + 8192, &maps.lanes, lane_row + 64, k0, t.group);
+                load(sl + 8192, &maps.lanes, lane_row + 64, k0, t.group);
               } else {
-                load(sl, map_l, k0, lane_row, t.group);
+                load(sl, &maps.lanes, k0, lane_row, t.group);
               }
               load(sc, map_c, k0, col_row, 0);
               if constexpr (kMx) {
@@ -578,15 +529,13 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           break;
         }
         tcgen05_fence_after();
-        BlockLayout<Cfg> at(p, t, rank);
-        at.make_uniform();
         const uint32_t tmem_d = tmem_base + acc * Cfg::kCols;
         const uint32_t idesc =
             kMx ? make_idesc_mxf4(Cfg::kLaneTile, static_cast<uint32_t>(t.mma_n))
                 : make_idesc_bf16(Cfg::kLaneTile, static_cast<uint32_t>(t.mma_n)) |
                       (Cfg::kOp == kGroupedDx ? kIdescTransposeA : 0u) |
                       (kDw ? kIdescTransposeA | kIdescTransposeB : 0u);
-        for (int kb0 = 0; kb0 < t.blocks; kb0 += at.per_slot) {
+        for (int kb0 = 0; kb0 < t.blocks; kb0 += per_slot) {
           if (!__all_sync(0xffffffffu,
                           mbar_wait<kDw && kCtaGroup == 2>(full_bar + 8 * stage, phase, abort_flag))) {
             if (lane == 0)
@@ -595,27 +544,26 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             break;
           }
           tcgen05_fence_after();
-          const int blocks = Cfg::kStream ? min(at.per_slot, t.blocks - kb0) : 1;
+          const int blocks = Cfg::kStream ? min(per_slot, t.blocks - kb0) : 1;
           uint32_t sl = ring + stage * slot_bytes;
-          for (int j = 0; j < blocks; ++j, sl += at.size) {
-            const int kb = kb0 + j;
-            const uint32_t sc = sl + at.lane_bytes;
+          for (int j = 0; j < blocks; ++j, sl += block_bytes) {
+            const int kb = t.first_kb + kb0 + j;
+            const uint32_t sc = sl + Cfg::kLaneBytes;
             // A K-major operand moves 32 bytes along its swizzled rows per step, an MN-major one two
             // groups of eight rows.
             constexpr uint64_t kLaneStep = (kDw || Cfg::kOp == kGroupedDx) ? 128 : 2;
             constexpr uint64_t kColStepDesc = kDw ? 128 : 2;
-            // MXFP4: lane 0 of the frame lies in front of the tile's first fetched row.
             const uint64_t dl = (kLaneStep == 128) ? make_smem_desc_mn_sw128(sl, 8192)
-                                                   : make_smem_desc_sw128(sl - t.lane_lo * 128);
+                                                   : make_smem_desc_sw128(sl);
             const uint64_t dc = kDw ? make_smem_desc_mn_sw128(sc, 8192) : make_smem_desc_sw128(sc);
             const int left = t.k_len - kb * Cfg::kBlockK;
-            const uint32_t first = kb > 0 ? 1u : 0u;
+            const uint32_t first = kb0 + j > 0 ? 1u : 0u;
             if constexpr (kMx) {
               // Scales of 128 values of K: four columns of tensor memory per block of 128 rows.
               const uint32_t set = Cfg::kStream ? stage * sets_per_slot + j : stage;
               const uint32_t tsl = tmem_base + Cfg::kAccs * Cfg::kCols + set * Cfg::kScaleTmemCols;
               const uint32_t tsc = tsl + 8;
-              const uint64_t ds = make_smem_desc_scales(sc + at.col_bytes);
+              const uint64_t ds = make_smem_desc_scales(sc + col_bytes);
               if (elect_one()) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -677,6 +625,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     const uint32_t stage_buf = epi_base + (warp - 2) * 4096;
     uint32_t buf = 0;
     int count = 0;
+    int parts = 0;   // column groups of partial sums so far
     for (; tiles.take(p, t); ++tile) {
       const uint32_t acc = count % Cfg::kAccs, acc_phase = (count / Cfg::kAccs) & 1;
       if (t.blocks > 0) {
@@ -689,8 +638,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         tcgen05_fence_after();
       }
       const int lane_first = t.lane0 + rank * Cfg::kLaneRows + quad * 32;   // of this warp
-      const int lane_end = min(p.lanes, t.lane0 + rank * Cfg::kLaneRows + t.lane_lo + t.lane_rows);
-      const bool lanes_in_use = lane_first < lane_end && quad * 32 + 32 > t.lane_lo;
+      const int lane_end = p.lanes;
       // 32 columns of this warp's lanes, rounded to bf16 and packed in pairs.
       auto pull = [&](int c, uint32_t (&w)[16]) {
         if (t.blocks > 0) {
@@ -765,8 +713,83 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           }
         }
       };
-      auto in_use = [&](int c) { return lanes_in_use && c < t.hi && c + 32 > t.lo; };
-      if constexpr (Cfg::kAccs == 1) {
+      auto in_use = [&](int c) { return lane_first < lane_end && c < t.hi && c + 32 > t.lo; };
+      if constexpr (Cfg::kSplit > 1) {
+        // Partial sums, kPartCols columns at a time: this warp's lanes go to the CTA that collects
+        // them, [source][four columns][lane][4]; then this warp adds up four columns of the lanes
+        // that its own CTA collects.  The next columns are on their way meanwhile.
+        constexpr int kSplit = Cfg::kSplit, kOwn = 128 / kSplit;   // lanes that a CTA collects
+        constexpr uint32_t kSource = kOwn * Cfg::kPartCols * 4;
+        const uint32_t dest = quad * kSplit / 4;
+        const uint32_t dest_lane = (quad * 32) % kOwn + lane;
+        const uint32_t dest_base = mapa_u32(epi_base, dest) + split_rank * kSource + dest_lane * 16;
+        const uint32_t dest_full = mapa_u32(part_full_bar, dest);
+        const int c_first = t.lo & ~(Cfg::kPartCols - 1);
+        bool ok = true;
+        auto send = [&](int c, int n) {
+          uint32_t r[16];
+          if (t.blocks > 0) {
+            tmem_ld_32x32b_x16(tmem_base + acc * Cfg::kCols + lane_base + c, r);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = 0u;
+          }
+          const uint32_t b = n & 1;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait<true>(part_free_bar + 16 * dest + 8 * b,
+                                                             ((n >> 1) & 1) ^ 1, abort_flag));
+          if (!ok) return;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            st_cluster_v4(dest_base + b * Cfg::kPartBytes + j * (kOwn * 16), r[4 * j], r[4 * j + 1],
+                          r[4 * j + 2], r[4 * j + 3]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_release_cluster(dest_full + 8 * b);
+        };
+        auto collect = [&](int c, int n) {
+          const uint32_t b = n & 1;
+          ok = ok && __all_sync(0xffffffffu,
+                                mbar_wait<true>(part_full_bar + 8 * b, (n >> 1) & 1, abort_flag));
+          if (!ok) return;
+          float sum[kOwn / 32][4];
+#pragma unroll
+          for (int h = 0; h < kOwn / 32; ++h) {
+            const uint32_t at = epi_base + b * Cfg::kPartBytes + (quad * kOwn + h * 32 + lane) * 16;
+#pragma unroll
+            for (int q = 0; q < kSplit; ++q) {
+              uint32_t v[4];
+              ld_shared_v4(at + q * kSource, v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                sum[h][j] = q == 0 ? __uint_as_float(v[j]) : sum[h][j] + __uint_as_float(v[j]);
+            }
+          }
+          __syncwarp();
+          if (lane < kSplit)
+            mbar_arrive_release_cluster(mapa_u32(part_free_bar + 16 * split_rank + 8 * b, lane));
+#pragma unroll
+          for (int h = 0; h < kOwn / 32; ++h) {
+            const int n_out = t.lane0 + split_rank * kOwn + h * 32 + static_cast<int>(lane);
+            const int row = c + quad * 4;
+            __nv_bfloat16* dst = p.out + static_cast<long long>(t.col_row + row) * p.out_pitch + n_out;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (row + j >= t.lo && row + j < t.hi && n_out < p.lanes)
+                dst[j * p.out_pitch] = __float2bfloat16_rn(sum[h][j]);
+          }
+        };
+        send(c_first, parts);
+        for (int c = c_first; c < t.hi; c += Cfg::kPartCols) {
+          const int n = parts++;
+          if (c + Cfg::kPartCols < t.hi) send(c + Cfg::kPartCols, n + 1);
+          else hand_back();   // all of the accumulator has been read
+          collect(c, n);
+        }
+        if (!ok) {
+          if (lane == 0) report_error(p.status, abort_flag, kDevTimeoutEpilogue, tile, 2);
+          break;
+        }
+      } else if constexpr (Cfg::kAccs == 1) {
         uint32_t w[Cfg::kEpiCols / 32][16];
 #pragma unroll
         for (int i = 0; i < Cfg::kEpiCols / 32; ++i)
@@ -837,13 +860,13 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
 
   // ---------------------------------------------------------------- tear-down
   tcgen05_fence_before();
-  if (kCtaGroup == 2) cluster_sync_all(); else __syncthreads();
+  if (Cfg::kCluster > 1) cluster_sync_all(); else __syncthreads();
   if (*abort_flag != 0) {
     // Let boxes still in flight land in this CTA's shared memory before it is released.
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
   }
-  if (kCtaGroup == 2) cluster_sync_all(); else __syncthreads();
+  if (Cfg::kCluster > 1) cluster_sync_all(); else __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
     tmem_dealloc<1>(tmem_base, Cfg::kTmemCols);

@@ -174,9 +174,10 @@ int neogemm_noalloc_clear_status(void);
  * multiples of 8; results may have any leading dimension (16-byte stores need multiples of 8).
  * T, N, K >= 0; an empty group is allowed (its dW is zero).  1 <= groups <= 1024 (0 groups: no-op).
  * zero_rest != 0 writes zeros to the rows of Y or dX that belong to no group (in front of offsets[0],
- * behind offsets[groups]); 0 leaves them as they are.  The sums of a row do not depend on the
- * other rows, and no atomics are used: results are the same bits from call to call.
- * No workspace; no counterpart in the reference. */
+ * behind offsets[groups]); 0 leaves them as they are.  Sums are added in a fixed order, without
+ * atomics: a call's result is the same bits each time.  (The order of a row's sum follows from the
+ * kernel, which is chosen from T / groups: a row alone and in a large batch may differ in the last
+ * bit.)  No workspace; no counterpart in the reference. */
 int neogemm_grouped_nt(const void* X, const void* W, void* Y, const void* offsets,
                        int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
                        int64_t ldx, int64_t ldw, int64_t stack_w, int64_t ldy, int zero_rest,
@@ -318,8 +319,8 @@ int neogemm_set_override(int cta_group, int block_n, int swap, int stream_k, int
  *          only publishes fp32 partials and a reduction kernel launched right behind it sums
  *          them, applies the epilogue and stores C; 0: wide tiles are not cut at all and the
  *          last contributor of a cut narrow tile sums it alone (the earlier behaviour).
- *   key 13: tiles of the grouped and MXFP4 products: -1 chosen from the average group, 0 narrow
- *          (one CTA), 1 wide.
+ *   key 13: kernels of the grouped and MXFP4 products: -1 chosen from the average rows of a group,
+ *          0 contraction split over four CTAs, 1 wide tiles on CTA pairs, 2 split over two CTAs.
  *   key 12: 128 x 64 tiles for small problems (twice as many CTAs as 128 x 128 tiles): -1 when
  *          the 128 x 128 tiles would occupy at most half of the SMs, 0 never, 1 whenever the
  *          single-CTA 128 x 128 TMA-store kernel would be used.

@@ -65,11 +65,11 @@ def call(op, x, w, dy, offsets, out=None):
     return ops.grouped_matmul_dw(dy, x, offsets, out=out)
 
 
-@pytest.fixture(params=[-1, 0, 1], ids=["auto", "narrow", "wide"])
+@pytest.fixture(params=[-1, 0, 2, 1], ids=["auto", "narrow", "middle", "wide"])
 def tiles(request):
-    ops.set_tuning("grouped_wide_tiles", request.param)
+    ops.set_tuning("grouped_kernel", request.param)
     yield request.param
-    ops.set_tuning("grouped_wide_tiles", -1)
+    ops.set_tuning("grouped_kernel", -1)
 
 
 COUNTS = {
@@ -182,7 +182,7 @@ def test_lengths_of_zero(op, tiles):
         assert (got == 0).all() and got.numel() == (80, 120)[("nt", "dx").index(op)]
 
 
-def test_results_are_the_same_bits_each_time_and_rows_do_not_depend_on_others():
+def test_results_are_the_same_bits_each_time_and_one_kernel_treats_rows_alike(tiles):
     counts, N, K = [100, 28, 0, 64], 512, 776
     x, w, dy = make(counts, N, K)
     _, off = offsets_of(counts)
@@ -190,8 +190,10 @@ def test_results_are_the_same_bits_each_time_and_rows_do_not_depend_on_others():
         a = call(op, x, w, dy, off)
         for _ in range(3):
             assert torch.equal(a, call(op, x, w, dy, off))
-    alone = ops.grouped_matmul(x[100:101], w[1:2], torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
-    assert torch.equal(alone[0], ops.grouped_matmul(x, w, off)[100])
+    if tiles >= 0:
+        one = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+        alone = ops.grouped_matmul(x[100:101], w[1:2], one)
+        assert torch.equal(alone[0], ops.grouped_matmul(x, w, off)[100])
 
 
 def test_a_captured_graph_replays_with_other_groups_beside_eager_calls():

@@ -61,11 +61,11 @@ def assert_product(got, want, mag, K):
     assert ops.device_status()[0] == 0
 
 
-@pytest.fixture(params=[-1, 0, 1], ids=["auto", "narrow", "wide"])
+@pytest.fixture(params=[-1, 0, 2, 1], ids=["auto", "narrow", "middle", "wide"])
 def tiles(request):
-    ops.set_tuning("grouped_wide_tiles", request.param)
+    ops.set_tuning("grouped_kernel", request.param)
     yield request.param
-    ops.set_tuning("grouped_wide_tiles", -1)
+    ops.set_tuning("grouped_kernel", -1)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
