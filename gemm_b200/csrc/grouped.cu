@@ -42,7 +42,7 @@ const KernelEntry kKernels[4][kVariants] = {
      make_entry<GroupedConfig<kGroupedNt, 1, 2, 128, 8>>()},
     {make_entry<GroupedConfig<kGroupedDx, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 1, 256, 6>>(),
      make_entry<GroupedConfig<kGroupedDx, 1, 2, 128, 8>>()},
-    {make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 1, 256, 6>>(),
+    {make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 1, 256, 5>>(),
      make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 6>>()},
     {make_entry<GroupedConfig<kMxNt, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 2, 1, 256, 5>>(),
      make_entry<GroupedConfig<kMxNt, 1, 2, 128, 8>>()},
@@ -199,16 +199,29 @@ int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, Gr
   return NEOGEMM_OK;
 }
 
-// Variant for an average of `rows` rows per group: CTA pairs with 256 x 256 tiles from kWideRows on;
-// below, the contraction is split over two CTAs, or over four where the columns of a tile are few and
-// their partial sums quickly exchanged.
-constexpr int64_t kWideRows = 96;
-constexpr int64_t kMiddleRows = 8;
-
-int variant_of(int64_t rows) {
+// Which kernel serves a product, from the average rows of a group (the groups themselves are known to
+// the GPU only).  Measured, us, four-way / two-way split / pairs:
+//   bf16, 32 groups of 3584 x 2048:  2 rows a group 56.7 57.6 60.1   32: 81.4 83.2 81.8   128: 148 115 91
+//   dX, the same groups:             2: 57.0 58.8 62.0               16: 75.7 74.8 74.7   64: 87.6 83.4 79.2
+//   MXFP4, the same groups:          0.25: 11.0 8.8 9.5              4: 32.0 24.6 24.9    16: 44.2 29.9 26.3
+//   MXFP4, one matrix 28672 x 8192:  16: 23.3 26.5 26.8              64: 26.1 30.7 28.2   128: 38.4 36.2 30.3
+// MXFP4 tiles of several groups reach over the batch's frame of 128 rows, so the pairs pay off from
+// 8 rows a group on; a single matrix has no such waste.  Pairs need tiles to go round, though: with
+// at most 16 of them and a long contraction its split wins (512 x 1024 x 8192 in MXFP4: 10.6 against
+// 15.5).  Below, the four-way split is taken where each CTA still has several k-blocks of a tile, or
+// where there is at most about one tile per cluster (8 groups of 1024 x 1024, 2 rows: 5.7 6.5 7.7).
+int variant_of(int op, int64_t groups, int64_t T, int64_t lanes, int64_t depth) {
   const int forced = tuning_value(13);
   if (forced >= 0) return forced;
-  return rows >= kWideRows ? kWide : rows >= kMiddleRows ? kMiddle : kNarrow;
+  const bool mx = op == kMxNt;
+  const int64_t blocks = ceil_div(depth, mx ? 256 : 64), rows = T / groups;
+  const int64_t wide_from = mx ? (groups == 1 ? 96 : 8) : op == kGroupedDx ? 16 : 32;
+  if (rows >= wide_from) {
+    const int64_t tiles = ceil_div(lanes, 256) * (groups == 1 ? ceil_div(T, 256) : groups);
+    if (tiles > 16 || blocks < 16 || rows > 1024) return kWide;
+  }
+  const int64_t tiles = ceil_div(lanes, 128) * std::min(groups, T);
+  return blocks >= (mx ? 16 : 24) || tiles <= 40 ? kNarrow : kMiddle;
 }
 
 // Y or dX: rows of the batch in, rows out.
@@ -234,7 +247,7 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  const KernelEntry& k = kKernels[op][variant_of(T / groups)];
+  const KernelEntry& k = kKernels[op][variant_of(op, groups, T, lanes, depth)];
   GroupedParams p;
   std::memset(&p, 0, sizeof(p));
   p.offsets = offsets;
@@ -291,7 +304,7 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
   int rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  const KernelEntry& k = kKernels[kMxNt][variant_of(T / groups)];
+  const KernelEntry& k = kKernels[kMxNt][variant_of(kMxNt, groups, T, N, K)];
   const int64_t k_tiles = ceil_div(K, 128), w_tiles = ceil_div(N, 128), x_tiles = ceil_div(T, 128);
   if (groups * w_tiles * k_tiles > kMaxExtent || x_tiles * k_tiles > kMaxExtent)
     return NEOGEMM_ERR_UNSUPPORTED;
@@ -367,7 +380,8 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  // The pair's tiles are 256 x 256 of a group's matrix whatever its rows.
+  // The pair's tiles are 256 x 256 of a group's matrix whatever its rows (513 rows over 8 groups,
+  // 1024 x 2048: 14.2 us, single CTAs 14.0; 16384 rows, 4096 x 4096: 390 and 480).
   const int forced = tuning_value(13);
   const bool wide = forced >= 0 ? forced == kWide : N >= 256 && K >= 256;
   const KernelEntry& k = kKernels[kGroupedDw][wide ? kWide : kNarrow];

@@ -103,7 +103,8 @@ struct GroupedConfig {
   // bound by shared memory - 256 x 128 reads and fills 192 bytes per cycle of the 128 there are - and
   // its eight epilogue warps pull the accumulator into registers, packed, before they store anything.
   static constexpr int kAccs = (kOp == kMxNt && kCtaGroup == 2) ? 1 : 2;
-  static constexpr int kEpiWarps = (kAccs == 1) ? 8 : 4;
+  // dW of short groups is bound by writing the result: eight warps there, too.
+  static constexpr int kEpiWarps = (kAccs == 1 || (kOp == kGroupedDw && kCtaGroup == 2)) ? 8 : 4;
   static constexpr int kEpiCols = kCols * 4 / kEpiWarps;   // columns that a warp stores at most
   // Per warp two buffers of 32 x 32 bf16; streaming: two buffers for the partial sums of 128 lanes
   // x 16 columns in fp32 (from kSplit CTAs 128 / kSplit lanes each).
@@ -164,13 +165,15 @@ __device__ __forceinline__ void report_error(int* status, volatile int* abort_fl
 template <class Cfg>
 __device__ __forceinline__ int column_tiles(const GroupedParams& p, int begin, int end) {
   if (end <= begin) return 0;
+  if (Cfg::kOp != kMxNt && end - begin <= p.col_cap) return 1;
   if (Cfg::kOp == kMxNt) return (end - begin / 128 * 128 + Cfg::kCols - 1) / Cfg::kCols;
   return (end - begin + p.col_cap - 1) / p.col_cap;
 }
 
-// The copy and matrix instructions take their operands from the warp's uniform registers: a value
-// that the compiler cannot prove uniform costs a transfer each time it is used.  One that came from
-// shared memory is made so once.
+// The copy and matrix instructions take their operands from the warp's uniform registers.  A value
+// that the compiler cannot prove uniform, or one in a branch or loop that it cannot, is moved there
+// each time it is used: about 90 cycles a copy instead of 17.  So whatever came from shared memory or
+// from the thread's index is made uniform once, the conditions of the roles' loops included.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 __device__ __forceinline__ void make_uniform(GroupedTile& t) {
@@ -200,7 +203,7 @@ struct GroupedTiles {
                                           const int* first_, int worker, int workers, int split_rank_)
       : begin(begin_), end(end_), first(first_), next(worker), step(workers), split_rank(split_rank_),
         group_last(0) {
-    last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : first[p.groups];
+    last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : uniform(first[p.groups]);
   }
 
   __device__ __forceinline__ bool take(const GroupedParams& p, GroupedTile& t) {
@@ -219,12 +222,15 @@ struct GroupedTiles {
     } else {
       if (next >= group_last) {
         // Last group whose first tile is not behind this one: groups without tiles share their
-        // first tile with the next group and lose the comparison.
-        int a = 0, b = p.groups - 1;
-        while (a < b) {
-          const int m = (a + b + 1) >> 1;
-          if (first[m] <= next) a = m; else b = m - 1;
-        }
+        // first tile with the next group and lose the comparison.  The warp looks at every 32nd
+        // group, then at the 32 from there (bisection cost 500 cycles a tile in each role).
+        const int lane = static_cast<int>(ptx::lane_id());
+        int a = 0;
+        if (p.groups > 32)
+          a = 32 * (__popc(__ballot_sync(0xffffffffu, lane * 32 < p.groups &&
+                                                          first[min(lane * 32, p.groups)] <= next)) - 1);
+        a += __popc(__ballot_sync(0xffffffffu, a + lane < p.groups &&
+                                                   first[min(a + lane, p.groups)] <= next)) - 1;
         group = a;
         g0 = begin[a];
         g1 = end[a];
@@ -233,17 +239,18 @@ struct GroupedTiles {
         // Equal shares of the columns, in steps of the MMA's granularity.
         share = Cfg::kCols;
         if (Cfg::kOp != kMxNt)
-          share = ((g1 - g0 + tiles - 1) / tiles + Cfg::kColStep - 1) / Cfg::kColStep * Cfg::kColStep;
+          share = ((tiles == 1 ? g1 - g0 : (g1 - g0 + tiles - 1) / tiles) + Cfg::kColStep - 1) /
+                  Cfg::kColStep * Cfg::kColStep;
       }
       t.group = group;
       const int local = next - first[group];
       // Streaming: tiles that are read at a time lie side by side.
       int c, lane_tile;
       if (Cfg::kStream) {
-        c = local / p.lane_tiles;
+        c = local < p.lane_tiles ? 0 : local / p.lane_tiles;
         lane_tile = local - c * p.lane_tiles;
       } else {
-        lane_tile = local / tiles;
+        lane_tile = tiles == 1 ? local : local / tiles;
         c = local - lane_tile * tiles;
       }
       t.lane0 = lane_tile * Cfg::kLaneTile;
@@ -320,7 +327,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   int* end = begin + kMaxGroups;                             // [kMaxGroups]
   int* first_tile = end + kMaxGroups;                        // [kMaxGroups + 1]
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform(static_cast<int>(threadIdx.x >> 5));
   const uint32_t lane = lane_id();
   const int cluster_rank = (Cfg::kCluster > 1) ? uniform(static_cast<int>(cluster_ctarank())) : 0;
   const int rank = (kCtaGroup == 2) ? cluster_rank : 0;          // in a pair
@@ -341,10 +348,12 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     for (int a = 0; a < 2; ++a) {
       mbar_init(tmem_full_bar + 8 * a, 1);
       mbar_init(tmem_empty_bar + 8 * a, Cfg::kEpiWarps * kCtaGroup);
-      mbar_init(part_full_bar + 8 * a, 4);   // four warps send to a CTA, whatever kSplit is
+      mbar_init(part_full_bar + 8 * a, 1);
       for (int d = 0; d < Cfg::kSplit; ++d) mbar_init(part_free_bar + 16 * d + 8 * a, 4);
     }
     fence_barrier_init();
+    if (Cfg::kSplit > 1)
+      for (int a = 0; a < 2; ++a) mbar_arrive_expect_tx(part_full_bar + 8 * a, Cfg::kPartBytes);
   }
   if (warp == 0 && lane == 0 && p.depth > 0) {   // without a contraction there are no maps
     prefetch_tensormap(&maps.lanes);
@@ -421,7 +430,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   const uint32_t slots = Cfg::kStream ? p.slots : kStages;
 
   // ---------------------------------------------------------------- roles
-  if (*abort_flag != 0) {
+  if (uniform(*abort_flag) != 0) {
     // The tensor-memory address check failed: nothing is issued.
   } else if (warp == 0) {
     // ======================= TMA producer =======================
@@ -639,18 +648,31 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       }
       const int lane_first = t.lane0 + rank * Cfg::kLaneRows + quad * 32;   // of this warp
       const int lane_end = p.lanes;
-      // 32 columns of this warp's lanes, rounded to bf16 and packed in pairs.
-      auto pull = [&](int c, uint32_t (&w)[16]) {
+      const int cols_end = min(t.hi, first_col + Cfg::kEpiCols);   // of this warp
+      auto in_use = [&](int c) { return lane_first < lane_end && c < cols_end && c + 32 > t.lo; };
+      // Up to four times 32 columns of this warp's lanes from `c`, rounded to bf16 and packed in
+      // pairs: two loads are issued before the first is waited for.
+      auto pull = [&](int c, uint32_t (&w)[4][16]) {
         if (t.blocks > 0) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(tmem_base + acc * Cfg::kCols + lane_base + c, r);
-          tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            w[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+          for (int h = 0; h < 4; h += 2) {
+            uint32_t r[2][32];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (in_use(c + (h + i) * 32))
+                tmem_ld_32x32b_x32(tmem_base + acc * Cfg::kCols + lane_base + c + (h + i) * 32, r[i]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                w[h + i][j] = pack_bf16x2(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1]));
+          }
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = 0u;
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[i][j] = 0u;
         }
       };
       auto hand_back = [&] {
@@ -713,7 +735,6 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           }
         }
       };
-      auto in_use = [&](int c) { return lane_first < lane_end && c < t.hi && c + 32 > t.lo; };
       if constexpr (Cfg::kSplit > 1) {
         // Partial sums, kPartCols columns at a time: this warp's lanes go to the CTA that collects
         // them, [source][four columns][lane][4]; then this warp adds up four columns of the lanes
@@ -736,21 +757,22 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             for (int j = 0; j < 16; ++j) r[j] = 0u;
           }
           const uint32_t b = n & 1;
-          ok = ok && __all_sync(0xffffffffu, mbar_wait<true>(part_free_bar + 16 * dest + 8 * b,
-                                                             ((n >> 1) & 1) ^ 1, abort_flag));
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(part_free_bar + 16 * dest + 8 * b,
+                                                       ((n >> 1) & 1) ^ 1, abort_flag));
           if (!ok) return;
+          // (Ordinary stores and a release at cluster scope took 1500 cycles: the release waits for
+          // every store in flight, those of the result included.)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            st_cluster_v4(dest_base + b * Cfg::kPartBytes + j * (kOwn * 16), r[4 * j], r[4 * j + 1],
-                          r[4 * j + 2], r[4 * j + 3]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive_release_cluster(dest_full + 8 * b);
+            st_async_v4(dest_base + b * Cfg::kPartBytes + j * (kOwn * 16), dest_full + 8 * b, r[4 * j],
+                        r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
         };
         auto collect = [&](int c, int n) {
           const uint32_t b = n & 1;
-          ok = ok && __all_sync(0xffffffffu,
-                                mbar_wait<true>(part_full_bar + 8 * b, (n >> 1) & 1, abort_flag));
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(part_full_bar + 8 * b, (n >> 1) & 1, abort_flag));
           if (!ok) return;
+          // Arm the buffer for its next use: nothing can arrive before this warp frees it below.
+          if (quad == 0 && lane == 0) mbar_arrive_expect_tx(part_full_bar + 8 * b, Cfg::kPartBytes);
           float sum[kOwn / 32][4];
 #pragma unroll
           for (int h = 0; h < kOwn / 32; ++h) {
@@ -766,7 +788,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           }
           __syncwarp();
           if (lane < kSplit)
-            mbar_arrive_release_cluster(mapa_u32(part_free_bar + 16 * split_rank + 8 * b, lane));
+            mbar_arrive_cluster(mapa_u32(part_free_bar + 16 * split_rank + 8 * b, lane));
 #pragma unroll
           for (int h = 0; h < kOwn / 32; ++h) {
             const int n_out = t.lane0 + split_rank * kOwn + h * 32 + static_cast<int>(lane);
@@ -789,22 +811,22 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           if (lane == 0) report_error(p.status, abort_flag, kDevTimeoutEpilogue, tile, 2);
           break;
         }
-      } else if constexpr (Cfg::kAccs == 1) {
-        uint32_t w[Cfg::kEpiCols / 32][16];
-#pragma unroll
-        for (int i = 0; i < Cfg::kEpiCols / 32; ++i)
-          if (in_use(first_col + i * 32)) pull(first_col + i * 32, w[i]);
-        hand_back();
-#pragma unroll
-        for (int i = 0; i < Cfg::kEpiCols / 32; ++i)
-          if (in_use(first_col + i * 32)) store(first_col + i * 32, w[i]);
       } else {
-        for (int c = t.lo & ~31; in_use(c); c += 32) {
-          uint32_t w[16];
+        // 128 columns at a time; the accumulator goes back once the last of them are in registers.
+        bool held = true;
+        const int c_first = max(first_col, t.lo & ~31);
+        for (int c = c_first; in_use(c); c += 128) {
+          uint32_t w[4][16];
           pull(c, w);
-          store(c, w);
+          if (c + 128 >= cols_end) {
+            hand_back();
+            held = false;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (in_use(c + i * 32)) store(c + i * 32, w[i]);
         }
-        hand_back();
+        if (held) hand_back();
       }
     }
     if (!kDw && p.zero_rest) {

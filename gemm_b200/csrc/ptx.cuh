@@ -591,11 +591,13 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
                "r"(d) : "memory");
 }
 
-// The same into the shared memory of any CTA of the cluster (an address from mapa_u32).
-__device__ __forceinline__ void st_cluster_v4(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t c,
-                                              uint32_t d) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(a), "r"(b),
-               "r"(c), "r"(d) : "memory");
+// Asynchronous store of 16 bytes into the shared memory of a CTA of the cluster; they are counted on
+// `cluster_bar`, a barrier of that CTA.  No fence of the sender's other stores is involved.
+__device__ __forceinline__ void st_async_v4(uint32_t cluster_addr, uint32_t cluster_bar, uint32_t a,
+                                            uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%2, %3, %4, %5}, [%1];"
+      ::"r"(cluster_addr), "r"(cluster_bar), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 __device__ __forceinline__ void st_shared_b16(uint32_t addr, unsigned short v) {
