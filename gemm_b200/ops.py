@@ -12,6 +12,9 @@ torch is used here for device memory and streams only.
 from __future__ import annotations
 
 import ctypes
+import importlib
+import sys
+from pathlib import Path
 from typing import NamedTuple, Optional
 
 import torch
@@ -183,97 +186,30 @@ def matmul_host(A_host: torch.Tensor, B_host: torch.Tensor, C_host: torch.Tensor
 # ----------------------------------------------------------------------------------------------
 # Products grouped by expert
 # ----------------------------------------------------------------------------------------------
-# These calls serve single decoding steps, where the host's time per call counts: each property of
-# a tensor is asked for once, and messages are put together only when something is wrong.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# These calls serve single decoding steps, where the host's time per call counts: their checks and
+# launches live in the neoGEMM extension (over the same C ABI), which costs about half of ctypes.
+class _Extension:
+    """The neoGEMM extension, imported on first use (it needs torch's CUDA libraries and a build)."""
+
+    def __getattr__(self, name):
+        root = str(Path(__file__).resolve().parent.parent)
+        try:
+            module = importlib.import_module("neoGEMM")
+        except ImportError:
+            sys.path.append(root)   # built in-tree beside the package
+            try:
+                module = importlib.import_module("neoGEMM")
+            except ImportError as e:
+                raise ImportError("the neoGEMM extension is missing: build it with `python -m "
+                                  "gemm_b200.build` (there is no fallback implementation)") from e
+            finally:
+                sys.path.remove(root)
+        value = getattr(module, name)
+        setattr(self, name, value)
+        return value
 
 
-def _call(fn, device: int, *args) -> None:
-    """fn(*args, stream) on torch's current stream of ``device``, with that device current."""
-    if _current_device() == device:
-        rc = fn(*args, _raw_stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device))
-    if rc:
-        check(rc)
-
-
-def _rows_operand(name: str, t: torch.Tensor, device: int = -1):
-    """(device, rows, width, pitch) of a bf16 matrix with contiguous rows that is read.  A single
-    row's pitch is nobody's to use: it gets a legal one."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype is not torch.bfloat16 or t.dim() != 2 or not t.is_cuda:
-        _require_cuda_bf16_matrix(name, t)
-    on = t.get_device()
-    if device >= 0 and on != device:
-        raise ValueError(f"{name} must be on cuda:{device}, not cuda:{on}")
-    rows, width = t.shape
-    pitch, step = t.stride()
-    if step != 1 and width > 1:
-        raise ValueError(f"{name} must have unit stride along its last dimension")
-    if rows <= 1:
-        pitch = (width + 15) & -8
-    return on, rows, width, pitch
-
-
-def _rows_result(out: Optional[torch.Tensor], like: torch.Tensor, device: int, T: int, width: int):
-    """(result, pitch, whether its rows of no group are to be zeroed)."""
-    if out is None:
-        return like.new_empty((T, width), dtype=torch.bfloat16), max(width, 1), 1
-    _require_cuda_bf16_matrix("out", out)
-    if out.shape != (T, width) or out.get_device() != device:
-        raise ValueError(f"out must be [{T},{width}] on cuda:{device}")
-    return out, _row_pitch("out", out), 0
-
-
-def _check_offsets(offsets: torch.Tensor, device: int):
-    """(groups, whether the indices are 64 bits wide)."""
-    if not isinstance(offsets, torch.Tensor):
-        raise TypeError("offsets must be a torch.Tensor")
-    wide = offsets.dtype is torch.int64
-    if not wide and offsets.dtype is not torch.int32:
-        raise TypeError(f"offsets must be int32 or int64, got {offsets.dtype}")
-    if not offsets.is_cuda or offsets.get_device() != device:
-        raise ValueError(f"offsets must be on cuda:{device}")
-    if offsets.dim() != 1 or offsets.shape[0] < 1 or not offsets.is_contiguous():
-        raise ValueError("offsets must be a contiguous vector of groups + 1 row indices")
-    return offsets.shape[0] - 1, 1 if wide else 0
-
-
-def _check_stack(name: str, w: torch.Tensor, device: int):
-    """(matrices, N, K, pitch, distance between matrices) of a [groups, N, K] operand."""
-    if not isinstance(w, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if w.dtype is not torch.bfloat16:
-        raise TypeError(f"{name} must be bfloat16, got {w.dtype}")
-    if w.dim() != 3:
-        raise ValueError(f"{name} must be [groups, N, K], got shape {tuple(w.shape)}")
-    if not w.is_cuda or w.get_device() != device:
-        raise ValueError(f"{name} must be on cuda:{device}")
-    groups, N, K = w.shape
-    stack, pitch, step = w.stride()
-    if step != 1 and K > 1:
-        raise ValueError(f"{name} must have unit stride along its last dimension")
-    return groups, N, K, pitch if N > 1 else (K + 15) & -8, stack if groups > 1 else 0
-
-
-def _grouped_rows(fn, name: str, rows: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
-                  out: Optional[torch.Tensor], transposed: bool) -> torch.Tensor:
-    device, T, depth, pitch = _rows_operand(name, rows)
-    matrices, N, K, pitch_w, stack_w = _check_stack("w", w, device)
-    groups, wide = _check_offsets(offsets, device)
-    if matrices != groups:
-        raise ValueError(f"w has {matrices} matrices but offsets delimit {groups} groups")
-    if depth != (N if transposed else K):
-        raise ValueError(f"{name} is [{T},{depth}] but w is [groups,{N},{K}]: expected rows of "
-                         f"{N if transposed else K}")
-    out, pitch_out, zero_rest = _rows_result(out, rows, device, T, K if transposed else N)
-    _call(fn, device, rows.data_ptr(), w.data_ptr(), out.data_ptr(), offsets.data_ptr(), wide, groups,
-          T, N, K, pitch, pitch_w, stack_w, pitch_out, zero_rest)
-    return out
+_ext = _Extension()
 
 
 def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
@@ -285,33 +221,21 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
     device; they are read on the GPU only.  Rows and matrices may be strided (contiguous along K,
     pitches multiples of 8).  Groups may be empty; at most 1024 of them.  Without ``out`` the rows
     of no group are zero; with ``out`` (bf16 [T, N], contiguous rows) they are left as they are."""
-    return _grouped_rows(lib.neogemm_grouped_nt, "x", x, w, offsets, out, False)
+    return _ext.grouped_matmul(x, w, offsets, out)
 
 
 def grouped_matmul_dx(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of :func:`grouped_matmul` by its rows: dx[t] = dy[t] @ w[e].  ``dy`` is bf16
     [T, N]; everything else as there."""
-    return _grouped_rows(lib.neogemm_grouped_dx, "dy", dy, w, offsets, out, True)
+    return _ext.grouped_matmul_dx(dy, w, offsets, out)
 
 
 def grouped_matmul_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of :func:`grouped_matmul` by its matrices: dw[e] = sum over the group's rows of
     dy[t]^T x[t], bf16 [groups, N, K]; zero for an empty group.  ``out`` must be contiguous."""
-    device, T, N, pitch_dy = _rows_operand("dy", dy)
-    _, rows, K, pitch_x = _rows_operand("x", x, device)
-    groups, wide = _check_offsets(offsets, device)
-    if rows != T:
-        raise ValueError(f"dy has {T} rows but x has {rows}")
-    if out is None:
-        out = dy.new_empty((groups, N, K))
-    elif (not isinstance(out, torch.Tensor) or out.dtype is not torch.bfloat16 or not out.is_cuda
-          or out.get_device() != device or out.shape != (groups, N, K) or not out.is_contiguous()):
-        raise ValueError(f"out must be a contiguous bfloat16 [{groups},{N},{K}] on cuda:{device}")
-    _call(lib.neogemm_grouped_dw, device, dy.data_ptr(), x.data_ptr(), out.data_ptr(),
-          offsets.data_ptr(), wide, groups, T, N, K, pitch_dy, pitch_x)
-    return out
+    return _ext.grouped_matmul_dw(dy, x, offsets, out)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -327,103 +251,35 @@ class MxFp4(NamedTuple):
     scales: torch.Tensor
 
 
-def _scales_shape(lead: tuple, rows: int, K: int) -> tuple:
-    return (*lead, (rows + 127) // 128, (K + 127) // 128, 32, 4, 4)
-
-
-def _check_mxfp4(name: str, q: MxFp4, dims: tuple, device: int = -1):
-    """(device, shape [.., rows, K]) of an MXFP4 operand with a number of dimensions in ``dims``."""
+def _mxfp4(name: str, q: MxFp4) -> tuple:
     if not isinstance(q, tuple) or len(q) != 2:
         raise TypeError(f"{name} must be an MxFp4 (codes, scales)")
-    codes, scales = q
-    if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
-        raise TypeError(f"{name} must be an MxFp4 (codes, scales)")
-    if not codes.is_cuda or not scales.is_cuda:
-        raise ValueError(f"{name} must live on a CUDA device (there is no CPU path)")
-    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
-        raise TypeError(f"{name}: codes and scales must be uint8")
-    shape = codes.shape
-    if len(shape) not in dims:
-        raise ValueError(f"{name}: codes must have {' or '.join(map(str, dims))} dimensions, got "
-                         f"shape {tuple(shape)}")
-    on = codes.get_device()
-    if scales.get_device() != on or (device >= 0 and on != device):
-        raise ValueError(f"{name}: all operands must be on the same device")
-    *lead, rows, packed = shape
-    if scales.shape != _scales_shape(lead, rows, 2 * packed):
-        raise ValueError(f"{name}: scales of codes {tuple(shape)} must be "
-                         f"{_scales_shape(lead, rows, 2 * packed)}, got {tuple(scales.shape)}")
-    if not codes.is_contiguous() or not scales.is_contiguous():
-        raise ValueError(f"{name}: codes and scales must be contiguous")
-    return on, (*lead, rows, 2 * packed)
+    return q
 
 
 def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
     """bf16 or fp32 [rows, K] or [stack, rows, K] (contiguous along K, K a multiple of 32) to MXFP4:
     per row and 32 values one scale 2^(floor(log2(largest magnitude)) - 2), values rounded to the
     nearest code (ties to even) and saturated at 6 scales.  A block with an Inf or NaN becomes NaN."""
-    if not isinstance(x, torch.Tensor):
-        raise TypeError("x must be a torch.Tensor")
-    if not x.is_cuda:
-        raise ValueError("x must live on a CUDA device (there is no CPU path)")
-    is_f32 = x.dtype is torch.float32
-    if not is_f32 and x.dtype is not torch.bfloat16:
-        raise TypeError(f"x must be bfloat16 or float32, got {x.dtype}")
-    shape = x.shape
-    if len(shape) not in (2, 3):
-        raise ValueError(f"x must be [rows, K] or [stack, rows, K], got shape {tuple(shape)}")
-    *lead, rows, K = shape
-    if K % 32 != 0:
-        raise ValueError(f"K must be a multiple of 32, got {K}")
-    stride = x.stride()
-    if K > 1 and stride[-1] != 1:
-        raise ValueError("x must have unit stride along its last dimension")
-    stack = lead[0] if lead else 1
-    codes = x.new_empty((*lead, rows, K // 2), dtype=torch.uint8)
-    scales = x.new_empty(_scales_shape(lead, rows, K), dtype=torch.uint8)
-    _call(lib.neogemm_mxfp4_quantize, x.get_device(), x.data_ptr(), 1 if is_f32 else 0,
-          codes.data_ptr(), scales.data_ptr(), stack, rows, K, stride[-2] if rows > 1 else K,
-          stride[0] if stack > 1 else 0)
-    return MxFp4(codes, scales)
+    return MxFp4(*_ext.quantize_mxfp4(x))
 
 
 def dequantize_mxfp4(q: MxFp4) -> torch.Tensor:
     """The values of an MXFP4 matrix (or stack) as bf16, which holds them exactly."""
-    device, shape = _check_mxfp4("q", q, (2, 3))
-    out = q[0].new_empty(shape, dtype=torch.bfloat16)
-    _call(lib.neogemm_mxfp4_dequantize, device, q[0].data_ptr(), q[1].data_ptr(), out.data_ptr(),
-          shape[0] if len(shape) == 3 else 1, shape[-2], shape[-1])
-    return out
+    return _ext.dequantize_mxfp4(*_mxfp4("q", q))
 
 
 def matmul_mxfp4(a: MxFp4, b: MxFp4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """C[M,N] = A[M,K] @ B[N,K]^T of two MXFP4 matrices, fp32 accumulation, bf16 result.  K must be
     a multiple of 64.  ``out`` may be any bf16 [M,N] tensor with contiguous rows."""
-    device, (M, K) = _check_mxfp4("a", a, (2,))
-    _, (N, Kb) = _check_mxfp4("b", b, (2,), device)
-    if Kb != K:
-        raise ValueError(f"a is [M,K]=[{M},{K}] but b is [N,K]=[{N},{Kb}]: K differs")
-    out, pitch, _ = _rows_result(out, a[0], device, M, N)
-    _call(lib.neogemm_mxfp4_nt, device, a[0].data_ptr(), a[1].data_ptr(), b[0].data_ptr(),
-          b[1].data_ptr(), out.data_ptr(), M, N, K, pitch)
-    return out
+    return _ext.matmul_mxfp4(*_mxfp4("a", a), *_mxfp4("b", b), out)
 
 
 def grouped_matmul_mxfp4(x: MxFp4, w: MxFp4, offsets: torch.Tensor,
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`grouped_matmul` with both operands in MXFP4: ``x`` [T, K], ``w`` [groups, N, K], K a
     multiple of 64."""
-    device, (T, K) = _check_mxfp4("x", x, (2,))
-    _, (matrices, N, Kw) = _check_mxfp4("w", w, (3,), device)
-    groups, wide = _check_offsets(offsets, device)
-    if matrices != groups:
-        raise ValueError(f"w has {matrices} matrices but offsets delimit {groups} groups")
-    if Kw != K:
-        raise ValueError(f"x is [T,K]=[{T},{K}] but w is [groups,N,K]=[{groups},{N},{Kw}]: K differs")
-    out, pitch, zero_rest = _rows_result(out, x[0], device, T, N)
-    _call(lib.neogemm_grouped_mxfp4_nt, device, x[0].data_ptr(), x[1].data_ptr(), w[0].data_ptr(),
-          w[1].data_ptr(), out.data_ptr(), offsets.data_ptr(), wide, groups, T, N, K, pitch, zero_rest)
-    return out
+    return _ext.grouped_matmul_mxfp4(*_mxfp4("x", x), *_mxfp4("w", w), offsets, out)
 
 
 def workspace_bytes(M: int, N: int, K: int, col_major: bool = False) -> int:
