@@ -62,11 +62,18 @@ int encode(const DeviceView& dev, CUtensorMap* map, CUtensorMapDataType type, co
                               static_cast<cuuint64_t>(stack)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(stack_pitch)};
   const cuuint32_t box[3] = {box_inner, box_rows, box_stack}, ones[3] = {1, 1, 1};
-  const CUresult r = dev.encode(
-      map, type, 3, const_cast<void*>(base), dims, strides, box, ones,
-      CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? NEOGEMM_OK : NEOGEMM_ERR_DESCRIPTOR;
+  auto try_encode = [&] {
+    return dev.encode(
+        map, type, 3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (try_encode()) return NEOGEMM_OK;
+  // A host thread that has made no runtime call yet (autograd runs a backward pass in one of its own) has
+  // no context for the driver call: bind the device's and try again.
+  if (cudaSetDevice(dev.index) == cudaSuccess && try_encode()) return NEOGEMM_OK;
+  cudaGetLastError();
+  return NEOGEMM_ERR_DESCRIPTOR;
 }
 
 // bf16 matrices, boxes of 64 elements (a 128-byte swizzle row); pitches in elements.  A single

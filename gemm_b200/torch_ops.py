@@ -70,3 +70,150 @@ class NeoLinear(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return torch.ops.neogemm.linear(x, self.weight)
+
+
+# ----------------------------------------------------------------------------------------------
+# Products grouped by expert, with their gradients
+# ----------------------------------------------------------------------------------------------
+def _check_grouped(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> None:
+    if x.dim() != 2 or weight.dim() != 3 or offsets.dim() != 1:
+        raise ValueError("grouped_linear expects x[T, K], weight[groups, N, K] and offsets[groups + 1]")
+    if x.shape[1] != weight.shape[2]:
+        raise ValueError(f"K mismatch: x has {x.shape[1]}, weight has {weight.shape[2]}")
+    if offsets.shape[0] != weight.shape[0] + 1:
+        raise ValueError(f"{weight.shape[0]} matrices need {weight.shape[0] + 1} offsets, got "
+                         f"{offsets.shape[0]}")
+    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError("grouped_linear expects bfloat16 tensors")
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """``t`` in a layout that the kernels read: contiguous rows that start on 16 bytes."""
+    if (t.shape[1] <= 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0 and (
+            t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
+        return t
+    rows, width = t.shape
+    return t.new_empty((rows, (width + 7) // 8 * 8))[:, :width].copy_(t)
+
+
+@torch.library.custom_op(f"{_LIB_NAME}::grouped_linear", mutates_args=())
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """y[t] = x[t] @ weight[e]^T for the rows of group e (``ops.grouped_matmul``); differentiable in
+    ``x`` and ``weight``.  Rows of no group are zero, and so are their gradients."""
+    _check_grouped(x, weight, offsets)
+    return _ops.grouped_matmul(x, weight, offsets)
+
+
+@grouped_linear.register_fake
+def _(x, weight, offsets):
+    _check_grouped(x, weight, offsets)
+    return x.new_empty((x.shape[0], weight.shape[1]))
+
+
+@torch.library.custom_op(f"{_LIB_NAME}::grouped_linear_dx", mutates_args=())
+def _grouped_linear_dx(dy: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    return _ops.grouped_matmul_dx(_readable(dy), weight, offsets)
+
+
+@_grouped_linear_dx.register_fake
+def _(dy, weight, offsets):
+    return dy.new_empty((dy.shape[0], weight.shape[2]))
+
+
+@torch.library.custom_op(f"{_LIB_NAME}::grouped_linear_dw", mutates_args=())
+def _grouped_linear_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    return _ops.grouped_matmul_dw(_readable(dy), x, offsets)
+
+
+@_grouped_linear_dw.register_fake
+def _(dy, x, offsets):
+    return dy.new_empty((offsets.shape[0] - 1, dy.shape[1], x.shape[1]))
+
+
+def _grouped_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _grouped_backward(ctx, dy):
+    x, weight, offsets = ctx.saved_tensors
+    dx = _grouped_linear_dx(dy, weight, offsets) if ctx.needs_input_grad[0] else None
+    dw = _grouped_linear_dw(dy, x, offsets) if ctx.needs_input_grad[1] else None
+    return dx, dw, None
+
+
+grouped_linear.register_autograd(_grouped_backward, setup_context=_grouped_setup)
+
+
+class NeoGroupedLinear(torch.nn.Module):
+    """One bias-free linear layer per group (expert): rows sorted by group in, rows out, trainable."""
+
+    def __init__(self, groups: int, in_features: int, out_features: int, device=None):
+        super().__init__()
+        self.groups, self.in_features, self.out_features = groups, in_features, out_features
+        self.weight = torch.nn.Parameter(
+            torch.empty(groups, out_features, in_features, dtype=torch.bfloat16, device=device))
+        torch.nn.init.normal_(self.weight, std=in_features ** -0.5)
+
+    def forward(self, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+        return torch.ops.neogemm.grouped_linear(x, self.weight, offsets)
+
+
+# ----------------------------------------------------------------------------------------------
+# Linear layers with weights held in MXFP4 (inference)
+# ----------------------------------------------------------------------------------------------
+def _check_mxfp4_linear(x: torch.Tensor, codes: torch.Tensor, dims: int) -> None:
+    if x.dim() < 1 or codes.dim() != dims:
+        raise ValueError(f"expected x[..., K] and codes of {dims} dimensions")
+    if x.shape[-1] != 2 * codes.shape[-1]:
+        raise ValueError(f"K mismatch: x has {x.shape[-1]}, weight has {2 * codes.shape[-1]}")
+    if x.dtype not in (torch.bfloat16, torch.float32) or codes.dtype != torch.uint8:
+        raise TypeError("expected x in bfloat16 or float32 and codes in uint8")
+
+
+@torch.library.custom_op(f"{_LIB_NAME}::mxfp4_linear", mutates_args=())
+def mxfp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """y = x @ W^T with x[..., K] quantised to MXFP4 on the way and W[N, K] held in it; bf16 result."""
+    _check_mxfp4_linear(x, codes, 2)
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.size(1) > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    y = _ops.matmul_mxfp4(_ops.quantize_mxfp4(x2), _ops.MxFp4(codes, scales))
+    return y.reshape(*x.shape[:-1], codes.shape[0])
+
+
+@mxfp4_linear.register_fake
+def _(x, codes, scales):
+    _check_mxfp4_linear(x, codes, 2)
+    return x.new_empty((*x.shape[:-1], codes.shape[0]), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_LIB_NAME}::mxfp4_grouped_linear", mutates_args=())
+def mxfp4_grouped_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                         offsets: torch.Tensor) -> torch.Tensor:
+    """``grouped_linear`` with x quantised to MXFP4 on the way and the weights held in it."""
+    _check_mxfp4_linear(x, codes, 3)
+    return _ops.grouped_matmul_mxfp4(_ops.quantize_mxfp4(x), _ops.MxFp4(codes, scales), offsets)
+
+
+@mxfp4_grouped_linear.register_fake
+def _(x, codes, scales, offsets):
+    _check_mxfp4_linear(x, codes, 3)
+    return x.new_empty((x.shape[0], codes.shape[1]), dtype=torch.bfloat16)
+
+
+class NeoLinearMxFp4(torch.nn.Module):
+    """Bias-free linear layer (or one per group, from a [groups, N, K] weight) whose weight is held in
+    MXFP4, 17/32 of a byte per value, and whose input is quantised on the way in.  Inference only."""
+
+    def __init__(self, weight: torch.Tensor):
+        super().__init__()
+        q = _ops.quantize_mxfp4(weight.detach())
+        self.register_buffer("codes", q.codes)
+        self.register_buffer("scales", q.scales)
+
+    def forward(self, x: torch.Tensor, offsets: torch.Tensor | None = None) -> torch.Tensor:
+        if self.codes.dim() == 3:
+            if offsets is None:
+                raise ValueError("a layer per group needs the groups' offsets")
+            return torch.ops.neogemm.mxfp4_grouped_linear(x, self.codes, self.scales, offsets)
+        return torch.ops.neogemm.mxfp4_linear(x, self.codes, self.scales)
