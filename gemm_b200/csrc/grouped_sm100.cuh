@@ -189,21 +189,93 @@ __device__ __forceinline__ void make_uniform(GroupedTile& t) {
   t.blocks = uniform(t.blocks);
 }
 
+// Rows [begin, end) of group e, clamped to the batch: indices that are out of order or out of range cost
+// the result, never an access.  True if they were in order.
+__device__ __forceinline__ bool group_range(const GroupedParams& p, int e, int* begin, int* end) {
+  long long b = 0, f = p.rows;
+  if (p.offsets != nullptr) {
+    if (p.offsets_are_64) {
+      b = static_cast<const long long*>(p.offsets)[e];
+      f = static_cast<const long long*>(p.offsets)[e + 1];
+    } else {
+      b = static_cast<const int*>(p.offsets)[e];
+      f = static_cast<const int*>(p.offsets)[e + 1];
+    }
+  }
+  const bool good = b >= 0 && f >= b && f <= p.rows;
+  b = b < 0 ? 0 : b > p.rows ? p.rows : b;
+  f = f < b ? b : f > p.rows ? p.rows : f;
+  *begin = static_cast<int>(b);
+  *end = static_cast<int>(f);
+  return good;
+}
+
+// Records offsets that were clamped: the launch is not aborted.
+__device__ __forceinline__ void report_offsets(const GroupedParams& p, int e) {
+  if (blockIdx.x == 0 && p.status != nullptr && atomicCAS(p.status, 0, kDevBounds) == 0) {
+    p.status[1] = 0;
+    p.status[2] = e;
+    p.status[3] = 4;
+    __threadfence_system();
+  }
+}
+
+// In shared memory, for more than 32 groups.
+struct GroupTable {
+  int *begin, *end;   // [kMaxGroups]
+  int* first;         // [kMaxGroups + 1]
+};
+
 // The tiles of one worker (a CTA, a pair, or a cluster that splits the contraction), in order.
 // Every role walks its own copy.
 template <class Cfg>
 struct GroupedTiles {
-  const int *begin, *end, *first;   // row ranges, and the first tile of every group
+  // Row ranges and first tiles of the groups: up to 32 of them are held by the lanes of each warp, which
+  // then needs neither shared memory nor a barrier between reading the offsets and its first tile; more
+  // are in shared memory.
+  const GroupTable& table;
+  int my_begin, my_end, my_first, total;
+  bool good;   // this lane's group was in order
   int next, last, step;
   int split_rank;
   int group, g0, g1, tiles, share;  // the group of the last tile: its rows and its columns' tiles
-  int group_last;                   // first tile of the next group
+  int group_first, group_last;      // its first tile and the next group's
 
-  __device__ __forceinline__ GroupedTiles(const GroupedParams& p, const int* begin_, const int* end_,
-                                          const int* first_, int worker, int workers, int split_rank_)
-      : begin(begin_), end(end_), first(first_), next(worker), step(workers), split_rank(split_rank_),
+  __device__ __forceinline__ GroupedTiles(const GroupedParams& p, const GroupTable& table_, int worker,
+                                          int workers, int split_rank_)
+      : table(table_), good(true), next(worker), step(workers), split_rank(split_rank_),
         group_last(0) {
-    last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : uniform(first[p.groups]);
+    if (p.groups <= 32) {
+      const int lane = static_cast<int>(ptx::lane_id());
+      good = group_range(p, min(lane, p.groups - 1), &my_begin, &my_end);
+      const int mine = Cfg::kOp == kGroupedDw || lane >= p.groups
+                           ? 0 : column_tiles<Cfg>(p, my_begin, my_end) * p.lane_tiles;
+      int scan = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int other = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += other;
+      }
+      my_first = scan - mine;
+      total = __shfl_sync(0xffffffffu, scan, 31);
+    } else {
+      total = table.first[p.groups];
+    }
+    total = uniform(total);
+    last = Cfg::kOp == kGroupedDw ? p.groups * p.lane_tiles * p.col_tiles : total;
+  }
+
+  __device__ __forceinline__ int begin_of(const GroupedParams& p, int e) const {
+    return p.groups <= 32 ? __shfl_sync(0xffffffffu, my_begin, e) : table.begin[e];
+  }
+  __device__ __forceinline__ int end_of(const GroupedParams& p, int e) const {
+    return p.groups <= 32 ? __shfl_sync(0xffffffffu, my_end, e) : table.end[e];
+  }
+  // First tile of group e <= groups.
+  __device__ __forceinline__ int first_of(const GroupedParams& p, int e) const {
+    if (p.groups > 32) return table.first[e];
+    const int first = __shfl_sync(0xffffffffu, my_first, e & 31);
+    return e < p.groups ? first : total;
   }
 
   __device__ __forceinline__ bool take(const GroupedParams& p, GroupedTile& t) {
@@ -217,24 +289,27 @@ struct GroupedTiles {
       t.col_row = (local - lane_tile * p.col_tiles) * Cfg::kCols;
       t.lo = 0;
       t.hi = min(Cfg::kCols, p.cols - t.col_row);
-      t.k_row = begin[t.group];
-      t.k_len = end[t.group] - t.k_row;
+      t.k_row = begin_of(p, t.group);
+      t.k_len = end_of(p, t.group) - t.k_row;
     } else {
       if (next >= group_last) {
         // Last group whose first tile is not behind this one: groups without tiles share their
         // first tile with the next group and lose the comparison.  The warp looks at every 32nd
         // group, then at the 32 from there (bisection cost 500 cycles a tile in each role).
         const int lane = static_cast<int>(ptx::lane_id());
-        int a = 0;
-        if (p.groups > 32)
-          a = 32 * (__popc(__ballot_sync(0xffffffffu, lane * 32 < p.groups &&
-                                                          first[min(lane * 32, p.groups)] <= next)) - 1);
-        a += __popc(__ballot_sync(0xffffffffu, a + lane < p.groups &&
-                                                   first[min(a + lane, p.groups)] <= next)) - 1;
-        group = a;
-        g0 = begin[a];
-        g1 = end[a];
-        group_last = first[a + 1];
+        if (p.groups <= 32) {
+          group = __popc(__ballot_sync(0xffffffffu, lane < p.groups && my_first <= next)) - 1;
+        } else {
+          int a = 32 * (__popc(__ballot_sync(0xffffffffu, lane * 32 < p.groups &&
+                                             table.first[min(lane * 32, p.groups)] <= next)) - 1);
+          a += __popc(__ballot_sync(0xffffffffu, a + lane < p.groups &&
+                                                     table.first[min(a + lane, p.groups)] <= next)) - 1;
+          group = a;
+        }
+        g0 = begin_of(p, group);
+        g1 = end_of(p, group);
+        group_first = first_of(p, group);
+        group_last = first_of(p, group + 1);
         tiles = column_tiles<Cfg>(p, g0, g1);
         // Equal shares of the columns, in steps of the MMA's granularity.
         share = Cfg::kCols;
@@ -243,7 +318,7 @@ struct GroupedTiles {
                   Cfg::kColStep * Cfg::kColStep;
       }
       t.group = group;
-      const int local = next - first[group];
+      const int local = next - group_first;
       // Streaming: tiles that are read at a time lie side by side.
       int c, lane_tile;
       if (Cfg::kStream) {
@@ -323,9 +398,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   uint8_t* tail_gen = smem_gen + (part_free_bar + 16 * Cfg::kSplit - smem_base);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail_gen);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_gen + 4);
-  int* begin = reinterpret_cast<int*>(tail_gen + 16);        // [kMaxGroups]
-  int* end = begin + kMaxGroups;                             // [kMaxGroups]
-  int* first_tile = end + kMaxGroups;                        // [kMaxGroups + 1]
+  int* const words = reinterpret_cast<int*>(tail_gen + 16);
+  const GroupTable table{words, words + kMaxGroups, words + 2 * kMaxGroups};
 
   const int warp = uniform(static_cast<int>(threadIdx.x >> 5));
   const uint32_t lane = lane_id();
@@ -368,58 +442,40 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::kTmemCols);
     tmem_relinquish<1>();
   }
-  // Global memory from here on: wait for the previous kernel of the stream.
-  griddep_wait();
-  // Row ranges of the groups, clamped to the batch: indices that are out of order or out of range
-  // cost the result, never an access.
-  for (int e = threadIdx.x; e < p.groups; e += Cfg::kThreads) {
-    long long b = 0, f = p.rows;
-    if (p.offsets != nullptr) {
-      if (p.offsets_are_64) {
-        b = static_cast<const long long*>(p.offsets)[e];
-        f = static_cast<const long long*>(p.offsets)[e + 1];
-      } else {
-        b = static_cast<const int*>(p.offsets)[e];
-        f = static_cast<const int*>(p.offsets)[e + 1];
-      }
-    }
-    if (b < 0 || f < b || f > p.rows) {
-      if (blockIdx.x == 0 && p.status != nullptr && atomicCAS(p.status, 0, kDevBounds) == 0) {
-        p.status[1] = 0;
-        p.status[2] = e;
-        p.status[3] = 4;
-        __threadfence_system();
-      }
-      b = b < 0 ? 0 : b > p.rows ? p.rows : b;
-      f = f < b ? b : f > p.rows ? p.rows : f;
-    }
-    begin[e] = static_cast<int>(b);
-    end[e] = static_cast<int>(f);
-  }
   tcgen05_fence_before();
   if (Cfg::kCluster > 1) cluster_sync_all(); else __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  if (kCtaGroup == 2 && tmem_base != 0 && threadIdx.x == 0)
+  const uint32_t tmem_base = uniform(*tmem_slot);
+  // The pair's MMA addresses both CTAs' tensor memory with the leader's address.
+  const bool usable = kCtaGroup == 1 || tmem_base == 0;
+  if (!usable && threadIdx.x == 0)
     report_error(p.status, abort_flag, kDevTmemAddress, 0, static_cast<int>(tmem_base));
-  if (!kDw && warp == 0) {
-    int sum = 0;
-    for (int base = 0; base < p.groups; base += 32) {
-      const int e = base + static_cast<int>(lane);
-      const int mine = e < p.groups ? column_tiles<Cfg>(p, begin[e], end[e]) * p.lane_tiles : 0;
-      int scan = mine;
+  // Global memory from here on: wait for the previous kernel of the stream.
+  griddep_wait();
+  if (p.groups > 32) {
+    for (int e = threadIdx.x; e < p.groups; e += Cfg::kThreads)
+      if (!group_range(p, e, table.begin + e, table.end + e)) report_offsets(p, e);
+    __syncthreads();
+    if (warp == 0) {
+      int sum = 0;
+      for (int base = 0; base < p.groups; base += 32) {
+        const int e = base + static_cast<int>(lane);
+        const int mine =
+            !kDw && e < p.groups ? column_tiles<Cfg>(p, table.begin[e], table.end[e]) * p.lane_tiles : 0;
+        int scan = mine;
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int other = __shfl_up_sync(0xffffffffu, scan, d);
-        if (static_cast<int>(lane) >= d) scan += other;
+        for (int d = 1; d < 32; d *= 2) {
+          const int other = __shfl_up_sync(0xffffffffu, scan, d);
+          if (static_cast<int>(lane) >= d) scan += other;
+        }
+        if (e < p.groups) table.first[e] = sum + scan - mine;
+        sum += __shfl_sync(0xffffffffu, scan, 31);
       }
-      if (e < p.groups) first_tile[e] = sum + scan - mine;
-      sum += __shfl_sync(0xffffffffu, scan, 31);
+      if (lane == 0) table.first[p.groups] = sum;
     }
-    if (lane == 0) first_tile[p.groups] = sum;
+    __syncthreads();
   }
-  __syncthreads();
-  GroupedTiles<Cfg> tiles(p, begin, end, first_tile, worker, num_workers, split_rank);
+  GroupedTiles<Cfg> tiles(p, table, worker, num_workers, split_rank);
   GroupedTile t;
   int tile = 0;   // of this worker, for error records
   // Ring slots.  Streaming: sized for the widest tile of the launch, of one or two k-blocks.
@@ -430,8 +486,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   const uint32_t slots = Cfg::kStream ? p.slots : kStages;
 
   // ---------------------------------------------------------------- roles
-  if (uniform(*abort_flag) != 0) {
-    // The tensor-memory address check failed: nothing is issued.
+  if (!usable) {
+    // Nothing is issued.
   } else if (warp == 0) {
     // ======================= TMA producer =======================
     uint32_t stage = 0, phase = 0;
@@ -531,8 +587,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         make_uniform(t);
         const uint32_t acc = count % Cfg::kAccs, acc_phase = (count / Cfg::kAccs) & 1;
         ++count;
-        if (!__all_sync(0xffffffffu, mbar_wait<kCtaGroup == 2>(tmem_empty_bar + 8 * acc,
-                                                               acc_phase ^ 1, abort_flag))) {
+        if (!__all_sync(0xffffffffu, mbar_wait<kCtaGroup == 2, Cfg::kAccs == 1>(
+                                             tmem_empty_bar + 8 * acc, acc_phase ^ 1, abort_flag))) {
           if (lane == 0)
             report_error(p.status, abort_flag, kDevTimeoutMmaTmem, tile, static_cast<int>(acc));
           break;
@@ -650,20 +706,32 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       const int lane_end = p.lanes;
       const int cols_end = min(t.hi, first_col + Cfg::kEpiCols);   // of this warp
       auto in_use = [&](int c) { return lane_first < lane_end && c < cols_end && c + 32 > t.lo; };
+      auto hand_back = [&] {
+        if (t.blocks == 0) return;
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kCtaGroup == 2) mbar_arrive_cluster(mapa_u32(tmem_empty_bar + 8 * acc, 0));
+          else mbar_arrive(tmem_empty_bar + 8 * acc);
+        }
+      };
       // Up to four times 32 columns of this warp's lanes from `c`, rounded to bf16 and packed in
-      // pairs: two loads are issued before the first is waited for.
+      // pairs: two loads are issued before the first is waited for.  The accumulator goes back after
+      // the last of them.
       auto pull = [&](int c, uint32_t (&w)[4][16]) {
         if (t.blocks > 0) {
+          constexpr int kBatch = 2;
 #pragma unroll
-          for (int h = 0; h < 4; h += 2) {
-            uint32_t r[2][32];
+          for (int h = 0; h < 4; h += kBatch) {
+            uint32_t r[kBatch][32];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kBatch; ++i)
               if (in_use(c + (h + i) * 32))
                 tmem_ld_32x32b_x32(tmem_base + acc * Cfg::kCols + lane_base + c + (h + i) * 32, r[i]);
             tmem_ld_wait();
+            if (h + kBatch == 4 && c + 128 >= cols_end) hand_back();
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kBatch; ++i)
 #pragma unroll
               for (int j = 0; j < 16; ++j)
                 w[h + i][j] = pack_bf16x2(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1]));
@@ -673,15 +741,6 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[i][j] = 0u;
-        }
-      };
-      auto hand_back = [&] {
-        if (t.blocks == 0) return;
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (kCtaGroup == 2) mbar_arrive_cluster(mapa_u32(tmem_empty_bar + 8 * acc, 0));
-          else mbar_arrive(tmem_empty_bar + 8 * acc);
         }
       };
       auto store = [&](int c, const uint32_t (&w)[16]) {
@@ -812,26 +871,20 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           break;
         }
       } else {
-        // 128 columns at a time; the accumulator goes back once the last of them are in registers.
-        bool held = true;
         const int c_first = max(first_col, t.lo & ~31);
+        if (!in_use(c_first)) hand_back();
         for (int c = c_first; in_use(c); c += 128) {
           uint32_t w[4][16];
           pull(c, w);
-          if (c + 128 >= cols_end) {
-            hand_back();
-            held = false;
-          }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (in_use(c + i * 32)) store(c + i * 32, w[i]);
         }
-        if (held) hand_back();
       }
     }
     if (!kDw && p.zero_rest) {
       // Rows of no group: in front of the first and behind the last.
-      const int head = begin[0], tail = end[p.groups - 1];
+      const int head = tiles.begin_of(p, 0), tail = tiles.end_of(p, p.groups - 1);
       const int rest = head + p.rows - tail;
       for (int i = static_cast<int>(blockIdx.x) * Cfg::kEpiWarps + warp - 2; i < rest;
            i += static_cast<int>(gridDim.x) * Cfg::kEpiWarps) {
@@ -880,6 +933,9 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   }
   __syncwarp();
 
+  if (warp == 0 && !tiles.good) report_offsets(p, min(static_cast<int>(lane), p.groups - 1));
+  __syncwarp();
+
   // ---------------------------------------------------------------- tear-down
   tcgen05_fence_before();
   if (Cfg::kCluster > 1) cluster_sync_all(); else __syncthreads();
@@ -887,8 +943,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     // Let boxes still in flight land in this CTA's shared memory before it is released.
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
+    if (Cfg::kCluster > 1) cluster_sync_all(); else __syncthreads();
   }
-  if (Cfg::kCluster > 1) cluster_sync_all(); else __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
     tmem_dealloc<1>(tmem_base, Cfg::kTmemCols);
