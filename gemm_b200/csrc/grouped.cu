@@ -387,10 +387,14 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  // The pair's tiles are 256 x 256 of a group's matrix whatever its rows (513 rows over 8 groups,
-  // 1024 x 2048: 14.2 us, single CTAs 14.0; 16384 rows, 4096 x 4096: 390 and 480).
+  // Tiles of 128 x 128 on single CTAs, or 256 x 256 on pairs where many of them go round, or enough with
+  // a long contraction each.  Measured, us, single / pairs: 8 groups of 1024 x 2048 with 64 rows 11.2
+  // 11.8, 512 rows 23.8 24.2, 2048 rows 65.0 60.4; of 4096 x 4096 with 1 row 53.8 48.3, 128 rows 71.0
+  // 71.9, 2048 rows 474 403; 4 groups of 256 x 512 with 2048 rows 11.8 18.9.
   const int forced = tuning_value(13);
-  const bool wide = forced >= 0 ? forced == kWide : N >= 256 && K >= 256;
+  const int64_t pair_tiles = groups * ceil_div(N, 256) * ceil_div(K, 256);
+  const bool wide = forced >= 0 ? forced == kWide
+                                : pair_tiles >= 592 || (pair_tiles >= 148 && T / groups >= 512);
   const KernelEntry& k = kKernels[kGroupedDw][wide ? kWide : kNarrow];
   GroupedMaps maps;
   std::memset(&maps, 0, sizeof(maps));
@@ -414,6 +418,10 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   p.lane_tiles = static_cast<int>(lane_tiles);
   p.col_tiles = static_cast<int>(col_tiles);
   p.vector_out = K % 8 == 0 && aligned16(dW);
+  if (p.vector_out) {
+    rc = encode_bf16(dev, &maps.result, dW, K, N, groups, K, N * K, 32);
+    if (rc != NEOGEMM_OK) return rc;
+  }
   p.out = static_cast<__nv_bfloat16*>(dW);
   p.out_pitch = K;
   p.out_stack = N * K;

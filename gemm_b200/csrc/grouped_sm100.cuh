@@ -54,7 +54,8 @@ struct GroupedParams {
   int slots, per_slot;      // streaming kernels: ring slots, and the k-blocks that each takes
   int col_tiles;            // kGroupedDw: tiles along `cols`
   int zero_rest;            // write zeros to the rows of no group (0: leave them)
-  int vector_out;           // 16-byte stores are possible (alignment of base and pitches)
+  int vector_out;           // 16-byte stores are possible (alignment of base and pitches); for dW the
+                            // result leaves by TMA then
   __nv_bfloat16* out;
   long long out_pitch;      // elements between rows of the result
   long long out_stack;      // kGroupedDw: elements between the groups' matrices
@@ -368,9 +369,10 @@ struct BlockLayout {
 };
 
 // Tensor maps of the operands, by box: lanes (128 rows, MN-major lanes 64 x 64), columns (col_box and
-// small_box rows), scales (MXFP4) of the lanes and of the columns.
+// small_box rows), scales (MXFP4) of the lanes and of the columns; the result of dW (boxes of 32 rows
+// x 64 columns, clipped at the matrices' edges).
 struct GroupedMaps {
-  CUtensorMap lanes, cols, small_cols, lane_scales, col_scales;
+  CUtensorMap lanes, cols, small_cols, lane_scales, col_scales, result;
 };
 
 template <class Cfg>
@@ -433,6 +435,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     prefetch_tensormap(&maps.lanes);
     prefetch_tensormap(&maps.cols);
     if (!kDw) prefetch_tensormap(&maps.small_cols);
+    if (kDw && p.vector_out) prefetch_tensormap(&maps.result);
     if (kMx) {
       prefetch_tensormap(&maps.lane_scales);
       prefetch_tensormap(&maps.col_scales);
@@ -876,12 +879,37 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         for (int c = c_first; in_use(c); c += 128) {
           uint32_t w[4][16];
           pull(c, w);
+          if (kDw && p.vector_out) {
+            // 32 rows x 64 columns through the warp's 4 KB as one swizzled box (dW of short groups is
+            // bound by its stores).
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              if (!in_use(c + i * 32)) continue;
+              if (lane == 0) tma_store_wait_read<0>();
+              __syncwarp();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const uint32_t* v = &w[i + j / 4][4 * (j & 3)];
+                st_shared_v4(stage_buf + lane * 128 + ((j ^ (lane & 7)) << 4), v[0], v[1], v[2], v[3]);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_3d(&maps.result, stage_buf, t.col_row + c + i * 32, lane_first, t.group);
+                tma_store_commit();
+              }
+            }
+            continue;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (in_use(c + i * 32)) store(c + i * 32, w[i]);
         }
       }
     }
+    // Shared memory outlives the stores' reads of it.
+    if (kDw && lane == 0) tma_store_wait_read<0>();
+    __syncwarp();
     if (!kDw && p.zero_rest) {
       // Rows of no group: in front of the first and behind the last.
       const int head = tiles.begin_of(p, 0), tail = tiles.end_of(p, p.groups - 1);
@@ -915,11 +943,13 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           break;
         }
         parities ^= 1u << stage;
-        // A box is 64 rows of 128 bytes; the swizzle moves bytes inside a row only.
+        // A box is 64 rows of 128 bytes; the swizzle moves bytes inside a row only.  The products
+        // stop at the next multiple of 16 rows.
+        const uint32_t last_byte = static_cast<uint32_t>((valid + 15) / 16 * 16) * 128;
         const uint32_t sl = ring + stage * Cfg::kStageBytes;
         const int boxes = 2 + (t.mma_n / kCtaGroup + 63) / 64;   // the lane operand's two in front
         for (int b = 0; b < boxes; ++b)
-          for (uint32_t o = static_cast<uint32_t>(valid) * 128 + lane * 16; o < 8192; o += 512)
+          for (uint32_t o = static_cast<uint32_t>(valid) * 128 + lane * 16; o < last_byte; o += 512)
             st_shared_v4(sl + b * 8192 + o, 0, 0, 0, 0);
         fence_proxy_async_smem();
         __syncwarp();
