@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 constexpr int64_t kMaxExtent = 0x7fffffffll - 4096;   // room for tile coordinates past the end
+constexpr int64_t kMaxPitch = 1ll << 38;              // elements; keeps every product below in 64 bits
 
 struct KernelEntry {
   int op, cta_group, split, columns, stages;
@@ -241,6 +242,8 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   const int64_t lanes = op == kGroupedDx ? K : N;    // width of the result
   if (T == 0 || lanes == 0) return NEOGEMM_OK;
   if (out == nullptr || ldo < lanes) return NEOGEMM_ERR_BAD_ARG;
+  if (ldo > kMaxPitch || ldr > kMaxPitch || ldw > kMaxPitch || stack_w > kMaxPitch)
+    return NEOGEMM_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(out) & 1) != 0) return NEOGEMM_ERR_UNSUPPORTED;
   if (groups == 0) return zero_rest ? zero_rows(out, ldo, T, lanes, stream) : NEOGEMM_OK;
   if (depth > 0) {
@@ -300,6 +303,7 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
             int64_t ldy, int zero_rest, cudaStream_t stream) {
   if (T == 0 || N == 0) return NEOGEMM_OK;
   if (Y == nullptr || ldy < N) return NEOGEMM_ERR_BAD_ARG;
+  if (ldy > kMaxPitch) return NEOGEMM_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(Y) & 1) != 0 || K % 64 != 0) return NEOGEMM_ERR_UNSUPPORTED;
   if (groups == 0) return zero_rest ? zero_rows(Y, ldy, T, N, stream) : NEOGEMM_OK;
   if (K > 0) {
@@ -313,8 +317,7 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
 
   const KernelEntry& k = kKernels[kMxNt][variant_of(kMxNt, groups, T, N, K)];
   const int64_t k_tiles = ceil_div(K, 128), w_tiles = ceil_div(N, 128), x_tiles = ceil_div(T, 128);
-  if (groups * w_tiles * k_tiles > kMaxExtent || x_tiles * k_tiles > kMaxExtent)
-    return NEOGEMM_ERR_UNSUPPORTED;
+  if (groups * w_tiles * k_tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
   GroupedParams p;
   std::memset(&p, 0, sizeof(p));
   p.offsets = offsets;
@@ -380,6 +383,7 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   if ((reinterpret_cast<uintptr_t>(dW) & 1) != 0) return NEOGEMM_ERR_UNSUPPORTED;
   if (T > 0) {
     if (dY == nullptr || X == nullptr || lddy < N || ldx < K) return NEOGEMM_ERR_BAD_ARG;
+    if (lddy > kMaxPitch || ldx > kMaxPitch) return NEOGEMM_ERR_UNSUPPORTED;
     if (lddy % 8 != 0 || ldx % 8 != 0 || !aligned16(dY) || !aligned16(X))
       return NEOGEMM_ERR_UNSUPPORTED;
   }

@@ -248,6 +248,7 @@ int neogemm_mxfp4_quantize(const void* X, int x_is_f32, void* codes, void* scale
   if (stack == 0 || rows == 0 || K == 0) return NEOGEMM_OK;
   if (X == nullptr || ldx < K || stack_x < 0) return NEOGEMM_ERR_BAD_ARG;
   const int64_t step = x_is_f32 ? 4 : 8;   // elements in 16 bytes
+  if (ldx > 1ll << 45 || stack_x > 1ll << 45) return NEOGEMM_ERR_UNSUPPORTED;
   if (!aligned16(X) || (rows > 1 && ldx % step != 0) || (stack > 1 && stack_x % step != 0))
     return NEOGEMM_ERR_UNSUPPORTED;
   DeviceView dev;

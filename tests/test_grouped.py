@@ -40,7 +40,8 @@ def test_rows_products_refuse(name, memory):
         assert rows_call(fn, p, **bad) == BAD_ARG, bad
     for bad in (dict(ldr=28), dict(ldw=28), dict(stack=388), dict(R=p + 2), dict(W=p + 8), dict(out=p + 1),
                 dict(offsets=p + 2), dict(offsets=p + 4, wide=1), dict(groups=1025), dict(T=1 << 31),
-                dict(N=1 << 40, ldo=1 << 40), dict(K=1 << 31)):
+                dict(N=1 << 40, ldo=1 << 40), dict(K=1 << 31), dict(ldr=1 << 62), dict(stack=1 << 62),
+                dict(ldw=1 << 40), dict(ldo=1 << 60)):
         assert rows_call(fn, p, **bad) in (UNSUPPORTED, BAD_ARG), bad
     # nothing to do
     assert rows_call(fn, p, T=0) == OK

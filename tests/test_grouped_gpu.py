@@ -301,3 +301,43 @@ def test_refusals_on_the_device():
         ops.grouped_matmul(x, torch.empty(1025, 8, 16, device="cuda").bfloat16(),
                            torch.zeros(1026, dtype=torch.int32, device="cuda"))
     assert ops.device_status()[0] == 0
+
+
+def test_as_many_groups_as_there_may_be(tiles):
+    counts = [0] * 1024
+    for e, c in ((0, 1), (31, 2), (32, 1), (33, 3), (500, 17), (1022, 1), (1023, 40)):
+        counts[e] = c
+    N, K = 40, 72
+    x, w, dy = make(counts, N, K, tail=2)
+    ends, off = offsets_of(counts)
+    for op, depth in (("nt", K), ("dx", N), ("dw", 40)):
+        want, mag = plain(op, ends, x, w, dy)
+        assert_close(call(op, x, w, dy, off), want, mag, depth)
+
+
+@pytest.mark.parametrize("op", ["nt", "dx", "dw"])
+def test_results_of_more_than_2_31_values(op):
+    """Offsets past 32 bits: the last rows and the last matrix are where they belong."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").bfloat16()
+
+    if op == "dw":
+        E, N, K, T = 34, 8192, 8192, 70
+        dy, x = normal(T, N), normal(T, K)
+        off = torch.tensor([0] * 33 + [3, T], dtype=torch.int32, device="cuda")
+        out = ops.grouped_matmul_dw(dy, x, off)
+        assert out.numel() > 2 ** 31 and (out[:32, ::1000, ::1000] == 0).all()
+        want = dy[3:, -40:].double().t() @ x[3:, -50:].double()
+        mag = dy[3:, -40:].double().abs().t() @ x[3:, -50:].double().abs()
+        assert_close(out[33, -40:, -50:], want, mag, T)
+        return
+    wide, deep, T = 65536, 64, 33000
+    w = normal(2, wide, deep) if op == "nt" else normal(2, deep, wide)
+    r = normal(T, deep)
+    off = torch.tensor([0, 10, T], dtype=torch.int64, device="cuda")
+    out = ops.grouped_matmul(r, w, off) if op == "nt" else ops.grouped_matmul_dx(r, w, off)
+    assert out.numel() > 2 ** 31
+    m = w[1].double().t() if op == "nt" else w[1].double()
+    assert_close(out[-20:], r[-20:].double() @ m, r[-20:].double().abs() @ m.abs(), deep)

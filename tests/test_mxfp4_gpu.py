@@ -252,3 +252,19 @@ def test_refusals_on_the_device():
         ops.quantize_mxfp4(torch.zeros(4, 104, device="cuda")[:, 2:66])
     with pytest.raises(ValueError):
         ops.grouped_matmul_mxfp4(a, a, torch.tensor([0, 10], dtype=torch.int32, device="cuda"))
+
+
+def test_tensors_of_more_than_2_31_values():
+    """Conversion there and back, and a product whose result passes 32 bits."""
+    x = make(64, 8192)
+    big = x.repeat(4200, 1)                      # 2.2e9 values
+    q = ops.quantize_mxfp4(big)
+    want = ops.dequantize_mxfp4(ops.quantize_mxfp4(x))
+    back = ops.dequantize_mxfp4(q)
+    assert big.numel() > 2 ** 31 and torch.equal(back[-64:], want) and torch.equal(back[:64], want)
+    del big, back, q
+    a, b = ops.quantize_mxfp4(make(33000, 64)), ops.quantize_mxfp4(make(65536, 64, seed=2))
+    c = ops.matmul_mxfp4(a, b)
+    va, vb = values(ops.MxFp4(a.codes, a.scales))[-9:], values(b)
+    assert c.numel() > 2 ** 31
+    assert_product(c[-9:], va @ vb.t(), va.abs() @ vb.abs().t(), 64)
