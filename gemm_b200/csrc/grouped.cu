@@ -43,8 +43,8 @@ const KernelEntry kKernels[4][kVariants] = {
      make_entry<GroupedConfig<kGroupedNt, 1, 2, 128, 8>>()},
     {make_entry<GroupedConfig<kGroupedDx, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 1, 256, 6>>(),
      make_entry<GroupedConfig<kGroupedDx, 1, 2, 128, 8>>()},
-    {make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 6>>(), make_entry<GroupedConfig<kGroupedDw, 2, 1, 256, 5>>(),
-     make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 6>>()},
+    {make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 5>>(), make_entry<GroupedConfig<kGroupedDw, 2, 1, 256, 5>>(),
+     make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 5>>()},
     {make_entry<GroupedConfig<kMxNt, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 2, 1, 256, 5>>(),
      make_entry<GroupedConfig<kMxNt, 1, 2, 128, 8>>()},
 };
@@ -392,13 +392,13 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   if (rc != NEOGEMM_OK) return rc;
 
   // Tiles of 128 x 128 on single CTAs, or 256 x 256 on pairs where many of them go round, or enough with
-  // a long contraction each.  Measured, us, single / pairs: 8 groups of 1024 x 2048 with 64 rows 11.2
-  // 11.8, 512 rows 23.8 24.2, 2048 rows 65.0 60.4; of 4096 x 4096 with 1 row 53.8 48.3, 128 rows 71.0
-  // 71.9, 2048 rows 474 403; 4 groups of 256 x 512 with 2048 rows 11.8 18.9.
+  // a long contraction each.  Measured, us, single / pairs: 8 groups of 1024 x 2048 with 64 rows 10.1
+  // 11.6, 256 rows 16.0 16.1, 2048 rows 65 60; of 4096 x 4096 with 64 rows 58 61, 512 rows 171 141,
+  // 2048 rows 474 403; 4 groups of 256 x 512 with 2048 rows 11.8 18.9.
   const int forced = tuning_value(13);
   const int64_t pair_tiles = groups * ceil_div(N, 256) * ceil_div(K, 256);
   const bool wide = forced >= 0 ? forced == kWide
-                                : pair_tiles >= 592 || (pair_tiles >= 148 && T / groups >= 512);
+                                : pair_tiles >= 592 || (pair_tiles >= 148 && T / groups >= 256);
   const KernelEntry& k = kKernels[kGroupedDw][wide ? kWide : kNarrow];
   GroupedMaps maps;
   std::memset(&maps, 0, sizeof(maps));

@@ -111,7 +111,10 @@ struct GroupedConfig {
   // x 16 columns in fp32 (from kSplit CTAs 128 / kSplit lanes each).
   static constexpr int kPartCols = 16;
   static constexpr int kPartBytes = 128 * kPartCols * 4;
-  static constexpr int kEpiBytes = kEpiWarps * 2 * 2048;
+  // dW: one or two boxes of 32 x 64 bf16 per warp.
+  static constexpr int kBoxBufs = (kOp == kGroupedDw && kCtaGroup == 1) ? 2 : 1;
+  static constexpr int kEpiWarpBytes = 4096 * kBoxBufs;
+  static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
   static_assert(!kStream || kEpiBytes >= 2 * kPartBytes, "partial sums");
   static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
   static constexpr int kBarrierBytes = (3 * kStages + 4 + 2 + 2 * kSplit) * 8 + 16;
@@ -690,7 +693,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     const int quad = warp & 3;   // the warp's quarter of the tensor-memory lanes
     const int first_col = (warp - 2) / 4 * Cfg::kEpiCols;   // and its share of the columns
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t stage_buf = epi_base + (warp - 2) * 4096;
+    const uint32_t stage_buf = epi_base + (warp - 2) * Cfg::kEpiWarpBytes;
     uint32_t buf = 0;
     int count = 0;
     int parts = 0;   // column groups of partial sums so far
@@ -885,17 +888,19 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
               if (!in_use(c + i * 32)) continue;
-              if (lane == 0) tma_store_wait_read<0>();
+              if (lane == 0) tma_store_wait_read<Cfg::kBoxBufs - 1>();
               __syncwarp();
+              const uint32_t box = stage_buf + buf * 4096;
+              buf = (buf + 1) % Cfg::kBoxBufs;
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const uint32_t* v = &w[i + j / 4][4 * (j & 3)];
-                st_shared_v4(stage_buf + lane * 128 + ((j ^ (lane & 7)) << 4), v[0], v[1], v[2], v[3]);
+                st_shared_v4(box + lane * 128 + ((j ^ (lane & 7)) << 4), v[0], v[1], v[2], v[3]);
               }
               fence_proxy_async_smem();
               __syncwarp();
               if (lane == 0) {
-                tma_store_3d(&maps.result, stage_buf, t.col_row + c + i * 32, lane_first, t.group);
+                tma_store_3d(&maps.result, box, t.col_row + c + i * 32, lane_first, t.group);
                 tma_store_commit();
               }
             }
