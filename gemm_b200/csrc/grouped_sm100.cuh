@@ -725,6 +725,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       // pairs: two loads are issued before the first is waited for.  The accumulator goes back after
       // the last of them.
       auto pull = [&](int c, uint32_t (&w)[4][16]) {
+        __syncwarp();   // the aligned loads need the warp converged after its predicated stores
         if (t.blocks > 0) {
           constexpr int kBatch = 2;
 #pragma unroll
@@ -814,6 +815,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         bool ok = true;
         auto send = [&](int c, int n) {
           uint32_t r[16];
+          __syncwarp();   // the aligned load needs the warp converged after its predicated stores
           if (t.blocks > 0) {
             tmem_ld_32x32b_x16(tmem_base + acc * Cfg::kCols + lane_base + c, r);
             tmem_ld_wait();

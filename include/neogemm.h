@@ -5,6 +5,9 @@
  * reference's PyTorch-extension function neoGemmV1(A, B, C) (nemgemmV03.cu:343-391; older name
  * neogemm(), neogemmV02.cu:262-303), driven by benchmark.py:24.
  *
+ * Beside it, two relatives: the same product per group of a ragged batch, with its gradients
+ * (neogemm_grouped_*), and products of matrices held in 4 bits (neogemm_mxfp4_*).
+ *
  * Plain pointers and sizes only: no torch or C++ types cross this boundary.  All device pointers
  * must belong to the CUDA device that is current on the calling thread.  Calls are asynchronous
  * with respect to the host unless stated otherwise; `stream` is a cudaStream_t passed as void*
