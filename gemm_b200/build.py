@@ -72,8 +72,10 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     failed = [cmd for cmd, process in running if process.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
-    subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", str(LIB_PATH), *objects], check=True,
-                   cwd=str(ROOT))
+    # With a soname the extension finds the copy that a process has loaded already, even if the file was
+    # rebuilt since: two copies would have two sets of overrides and error records.
+    subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-Xlinker", "-soname", "-Xlinker", LIB_PATH.name,
+                    "-o", str(LIB_PATH), *objects], check=True, cwd=str(ROOT))
     return LIB_PATH
 
 

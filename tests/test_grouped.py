@@ -127,3 +127,24 @@ def test_python_face_refuses_cpu_tensors_and_other_things():
         ops.matmul_mxfp4(x, x)
     with pytest.raises(TypeError):
         ops.dequantize_mxfp4(None)
+
+
+def test_extension_and_ctypes_share_one_library(tmp_path):
+    """Also when the library file is replaced between the two loads (a rebuild in a running session)."""
+    import subprocess
+    import sys
+    script = """
+import os, shutil, sys, torch
+from gemm_b200 import _lib
+path = str(_lib.LIB_PATH)
+copy = sys.argv[1]
+shutil.copy2(path, copy)          # another file of the same name takes its place, then the first returns
+os.replace(copy, path)
+import neoGEMM
+maps = {line.split()[-1] + line.split()[4] for line in open('/proc/self/maps') if 'libneogemm' in line}
+assert len({m.replace(' (deleted)', '') for m in maps}) == 1, maps
+print('one')
+"""
+    target = _lib.LIB_PATH.with_name("libneogemm.replaced.so")
+    out = subprocess.run([sys.executable, "-c", script, str(target)], cwd=str(build.ROOT), capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.strip() == "one", out.stderr[-500:]
