@@ -214,21 +214,31 @@ int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, Gr
 //   MXFP4, the same groups:          0.25: 11.0 8.8 9.5              4: 32.0 24.6 24.9    16: 44.2 29.9 26.3
 //   MXFP4, one matrix 28672 x 8192:  16: 23.3 26.5 26.8              64: 26.1 30.7 28.2   128: 38.4 36.2 30.3
 // MXFP4 tiles of several groups reach over the batch's frame of 128 rows, so the pairs pay off from
-// 8 rows a group on; a single matrix has no such waste.  Pairs need tiles to go round, though: with
-// at most 16 of them and a long contraction its split wins (512 x 1024 x 8192 in MXFP4: 10.6 against
-// 15.5).  Below, the four-way split is taken where each CTA still has several k-blocks of a tile, or
-// where there is at most about one tile per cluster (8 groups of 1024 x 1024, 2 rows: 5.7 6.5 7.7).
-int variant_of(int op, int64_t groups, int64_t T, int64_t lanes, int64_t depth) {
+// 8 rows a group on; a single matrix has no such waste.  Where a few long tiles would leave most pairs
+// idle their contraction is split after all: estimated in k-blocks, eight of which stand for a tile's
+// start and end (512 x 1024 x 8192 in MXFP4: 10.6 15.5 for four-way and pairs; dX of 946 rows, 8
+// groups of 3704 x 424: 20.3 27.5).  Below, the four-way split is taken where each CTA still has several
+// k-blocks of a tile, or where there is at most about one tile per cluster (8 groups of 1024 x 1024,
+// 2 rows: 5.7 6.5 7.7); many tiles of a short contraction have nothing to split (dX of 373 rows, 52
+// groups of 112 x 1344: 23.3 14.9 10.0).
+int variant_of(int op, int64_t groups, int64_t T, int64_t lanes, int64_t depth, int sm_count) {
   const int forced = tuning_value(13);
   if (forced >= 0) return forced;
   const bool mx = op == kMxNt;
   const int64_t blocks = ceil_div(depth, mx ? 256 : 64), rows = T / groups;
   const int64_t wide_from = mx ? (groups == 1 ? 96 : 8) : op == kGroupedDx ? 16 : 32;
   if (rows >= wide_from) {
-    const int64_t tiles = ceil_div(lanes, 256) * (groups == 1 ? ceil_div(T, 256) : groups);
-    if (tiles > 16 || blocks < 16 || rows > 1024) return kWide;
+    const int64_t tiles = ceil_div(lanes, 256) * groups * ceil_div(rows, 256);
+    const int64_t split_tiles = ceil_div(lanes, 128) * groups * ceil_div(rows, 128);
+    const int64_t pairs = std::max(sm_count / 2, 1), fours = std::max(sm_count * 2 / 9, 1);
+    const int64_t wide = ceil_div(tiles, pairs) * (blocks + 8);
+    const int64_t two = ceil_div(split_tiles, pairs) * (ceil_div(blocks, 2) + 8);
+    const int64_t four = ceil_div(split_tiles, fours) * (ceil_div(blocks, 4) + 8);
+    if (4 * wide <= 5 * std::min(two, four)) return kWide;
+    return four < two ? kNarrow : kMiddle;
   }
   const int64_t tiles = ceil_div(lanes, 128) * std::min(groups, T);
+  if (tiles > 148 && blocks < 8) return kWide;
   return blocks >= (mx ? 16 : 24) || tiles <= 40 ? kNarrow : kMiddle;
 }
 
@@ -257,7 +267,7 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  const KernelEntry& k = kKernels[op][variant_of(op, groups, T, lanes, depth)];
+  const KernelEntry& k = kKernels[op][variant_of(op, groups, T, lanes, depth, dev.sm_count)];
   GroupedParams p;
   std::memset(&p, 0, sizeof(p));
   p.offsets = offsets;
@@ -315,7 +325,7 @@ int mx_rows(const void* Xc, const void* Xs, const void* Wc, const void* Ws, void
   int rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  const KernelEntry& k = kKernels[kMxNt][variant_of(kMxNt, groups, T, N, K)];
+  const KernelEntry& k = kKernels[kMxNt][variant_of(kMxNt, groups, T, N, K, dev.sm_count)];
   const int64_t k_tiles = ceil_div(K, 128), w_tiles = ceil_div(N, 128), x_tiles = ceil_div(T, 128);
   if (groups * w_tiles * k_tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
   GroupedParams p;
@@ -391,14 +401,14 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   rc = acquire_device(&dev);
   if (rc != NEOGEMM_OK) return rc;
 
-  // Tiles of 128 x 128 on single CTAs, or 256 x 256 on pairs where many of them go round, or enough with
-  // a long contraction each.  Measured, us, single / pairs: 8 groups of 1024 x 2048 with 64 rows 10.1
-  // 11.6, 256 rows 16.0 16.1, 2048 rows 65 60; of 4096 x 4096 with 64 rows 58 61, 512 rows 171 141,
-  // 2048 rows 474 403; 4 groups of 256 x 512 with 2048 rows 11.8 18.9.
+  // Tiles of 128 x 128 on single CTAs, or 256 x 256 on pairs where those have a tile each and a
+  // contraction that is longer than writing its result.  Measured, us, single / pairs: 32 groups of
+  // 2048 x 1024 with 32 rows 29.4 32.4, 128 rows 40.7 41.9, 512 rows 88.6 76.8; of 27 groups of
+  // 2608 x 1032 with 12 rows 37.1 40.6, 128 rows 55.8 53.6; 8 groups of 1024 x 2048 with 64 rows
+  // 10.1 11.6; 4 groups of 256 x 512 with 2048 rows 11.8 18.9.
   const int forced = tuning_value(13);
   const int64_t pair_tiles = groups * ceil_div(N, 256) * ceil_div(K, 256);
-  const bool wide = forced >= 0 ? forced == kWide
-                                : pair_tiles >= 592 || (pair_tiles >= 148 && T / groups >= 256);
+  const bool wide = forced >= 0 ? forced == kWide : pair_tiles >= 148 && T / groups >= 128;
   const KernelEntry& k = kKernels[kGroupedDw][wide ? kWide : kNarrow];
   GroupedMaps maps;
   std::memset(&maps, 0, sizeof(maps));

@@ -104,16 +104,17 @@ struct GroupedConfig {
   // bound by shared memory - 256 x 128 reads and fills 192 bytes per cycle of the 128 there are - and
   // its eight epilogue warps pull the accumulator into registers, packed, before they store anything.
   static constexpr int kAccs = (kOp == kMxNt && kCtaGroup == 2) ? 1 : 2;
-  // dW of short groups is bound by writing the result: eight warps there, too.
+  // Eight warps also where short contractions are bound by writing their result; Y and dX on pairs
+  // read their matrices for longer than four take (eight groups of 256 rows: 79.6 82.7).
   static constexpr int kEpiWarps = (kAccs == 1 || (kOp == kGroupedDw && kCtaGroup == 2)) ? 8 : 4;
   static constexpr int kEpiCols = kCols * 4 / kEpiWarps;   // columns that a warp stores at most
-  // Per warp two buffers of 32 x 32 bf16; streaming: two buffers for the partial sums of 128 lanes
-  // x 16 columns in fp32 (from kSplit CTAs 128 / kSplit lanes each).
+  // Per warp 32 x 32 bf16; streaming: two buffers for the partial sums of 128 lanes x 16 columns in
+  // fp32 (from kSplit CTAs 128 / kSplit lanes each).
   static constexpr int kPartCols = 16;
   static constexpr int kPartBytes = 128 * kPartCols * 4;
   // dW: one or two boxes of 32 x 64 bf16 per warp.
   static constexpr int kBoxBufs = (kOp == kGroupedDw && kCtaGroup == 1) ? 2 : 1;
-  static constexpr int kEpiWarpBytes = 4096 * kBoxBufs;
+  static constexpr int kEpiWarpBytes = (kOp == kGroupedDw || kStream) ? 4096 * kBoxBufs : 2048;
   static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
   static_assert(!kStream || kEpiBytes >= 2 * kPartBytes, "partial sums");
   static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
@@ -694,7 +695,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     const int first_col = (warp - 2) / 4 * Cfg::kEpiCols;   // and its share of the columns
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t stage_buf = epi_base + (warp - 2) * Cfg::kEpiWarpBytes;
-    uint32_t buf = 0;
+    uint32_t buf = 0;   // dW: the warp's next box
     int count = 0;
     int parts = 0;   // column groups of partial sums so far
     for (; tiles.take(p, t); ++tile) {
@@ -721,83 +722,101 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           else mbar_arrive(tmem_empty_bar + 8 * acc);
         }
       };
-      // Up to four times 32 columns of this warp's lanes from `c`, rounded to bf16 and packed in
-      // pairs: two loads are issued before the first is waited for.  The accumulator goes back after
-      // the last of them.
+      // Up to four times 32 columns of this warp's lanes from `c`, rounded to bf16 and packed in pairs of
+      // columns: lane by lane for dW, else as fragments of 8 x 8 matrices, which leave transposed.
+      // The accumulator goes back after the last load.
       auto pull = [&](int c, uint32_t (&w)[4][16]) {
         __syncwarp();   // the aligned loads need the warp converged after its predicated stores
-        if (t.blocks > 0) {
-          constexpr int kBatch = 2;
-#pragma unroll
-          for (int h = 0; h < 4; h += kBatch) {
-            uint32_t r[kBatch][32];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-              if (in_use(c + (h + i) * 32))
-                tmem_ld_32x32b_x32(tmem_base + acc * Cfg::kCols + lane_base + c + (h + i) * 32, r[i]);
-            tmem_ld_wait();
-            if (h + kBatch == 4 && c + 128 >= cols_end) hand_back();
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                w[h + i][j] = pack_bf16x2(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1]));
-          }
-        } else {
+        if (t.blocks == 0) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[i][j] = 0u;
+          return;
+        }
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {
+          uint32_t r[2][32];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t at = tmem_base + acc * Cfg::kCols + lane_base + c + (h + i) * 32;
+            if (in_use(c + (h + i) * 32)) {
+              if constexpr (kDw) {
+                tmem_ld_32x32b_x32(at, r[i]);
+              } else {
+                tmem_ld_16x256b_x4(at, reinterpret_cast<uint32_t(&)[16]>(r[i][0]));
+                tmem_ld_16x256b_x4(at + (16u << 16), reinterpret_cast<uint32_t(&)[16]>(r[i][16]));
+              }
+            }
+          }
+          tmem_ld_wait();
+          if (h == 2 && c + 128 >= cols_end) hand_back();
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[h + i][j] = pack_bf16x2(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1]));
         }
       };
+      // A block of 32 rows x 32 values of the result through shared memory: 64 bytes a row, 16-byte units
+      // swizzled against conflicts.
       auto store = [&](int c, const uint32_t (&w)[16]) {
-        const uint32_t s = stage_buf + buf * 2048;
-        buf ^= 1;
-        // 16 bytes of the result at `dst`, of which `left` values exist.
-        auto put = [&](__nv_bfloat16* dst, const uint32_t (&v)[4], int left) {
-          if (p.vector_out && left >= 8) {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (j < left)
-                reinterpret_cast<unsigned short*>(dst)[j] =
-                    static_cast<unsigned short>(v[j >> 1] >> ((j & 1) * 16));
-          }
-        };
+        const uint32_t s = stage_buf;
+        auto unit_at = [&](int row, int unit) { return s + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4); };
+        __syncwarp();   // the previous block has been read
         if constexpr (kDw) {
-          // Lane = row of the result: 64 bytes of it, 16-byte units swizzled against conflicts.
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            st_shared_v4(s + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[4 * j], w[4 * j + 1],
-                         w[4 * j + 2], w[4 * j + 3]);
-          __syncwarp();
+            st_shared_v4(unit_at(lane, j), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        } else {
+          // Eight rows of the batch at a time: w[2 u + s + 8 h] holds columns 8 u .. of lanes 16 h + 8 s ..
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            st_matrix_x4_trans(unit_at(u * 8 + (lane & 7), lane >> 3), w[2 * u], w[2 * u + 1],
+                               w[8 + 2 * u], w[8 + 2 * u + 1]);
+        }
+        __syncwarp();
+        // Rows [from, to) of the block exist, and `width` values of each.
+        const int from = kDw ? 0 : max(t.lo - c, 0);
+        const int to = kDw ? min(lane_end - lane_first, 32) : min(t.hi - c, 32);
+        const int width = kDw ? t.hi - c : lane_end - lane_first;
+        __nv_bfloat16* first =
+            kDw ? p.out + t.group * p.out_stack + lane_first * p.out_pitch + t.col_row + c
+                : p.out + static_cast<long long>(t.col_row + c) * p.out_pitch + lane_first;
+        if (p.vector_out) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
+            const int left = width - unit * 8;
+            if (row < from || row >= to || left <= 0) continue;
             uint32_t v[4];
-            ld_shared_v4(s + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4), v);
-            const int n = lane_first + row, col = c + unit * 8;
-            if (n < lane_end && col < t.hi)
-              put(p.out + t.group * p.out_stack + n * p.out_pitch + t.col_row + col, v, t.hi - col);
+            ld_shared_v4(unit_at(row, unit), v);
+            __nv_bfloat16* dst = first + row * p.out_pitch + unit * 8;
+            if (left >= 8) {
+              *reinterpret_cast<uint4*>(dst) = make_uint4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (j < left)
+                  reinterpret_cast<unsigned short*>(dst)[j] =
+                      static_cast<unsigned short>(v[j >> 1] >> ((j & 1) * 16));
+            }
           }
         } else {
-          // Lane = column of the result: transposed through shared memory, 32 values of one row
-          // of the batch side by side.
+          // Rows that do not start on 16 bytes: a row per instruction, 64 bytes side by side.
+          // (Eight values per lane, as above, took three times as long for 310 x 127: 20.3 and 7.9 us.)
+#pragma unroll 1
+          for (int row0 = 0; row0 < 32; row0 += 4) {
+            unsigned short v[4];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            st_shared_b16(s + 2 * j * 64 + lane * 2, static_cast<unsigned short>(w[j]));
-            st_shared_b16(s + (2 * j + 1) * 64 + lane * 2, static_cast<unsigned short>(w[j] >> 16));
-          }
-          __syncwarp();
+            for (int i = 0; i < 4; ++i)
+              v[i] = ld_shared_b16(unit_at(row0 + i, lane >> 3) + (lane & 7) * 2);
+            unsigned short* dst =
+                reinterpret_cast<unsigned short*>(first + row0 * p.out_pitch) + lane;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = c + i * 8 + static_cast<int>(lane >> 2), unit = static_cast<int>(lane & 3);
-            uint32_t v[4];
-            ld_shared_v4(s + (row - c) * 64 + unit * 16, v);
-            const int col = lane_first + unit * 8;
-            if (row >= t.lo && row < t.hi && col < lane_end)
-              put(p.out + static_cast<long long>(t.col_row + row) * p.out_pitch + col, v, lane_end - col);
+            for (int i = 0; i < 4; ++i)
+              if (row0 + i >= from && row0 + i < to && static_cast<int>(lane) < width)
+                dst[i * p.out_pitch] = v[i];
           }
         }
       };

@@ -528,6 +528,34 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
       : "memory");
 }
 
+// Sixteen lanes (`taddr`'s and the next fifteen) x 32 fp32 columns, dealt out like matrix fragments: of
+// every eight columns the thread holds columns 2 (lane % 4) and the next of rows lane / 4 (registers 0,
+// 1) and lane / 4 + 8 (2, 3).
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Stores four 8 x 8 matrices of 16-bit values, given as fragments, transposed: lane l gives the address
+// of row l % 8 (16 bytes) of the transpose of matrix l / 8.
+__device__ __forceinline__ void st_matrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                                   uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared::cta.b16 [%0], {%1, %2, %3, %4};"
+               ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ unsigned short ld_shared_b16(uint32_t addr) {
+  unsigned short v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
