@@ -36,7 +36,7 @@ KernelEntry make_entry() {
                      Cfg::kSmemBytes, Cfg::kThreads};
 }
 
-// [operation][variant]
+// [operation][variant]; the middle one of dW splits its contraction, the narrow one does not
 enum Variant : int { kNarrow = 0, kWide = 1, kMiddle = 2, kVariants = 3 };
 const KernelEntry kKernels[4][kVariants] = {
     {make_entry<GroupedConfig<kGroupedNt, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kGroupedNt, 2, 1, 256, 6>>(),
@@ -44,7 +44,7 @@ const KernelEntry kKernels[4][kVariants] = {
     {make_entry<GroupedConfig<kGroupedDx, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 1, 256, 6>>(),
      make_entry<GroupedConfig<kGroupedDx, 1, 2, 128, 8>>()},
     {make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 5>>(), make_entry<GroupedConfig<kGroupedDw, 2, 1, 256, 5>>(),
-     make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 5>>()},
+     make_entry<GroupedConfig<kGroupedDw, 1, 4, 128, 5>>()},
     {make_entry<GroupedConfig<kMxNt, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 2, 1, 256, 5>>(),
      make_entry<GroupedConfig<kMxNt, 1, 2, 128, 8>>()},
 };
@@ -234,7 +234,7 @@ int variant_of(int op, int64_t groups, int64_t T, int64_t lanes, int64_t depth, 
     const int64_t wide = ceil_div(tiles, pairs) * (blocks + 8);
     const int64_t two = ceil_div(split_tiles, pairs) * (ceil_div(blocks, 2) + 8);
     const int64_t four = ceil_div(split_tiles, fours) * (ceil_div(blocks, 4) + 8);
-    if (4 * wide <= 5 * std::min(two, four)) return kWide;
+    if (5 * wide <= 7 * std::min(two, four)) return kWide;
     return four < two ? kNarrow : kMiddle;
   }
   const int64_t tiles = ceil_div(lanes, 128) * std::min(groups, T);
@@ -406,10 +406,20 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   // 2048 x 1024 with 32 rows 29.4 32.4, 128 rows 40.7 41.9, 512 rows 88.6 76.8; of 27 groups of
   // 2608 x 1032 with 12 rows 37.1 40.6, 128 rows 55.8 53.6; 8 groups of 1024 x 2048 with 64 rows
   // 10.1 11.6; 4 groups of 256 x 512 with 2048 rows 11.8 18.9.
+  // Few tiles of a long contraction share it in clusters of four, at the cost of 14 blocks of 64 rows a
+  // tile.  Single / four: one group of 128 x 128 with 1024 rows 5.8 6.6, 2048 rows 8.2 7.4; 4 groups of
+  // 256 x 512 with 1024 rows 7.7 8.0, 2048 rows 11.3 9.2; 8 of them with 2048 rows 12.3 13.6, 4096 rows
+  // 27.9 20.9.
   const int forced = tuning_value(13);
   const int64_t pair_tiles = groups * ceil_div(N, 256) * ceil_div(K, 256);
-  const bool wide = forced >= 0 ? forced == kWide : pair_tiles >= 148 && T / groups >= 128;
-  const KernelEntry& k = kKernels[kGroupedDw][wide ? kWide : kNarrow];
+  const int64_t single_tiles = groups * ceil_div(N, 128) * ceil_div(K, 128);
+  const int64_t blocks = ceil_div(T, 64 * groups), fours = std::max(dev.sm_count * 2 / 9, 1);
+  int variant = kNarrow;
+  if (pair_tiles >= 148 && T / groups >= 128) variant = kWide;
+  else if (single_tiles <= dev.sm_count && ceil_div(single_tiles, fours) * (blocks + 56) < 4 * blocks)
+    variant = kMiddle;
+  if (forced >= 0) variant = forced;
+  const KernelEntry& k = kKernels[kGroupedDw][variant];
   GroupedMaps maps;
   std::memset(&maps, 0, sizeof(maps));
   if (T > 0) {
