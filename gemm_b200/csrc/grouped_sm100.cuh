@@ -111,6 +111,10 @@ struct GroupedConfig {
   // read their matrices for longer than four take (eight groups of 256 rows: 79.6 82.7).
   static constexpr int kEpiWarps = (kAccs == 1 || (kOp == kGroupedDw && kCtaGroup == 2)) ? 8 : 4;
   static constexpr int kEpiCols = kCols * 4 / kEpiWarps;   // columns that a warp stores at most
+  // And takes into registers at a time: all of them where the next tile waits for it, else half, so that
+  // nothing spills (of 227 KB shared memory no cache is left: in the MXFP4 pair a spill of 100 words
+  // cost 16 us of 77).
+  static constexpr int kPull = kAccs == 1 ? 128 : 64;
   // Per warp 32 x 32 bf16; streaming: two buffers for the partial sums of 128 lanes x 16 columns in
   // fp32 (from kSplit CTAs 128 / kSplit lanes each).
   static constexpr int kPartCols = 16;
@@ -694,6 +698,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     }
   } else if (warp < 2 + Cfg::kEpiWarps) {
     // ======================= epilogue =======================
+    constexpr int kPull = Cfg::kPull;
     const int quad = warp & 3;   // the warp's quarter of the tensor-memory lanes
     const int first_col = (warp - 2) / 4 * Cfg::kEpiCols;   // and its share of the columns
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
@@ -725,20 +730,20 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           else mbar_arrive(tmem_empty_bar + 8 * acc);
         }
       };
-      // Up to four times 32 columns of this warp's lanes from `c`, rounded to bf16 and packed in pairs of
+      // Up to kPull columns of this warp's lanes from `c`, rounded to bf16 and packed in pairs of
       // columns: lane by lane for dW, else as fragments of 8 x 8 matrices, which leave transposed.
       // The accumulator goes back after the last load.
-      auto pull = [&](int c, uint32_t (&w)[4][16]) {
+      auto pull = [&](int c, uint32_t (&w)[kPull / 32][16]) {
         __syncwarp();   // the aligned loads need the warp converged after its predicated stores
         if (t.blocks == 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < kPull / 32; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[i][j] = 0u;
           return;
         }
 #pragma unroll
-        for (int h = 0; h < 4; h += 2) {
+        for (int h = 0; h < kPull / 32; h += 2) {
           uint32_t r[2][32];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -753,7 +758,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             }
           }
           tmem_ld_wait();
-          if (h == 2 && c + 128 >= cols_end) hand_back();
+          if ((h + 2) * 32 == kPull && c + kPull >= cols_end) hand_back();
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -916,14 +921,14 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       } else {
         const int c_first = max(first_col, t.lo & ~31);
         if (!in_use(c_first)) hand_back();
-        for (int c = c_first; in_use(c); c += 128) {
-          uint32_t w[4][16];
+        for (int c = c_first; in_use(c); c += kPull) {
+          uint32_t w[kPull / 32][16];
           pull(c, w);
           if (kDw && p.vector_out) {
             // 32 rows x 64 columns through the warp's 4 KB as one swizzled box (dW of short groups is
             // bound by its stores).
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
+            for (int i = 0; i < kPull / 32; i += 2) {
               if (!in_use(c + i * 32)) continue;
               if (lane == 0) tma_store_wait_read<Cfg::kBoxBufs - 1>();
               __syncwarp();
@@ -944,7 +949,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             continue;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < kPull / 32; ++i)
             if (in_use(c + i * 32)) store(c + i * 32, w[i]);
         }
       }

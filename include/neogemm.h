@@ -323,7 +323,8 @@ int neogemm_set_override(int cta_group, int block_n, int swap, int stream_k, int
  *          them, applies the epilogue and stores C; 0: wide tiles are not cut at all and the
  *          last contributor of a cut narrow tile sums it alone (the earlier behaviour).
  *   key 13: kernels of the grouped and MXFP4 products: -1 chosen from the average rows of a group,
- *          0 contraction split over four CTAs, 1 wide tiles on CTA pairs, 2 split over two CTAs.
+ *          0 contraction split over four CTAs, 1 wide tiles on CTA pairs, 2 split over two CTAs
+ *          (dW: 0 tiles on single CTAs, 2 split over four).
  *   key 12: 128 x 64 tiles for small problems (twice as many CTAs as 128 x 128 tiles): -1 when
  *          the 128 x 128 tiles would occupy at most half of the SMs, 0 never, 1 whenever the
  *          single-CTA 128 x 128 TMA-store kernel would be used.
