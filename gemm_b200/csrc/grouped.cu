@@ -209,18 +209,18 @@ int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, Gr
 
 // Which kernel serves a product, from the average rows of a group (the groups themselves are known to
 // the GPU only).  Measured, us, four-way / two-way split / pairs:
-//   bf16, 32 groups of 3584 x 2048:  2 rows a group 56.7 57.6 60.1   32: 81.4 83.2 81.8   128: 148 115 91
-//   dX, the same groups:             2: 57.0 58.8 62.0               16: 75.7 74.8 74.7   64: 87.6 83.4 79.2
-//   MXFP4, the same groups:          0.25: 11.0 8.8 9.5              4: 32.0 24.6 24.9    16: 44.2 29.9 26.3
-//   MXFP4, one matrix 28672 x 8192:  16: 23.3 26.5 26.8              64: 26.1 30.7 28.2   128: 38.4 36.2 30.3
+//   bf16, 32 groups of 3584 x 2048:  2 rows a group 55.5 56.7 58.0   32: 80.1 81.5 79.6   128: 150 113 88
+//   dX, the same groups:             2: 56.3 57.9 61.5               16: 75.4 72.7 73.0   64: 86.3 82.1 77.0
+//   MXFP4, the same groups:          0.25: 10.6 8.1 8.5              4: 32.5 24.0 23.8    16: 44.4 29.5 25.1
+//   MXFP4, one matrix 28672 x 8192:  16: 23.0 25.5 25.7              64: 25.6 29.8 26.8   128: 38.4 35.3 28.6
 // MXFP4 tiles of several groups reach over the batch's frame of 128 rows, so the pairs pay off from
 // 8 rows a group on; a single matrix has no such waste.  Where a few long tiles would leave most pairs
 // idle their contraction is split after all: estimated in k-blocks, eight of which stand for a tile's
-// start and end (512 x 1024 x 8192 in MXFP4: 10.6 15.5 for four-way and pairs; dX of 946 rows, 8
-// groups of 3704 x 424: 20.3 27.5).  Below, the four-way split is taken where each CTA still has several
-// k-blocks of a tile, or where there is at most about one tile per cluster (8 groups of 1024 x 1024,
-// 2 rows: 5.7 6.5 7.7); many tiles of a short contraction have nothing to split (dX of 373 rows, 52
-// groups of 112 x 1344: 23.3 14.9 10.0).
+// start and end (512 x 1024 x 8192 in MXFP4: 10.5 13.4 14.2; dX of 946 rows, 8 groups of 3704 x 424:
+// 21.1 20.1 27.6); a ratio of 1.4 allows for the exchange of partial sums.  Below, the four-way split is
+// taken where each CTA still has several k-blocks of a tile, or where there is at most about one tile per
+// cluster (8 groups of 1024 x 1024, 2 rows: 4.9 5.7 6.4); many tiles of a short contraction have nothing
+// to split (dX of 373 rows, 52 groups of 112 x 1344: 23.1 14.7 8.1).
 int variant_of(int op, int64_t groups, int64_t T, int64_t lanes, int64_t depth, int sm_count) {
   const int forced = tuning_value(13);
   if (forced >= 0) return forced;
@@ -403,13 +403,13 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
 
   // Tiles of 128 x 128 on single CTAs, or 256 x 256 on pairs where those have a tile each and a
   // contraction that is longer than writing its result.  Measured, us, single / pairs: 32 groups of
-  // 2048 x 1024 with 32 rows 29.4 32.4, 128 rows 40.7 41.9, 512 rows 88.6 76.8; of 27 groups of
-  // 2608 x 1032 with 12 rows 37.1 40.6, 128 rows 55.8 53.6; 8 groups of 1024 x 2048 with 64 rows
-  // 10.1 11.6; 4 groups of 256 x 512 with 2048 rows 11.8 18.9.
+  // 2048 x 1024 with 32 rows 31.5 33.0, 128 rows 40.7 42.3, 512 rows 89.3 77.0; of 27 groups of
+  // 2608 x 1032 with 12 rows 37.5 40.8, 128 rows 56.2 54.1; 8 groups of 1024 x 2048 with 64 rows
+  // 10.4 11.9; 4 groups of 256 x 512 with 2048 rows 11.4 18.4.
   // Few tiles of a long contraction share it in clusters of four, at the cost of 14 blocks of 64 rows a
-  // tile.  Single / four: one group of 128 x 128 with 1024 rows 5.8 6.6, 2048 rows 8.2 7.4; 4 groups of
-  // 256 x 512 with 1024 rows 7.7 8.0, 2048 rows 11.3 9.2; 8 of them with 2048 rows 12.3 13.6, 4096 rows
-  // 27.9 20.9.
+  // tile.  Single / four: one group of 128 x 128 with 1024 rows 5.8 6.6, 2048 rows 8.2 7.3; 4 groups of
+  // 256 x 512 with 1024 rows 7.8 8.1, 2048 rows 11.4 9.4; 8 of them with 2048 rows 12.4 13.9, 4096 rows
+  // 28.2 21.0.
   const int forced = tuning_value(13);
   const int64_t pair_tiles = groups * ceil_div(N, 256) * ceil_div(K, 256);
   const int64_t single_tiles = groups * ceil_div(N, 128) * ceil_div(K, 128);

@@ -74,7 +74,7 @@ struct GroupedParams {
 // whole tiles, two rounds on 148 SMs for 1.14 rounds of work).  Two ways of evening out the lanes
 // instead were slower: tiles of fewer lanes take as many k-blocks, each with its fixed cost, and
 // contiguous runs per SM scatter the addresses that are read at a time (32 groups of 3584 x 2048:
-// 102 us against 86).
+// 102 us against 86 when this was tried).
 //
 // dW with kSplit > 1: for few tiles of a long contraction (two groups of 840 x 408 with 9254 rows:
 // 42.2 us on single CTAs, 23 on clusters of four).
@@ -108,7 +108,8 @@ struct GroupedConfig {
   // its eight epilogue warps pull the accumulator into registers, packed, before they store anything.
   static constexpr int kAccs = (kOp == kMxNt && kCtaGroup == 2) ? 1 : 2;
   // Eight warps also where short contractions are bound by writing their result; Y and dX on pairs
-  // read their matrices for longer than four take (eight groups of 256 rows: 79.6 82.7).
+  // read their matrices for longer than four take (32 groups of 3584 x 2048, 1001 rows: 79.6 us, and
+  // 82.7 with eight).
   static constexpr int kEpiWarps = (kAccs == 1 || (kOp == kGroupedDw && kCtaGroup == 2)) ? 8 : 4;
   static constexpr int kEpiCols = kCols * 4 / kEpiWarps;   // columns that a warp stores at most
   // And takes into registers at a time: all of them where the next tile waits for it, else half, so that
