@@ -10,6 +10,7 @@
 //   * failures raise RuntimeError (the reference prints to stderr, nemgemmV03.cu:387-390).
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -102,6 +103,13 @@ Rows rows_operand(const torch::Tensor& t, const char* name, const torch::Tensor&
   return Rows{t.size(0), t.size(1), t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 8 * 8};
 }
 
+// A result is written while the operands are read.  (Views whose overlap takes a search are let pass.)
+void check_apart(const torch::Tensor& out, const torch::Tensor& operand, const char* name) {
+  const at::MemOverlapStatus s = at::get_overlap_status(out, operand);
+  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial,
+                    "out must not share memory with ", name);
+}
+
 struct Result {
   torch::Tensor tensor;
   int64_t pitch;
@@ -155,8 +163,14 @@ torch::Tensor grouped_rows(RowsFunction fn, const char* name, bool transposed, c
   TORCH_CHECK_VALUE(r.width == (transposed ? N : K), name, " is [", text(r.count), ",", text(r.width),
                     "] but w is [groups,", text(N), ",", text(K), "]: expected rows of ",
                     text(transposed ? N : K));
+  TORCH_CHECK_VALUE(groups <= 1 || w.stride(0) > 0 || w.numel() == 0,
+                    "w must hold a matrix per group, not one expanded over them");
   c10::cuda::CUDAGuard guard(rows.device());
   Result y = rows_result(out, rows, r.count, transposed ? K : N);
+  if (out.has_value()) {
+    check_apart(*out, rows, name);
+    check_apart(*out, w, "w");
+  }
   check_status(fn(rows.data_ptr(), w.data_ptr(), y.tensor.data_ptr(), offsets.data_ptr(),
                   offsets.scalar_type() == at::kLong, groups, r.count, N, K, r.pitch,
                   N > 1 ? w.stride(1) : (K + 15) / 8 * 8, groups > 1 ? w.stride(0) : 0, y.pitch,
@@ -189,6 +203,8 @@ torch::Tensor grouped_matmul_dw(const torch::Tensor& dy, const torch::Tensor& x,
                       "out must be a contiguous bfloat16 [", text(groups), ",", text(d.width), ",",
                       text(r.width), "] on ",
                       dy.device());
+    check_apart(dw, dy, "dy");
+    check_apart(dw, x, "x");
   } else {
     dw = torch::empty({groups, d.width, r.width}, dy.options());
   }
@@ -266,6 +282,8 @@ torch::Tensor matmul_mxfp4(const torch::Tensor& a, const torch::Tensor& a_scales
                     text(N), ",", text(2 * b.size(1)), "]: K differs");
   c10::cuda::CUDAGuard guard(a.device());
   Result c = rows_result(out, a, M, N);
+  if (out.has_value())
+    for (const torch::Tensor* t : {&a, &a_scales, &b, &b_scales}) check_apart(*out, *t, "an operand");
   check_status(neogemm_mxfp4_nt(a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(),
                                 c.tensor.data_ptr(), M, N, K, c.pitch, stream_of(a)));
   return c.tensor;
@@ -283,6 +301,8 @@ torch::Tensor grouped_matmul_mxfp4(const torch::Tensor& x, const torch::Tensor& 
                     text(groups), ",", text(N), ",", text(2 * w.size(2)), "]: K differs");
   c10::cuda::CUDAGuard guard(x.device());
   Result y = rows_result(out, x, T, N);
+  if (out.has_value())
+    for (const torch::Tensor* t : {&x, &x_scales, &w, &w_scales}) check_apart(*out, *t, "an operand");
   check_status(neogemm_grouped_mxfp4_nt(x.data_ptr(), x_scales.data_ptr(), w.data_ptr(),
                                         w_scales.data_ptr(), y.tensor.data_ptr(), offsets.data_ptr(),
                                         offsets.scalar_type() == at::kLong, groups, T, N, K, y.pitch,

@@ -258,7 +258,7 @@ int grouped_rows(int op, const void* R, const void* W, void* out, const void* of
   if (groups == 0) return zero_rest ? zero_rows(out, ldo, T, lanes, stream) : NEOGEMM_OK;
   if (depth > 0) {
     if (R == nullptr || W == nullptr || ldr < depth || ldw < K) return NEOGEMM_ERR_BAD_ARG;
-    if (groups > 1 && stack_w < 0) return NEOGEMM_ERR_BAD_ARG;
+    if (groups > 1 && stack_w <= 0) return NEOGEMM_ERR_BAD_ARG;
     if (ldr % 8 != 0 || ldw % 8 != 0 || (groups > 1 && stack_w % 8 != 0) || !aligned16(R) ||
         !aligned16(W))
       return NEOGEMM_ERR_UNSUPPORTED;

@@ -174,7 +174,8 @@ int neogemm_noalloc_clear_status(void);
  *   X, dX [T,K] at x[t*ldx + k]; Y, dY [T,N] at y[t*ldy + n];
  *   W [groups,N,K] at w[e*stack_w + n*ldw + k];  dW [groups,N,K] packed.
  * Operands that are read have 16-byte aligned bases and leading dimensions (and stack_w) that are
- * multiples of 8; results may have any leading dimension (16-byte stores need multiples of 8).
+ * multiples of 8, stack_w > 0; results may have any leading dimension (16-byte stores need multiples
+ * of 8) and share no memory with the operands.
  * T, N, K >= 0; an empty group is allowed (its dW is zero).  1 <= groups <= 1024 (0 groups: no-op).
  * zero_rest != 0 writes zeros to the rows of Y or dX that belong to no group (in front of offsets[0],
  * behind offsets[groups]); 0 leaves them as they are.  Sums are added in a fixed order, without

@@ -303,6 +303,30 @@ def test_refusals_on_the_device():
     assert ops.device_status()[0] == 0
 
 
+def test_results_that_share_memory_with_an_operand_and_one_matrix_for_all_are_refused():
+    x = torch.randn(16, 64, device="cuda").bfloat16()
+    w = torch.randn(2, 64, 64, device="cuda").bfloat16()
+    _, off = offsets_of([10, 6])
+    for f in (ops.grouped_matmul, ops.grouped_matmul_dx):
+        with pytest.raises(ValueError, match="share memory"):
+            f(x, w, off, out=x)
+        with pytest.raises(ValueError, match="share memory"):
+            f(x, w, off, out=w.view(128, 64)[8:24])
+        with pytest.raises(ValueError, match="matrix per group"):
+            f(x, w[:1].expand(2, 64, 64), off)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.grouped_matmul_dw(w.view(128, 64)[:16], x, off, out=w)
+    q = ops.quantize_mxfp4(x)
+    with pytest.raises(ValueError, match="share memory"):
+        ops.matmul_mxfp4(q, q, out=q.codes.view(torch.bfloat16)[:, :16])
+    # Other columns of the same rows are fine.
+    both = torch.zeros(16, 128, device="cuda").bfloat16()
+    both[:, :64] = x
+    ops.grouped_matmul(both[:, :64], w, off, out=both[:, 64:])
+    assert torch.equal(both[:, 64:], ops.grouped_matmul(x, w, off)) and torch.equal(both[:, :64], x)
+    assert ops.device_status()[0] == 0
+
+
 def test_as_many_groups_as_there_may_be(tiles):
     counts = [0] * 1024
     for e, c in ((0, 1), (31, 2), (32, 1), (33, 3), (500, 17), (1022, 1), (1023, 40)):
