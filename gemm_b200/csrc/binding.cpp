@@ -12,6 +12,7 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -87,6 +88,11 @@ void check_status(int rc) {
   if (rc != NEOGEMM_OK) pybind11::module_::import("gemm_b200._lib").attr("check")(rc);
 }
 
+// A new tensor beside `like`, past the dispatcher (a quantisation, of two: 5.3 -> 4.7 us on the host).
+torch::Tensor empty_beside(const torch::Tensor& like, at::IntArrayRef shape, at::ScalarType type) {
+  return at::detail::empty_cuda(shape, type, like.device(), c10::nullopt);
+}
+
 struct Rows {
   int64_t count, width, pitch;
 };
@@ -119,7 +125,7 @@ struct Result {
 Result rows_result(const c10::optional<torch::Tensor>& out, const torch::Tensor& like, int64_t rows,
                    int64_t width) {
   if (!out.has_value())
-    return Result{torch::empty({rows, width}, like.options().dtype(at::kBFloat16)),
+    return Result{empty_beside(like, {rows, width}, at::kBFloat16),
                   std::max<int64_t>(width, 1), 1};
   const torch::Tensor& t = *out;
   TORCH_CHECK_VALUE(t.is_cuda(), "out must live on a CUDA device (there is no CPU path)");
@@ -206,7 +212,7 @@ torch::Tensor grouped_matmul_dw(const torch::Tensor& dy, const torch::Tensor& x,
     check_apart(dw, dy, "dy");
     check_apart(dw, x, "x");
   } else {
-    dw = torch::empty({groups, d.width, r.width}, dy.options());
+    dw = empty_beside(dy, {groups, d.width, r.width}, at::kBFloat16);
   }
   check_status(neogemm_grouped_dw(dy.data_ptr(), x.data_ptr(), dw.data_ptr(), offsets.data_ptr(),
                                   offsets.scalar_type() == at::kLong, groups, d.count, d.width, r.width,
@@ -250,11 +256,10 @@ std::pair<torch::Tensor, torch::Tensor> quantize_mxfp4(const torch::Tensor& x) {
   TORCH_CHECK_VALUE(K % 32 == 0, "K must be a multiple of 32, got ", text(K));
   TORCH_CHECK_VALUE(K <= 1 || x.stride(-1) == 1, "x must have unit stride along its last dimension");
   c10::cuda::CUDAGuard guard(x.device());
-  const auto bytes = x.options().dtype(at::kByte);
   c10::SmallVector<int64_t, 3> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = K / 2;
-  torch::Tensor codes = torch::empty(shape, bytes);
-  torch::Tensor scales = torch::empty(scales_shape(x.sizes(), K), bytes);
+  torch::Tensor codes = empty_beside(x, shape, at::kByte);
+  torch::Tensor scales = empty_beside(x, scales_shape(x.sizes(), K), at::kByte);
   check_status(neogemm_mxfp4_quantize(x.data_ptr(), f32, codes.data_ptr(), scales.data_ptr(), stack, rows,
                                       K, rows > 1 ? x.stride(-2) : K, stack > 1 ? x.stride(0) : 0,
                                       stream_of(x)));
@@ -266,7 +271,7 @@ torch::Tensor dequantize_mxfp4(const torch::Tensor& codes, const torch::Tensor& 
   c10::cuda::CUDAGuard guard(codes.device());
   c10::SmallVector<int64_t, 3> shape(codes.sizes().begin(), codes.sizes().end());
   shape.back() *= 2;
-  torch::Tensor out = torch::empty(shape, codes.options().dtype(at::kBFloat16));
+  torch::Tensor out = empty_beside(codes, shape, at::kBFloat16);
   check_status(neogemm_mxfp4_dequantize(codes.data_ptr(), scales.data_ptr(), out.data_ptr(),
                                         shape.size() == 3 ? shape[0] : 1, shape[shape.size() - 2],
                                         shape.back(), stream_of(codes)));
