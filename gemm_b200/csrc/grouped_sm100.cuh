@@ -126,7 +126,7 @@ struct GroupedConfig {
   static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
   static_assert(kSplit == 1 || kEpiBytes >= 2 * kPartBytes, "partial sums");
   static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
-  static constexpr int kBarrierBytes = (3 * kStages + 4 + 2 + 2 * kSplit) * 8 + 16;
+  static constexpr int kBarrierBytes = (3 * kStages + 4 + 2 + 2 + 2 * kSplit) * 8 + 16;
   static constexpr int kRestBytes = kEpiBytes + kTableBytes + 12 + kBarrierBytes + 1024;
   static constexpr int kRingBytes = kStream ? (232448 - kRestBytes) / 1024 * 1024 : kStages * kStageBytes;
   static_assert(kEpiBytes % 1024 == 0, "the ring starts on the swizzle's alignment");
@@ -138,7 +138,10 @@ struct GroupedConfig {
   static constexpr int kTmemNeeded = kAccs * kCols + kScaleSets * kScaleTmemCols;
   static constexpr int kTmemCols = (kCtaGroup == 2) ? 512 : kTmemNeeded <= 128 ? 128
                                  : kTmemNeeded <= 256 ? 256 : 512;
-  static constexpr int kThreads = 64 + 32 * kEpiWarps + ((kOp == kGroupedDw) ? 32 : 0);
+  // Behind the epilogue: the warp that clears rows (dW), and the one that frees buffers of partial sums.
+  static constexpr int kClearWarp = 2 + kEpiWarps;
+  static constexpr int kFreeWarp = kClearWarp + (kOp == kGroupedDw ? 1 : 0);
+  static constexpr int kThreads = 32 * (kFreeWarp + (kSplit > 1 ? 1 : 0));
   // Arrivals that complete a ring slot's phase besides its bytes: the slot's producer, and for
   // dW one per CTA (the last block of a tile is handed over by the warps that cleared its rows).
   static constexpr int kFullArrivals = (kOp == kGroupedDw) ? kCtaGroup : 1;
@@ -200,6 +203,12 @@ __device__ __forceinline__ void make_uniform(GroupedTile& t) {
   t.k_len = uniform(t.k_len);
   t.first_kb = uniform(t.first_kb);
   t.blocks = uniform(t.blocks);
+}
+
+// A wait for a phase that another CTA completes: the polls stay cheap, and one test at cluster scope behind
+// them orders what follows after what that CTA did.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
+  return ptx::mbar_wait(bar, parity, abort_flag) && ptx::mbar_wait<true>(bar, parity, abort_flag);
 }
 
 // Rows [begin, end) of group e, clamped to the batch: indices that are out of order or out of range cost
@@ -408,7 +417,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   const uint32_t tmem_full_bar = clear_bar + 8 * kStages;    // [2]
   const uint32_t tmem_empty_bar = tmem_full_bar + 16;        // [2]
   const uint32_t part_full_bar = tmem_empty_bar + 16;        // [2] partial sums have arrived
-  const uint32_t part_free_bar = part_full_bar + 16;         // [kSplit][2] CTA d's buffer is free
+  const uint32_t part_read_bar = part_full_bar + 16;         // [2] and have been read by this CTA's warps
+  const uint32_t part_free_bar = part_read_bar + 16;         // [kSplit][2] CTA d's buffer is free
   uint8_t* tail_gen = smem_gen + (part_free_bar + 16 * Cfg::kSplit - smem_base);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail_gen);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_gen + 4);
@@ -437,7 +447,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       mbar_init(tmem_full_bar + 8 * a, 1);
       mbar_init(tmem_empty_bar + 8 * a, Cfg::kEpiWarps * kCtaGroup);
       mbar_init(part_full_bar + 8 * a, 1);
-      for (int d = 0; d < Cfg::kSplit; ++d) mbar_init(part_free_bar + 16 * d + 8 * a, 4);
+      mbar_init(part_read_bar + 8 * a, 4);
+      for (int d = 0; d < Cfg::kSplit; ++d) mbar_init(part_free_bar + 16 * d + 8 * a, 1);
     }
     fence_barrier_init();
     if (Cfg::kSplit > 1)
@@ -852,8 +863,8 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             for (int j = 0; j < 16; ++j) r[j] = 0u;
           }
           const uint32_t b = n & 1;
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(part_free_bar + 16 * dest + 8 * b,
-                                                       ((n >> 1) & 1) ^ 1, abort_flag));
+          ok = ok && __all_sync(0xffffffffu, wait_cluster(part_free_bar + 16 * dest + 8 * b,
+                                                          ((n >> 1) & 1) ^ 1, abort_flag));
           if (!ok) return;
           // (Ordinary stores and a release at cluster scope took 1500 cycles: the release waits for
           // every store in flight, those of the result included.)
@@ -864,9 +875,10 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         };
         auto collect = [&](int c, int n) {
           const uint32_t b = n & 1;
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(part_full_bar + 8 * b, (n >> 1) & 1, abort_flag));
+          ok = ok &&
+               __all_sync(0xffffffffu, wait_cluster(part_full_bar + 8 * b, (n >> 1) & 1, abort_flag));
           if (!ok) return;
-          // Arm the buffer for its next use: nothing can arrive before this warp frees it below.
+          // Arm the buffer for its next use: nothing can arrive before this warp has read it, below.
           if (quad == 0 && lane == 0) mbar_arrive_expect_tx(part_full_bar + 8 * b, Cfg::kPartBytes);
           float sum[kOwn / 32][4];
 #pragma unroll
@@ -882,8 +894,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
             }
           }
           __syncwarp();
-          if (lane < kSplit)
-            mbar_arrive_cluster(mapa_u32(part_free_bar + 16 * split_rank + 8 * b, lane));
+          if (lane == 0) mbar_arrive(part_read_bar + 8 * b);
 #pragma unroll
           for (int h = 0; h < kOwn / 32; ++h) {
             const int n_out = t.lane0 + split_rank * kOwn + h * 32 + static_cast<int>(lane);
@@ -974,7 +985,7 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           for (int j = c; j < min(c + 8, p.lanes); ++j) dst[j] = __float2bfloat16_rn(0.f);
       }
     }
-  } else if (kDw) {
+  } else if (kDw && warp == Cfg::kClearWarp) {
     // ======================= rows of the next group =======================
     uint32_t stage = 0, parities = 0;
     bool ok = true;
@@ -1007,6 +1018,27 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         }
       }
       stage = (stage + 1) % kStages;
+    }
+  } else if (Cfg::kSplit > 1) {
+    // ======================= buffers of partial sums: back to the senders =======================
+    // The senders overwrite what this CTA's four warps have read, so the loads have to be ordered in front
+    // of their next stores by a release at cluster scope.  That waits for every store that its own warp
+    // has in flight, which in an epilogue warp are those of the result (28.0 -> 30.7 us for 16 x 28672 x
+    // 8192 in MXFP4, 26.8 -> 35.6 for 32 groups of 3584 x 2048 with two rows each); this warp has none.
+    int n = 0;   // column groups of partial sums so far
+    bool ok = true;
+    for (; ok && tiles.take(p, t); ++tile) {
+      for (int c = t.lo & ~(Cfg::kPartCols - 1); ok && c < t.hi; c += Cfg::kPartCols, ++n) {
+        const uint32_t b = n & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(part_read_bar + 8 * b, (n >> 1) & 1, abort_flag));
+        if (!ok) {
+          if (lane == 0) report_error(p.status, abort_flag, kDevTimeoutEpilogue, tile, 3);
+          break;
+        }
+        if (lane < Cfg::kSplit)
+          mbar_arrive_release_cluster(mapa_u32(part_free_bar + 16 * split_rank + 8 * b, lane));
+        __syncwarp();
+      }
     }
   }
   __syncwarp();

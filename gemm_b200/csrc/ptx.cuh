@@ -106,8 +106,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
-// Arrive on a barrier of the cluster after ordinary stores to shared memory that the other CTA's
-// tensor pipe is going to read (the stores are also fenced towards the async proxy by the caller).
+// The same with a release at cluster scope, for ordinary shared memory: stores that the other CTA's
+// tensor pipe is going to read (also fenced towards the async proxy by the caller), or loads of what the
+// other CTA is going to overwrite.  The other side waits with cluster scope.
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
                : "memory");
