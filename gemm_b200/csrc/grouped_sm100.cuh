@@ -212,7 +212,8 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, cons
 }
 
 // Rows [begin, end) of group e, clamped to the batch: indices that are out of order or out of range cost
-// the result, never an access.  True if they were in order.
+// the result, never an access.  True if they were in order.  If any were not, the ranges still overlap
+// and in_order() has to follow.
 __device__ __forceinline__ bool group_range(const GroupedParams& p, int e, int* begin, int* end) {
   long long b = 0, f = p.rows;
   if (p.offsets != nullptr) {
@@ -230,6 +231,23 @@ __device__ __forceinline__ bool group_range(const GroupedParams& p, int e, int* 
   *begin = static_cast<int>(b);
   *end = static_cast<int>(f);
   return good;
+}
+
+// Ranges of 32 consecutive groups, one per lane, of offsets that were not in order: an index that descends
+// counts as the largest in front of it (`before`, for the first lane).  So no two groups share a row - two
+// tiles would store it - and there are no more tiles than in order.  Returns the largest index so far.
+__device__ __forceinline__ int in_order(int before, int* begin, int* end) {
+  const int lane = static_cast<int>(ptx::lane_id());
+  int top = max(*end, before);
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int other = __shfl_up_sync(0xffffffffu, top, d);
+    if (lane >= d) top = max(top, other);
+  }
+  const int previous = __shfl_up_sync(0xffffffffu, top, 1);
+  *begin = lane > 0 ? previous : max(*begin, before);
+  *end = top;
+  return __shfl_sync(0xffffffffu, top, 31);
 }
 
 // Records offsets that were clamped: the launch is not aborted.
@@ -270,6 +288,7 @@ struct GroupedTiles {
     if (p.groups <= 32) {
       const int lane = static_cast<int>(ptx::lane_id());
       good = group_range(p, min(lane, p.groups - 1), &my_begin, &my_end);
+      if (!__all_sync(0xffffffffu, good)) in_order(0, &my_begin, &my_end);
       const int mine = Cfg::kOp == kGroupedDw || lane >= p.groups
                            ? 0 : column_tiles<Cfg>(p, my_begin, my_end) * p.lane_tiles;
       int scan = mine;
@@ -479,13 +498,22 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   // Global memory from here on: wait for the previous kernel of the stream.
   griddep_wait();
   if (p.groups > 32) {
+    int bad = 0;
     for (int e = threadIdx.x; e < p.groups; e += Cfg::kThreads)
-      if (!group_range(p, e, table.begin + e, table.end + e)) report_offsets(p, e);
-    __syncthreads();
+      if (!group_range(p, e, table.begin + e, table.end + e)) {
+        report_offsets(p, e);
+        bad = 1;
+      }
+    bad = __syncthreads_or(bad);
     if (warp == 0) {
-      int sum = 0;
+      int sum = 0, top = 0;
       for (int base = 0; base < p.groups; base += 32) {
         const int e = base + static_cast<int>(lane);
+        if (bad) {
+          int begin = e < p.groups ? table.begin[e] : 0, end = e < p.groups ? table.end[e] : 0;
+          top = in_order(top, &begin, &end);
+          if (e < p.groups) table.begin[e] = begin, table.end[e] = end;
+        }
         const int mine =
             !kDw && e < p.groups ? column_tiles<Cfg>(p, table.begin[e], table.end[e]) * p.lane_tiles : 0;
         int scan = mine;

@@ -162,9 +162,10 @@ int neogemm_noalloc_clear_status(void);
  * A batch of T rows is sorted by group (expert); group e owns the rows offsets[e] .. offsets[e+1]-1
  * and has a matrix of its own, W[e].  `offsets` is device memory: groups + 1 ascending indices
  * between 0 and T, int32 or (offsets_are_64) int64.  Nothing is read back to the host: the tiles
- * are laid out on the GPU, so a captured graph replays with other group sizes.  Indices that
- * descend or leave [0, T] are clamped (no access outside the operands) and recorded as a device
- * error, code 6 with field 3 = 4 (see neogemm_device_status).
+ * are laid out on the GPU, so a captured graph replays with other group sizes.  An index outside
+ * [0, T] counts as the nearest of the two and one that descends as the largest in front of it (so no
+ * access leaves the operands, and no row has two groups); either is recorded as a device error, code 6
+ * with field 3 = 4 (see neogemm_device_status).
  *
  *   neogemm_grouped_nt   Y[t,n]    = sum_k X[t,k] W[e][n,k]       t in group e
  *   neogemm_grouped_dx   dX[t,k]   = sum_n dY[t,n] W[e][n,k]      its gradient by the rows
