@@ -22,7 +22,6 @@ struct KernelEntry {
   int col_step;    // granularity of a tile's columns
   int lane_box;    // rows of the lane operand's boxes
   int ring_bytes, scale_bytes;   // shared memory: the ring, and the scales of a k-block
-  int scale_sets;  // MXFP4: k-blocks whose scales tensor memory holds
   const void* fn;
   int smem_bytes, threads;
 };
@@ -32,7 +31,7 @@ KernelEntry make_entry() {
   constexpr bool kMnMajor = Cfg::kOp == kGroupedDw || Cfg::kOp == kGroupedDx;   // boxes of 64 x 64
   return KernelEntry{Cfg::kOp, Cfg::kCtaGroup, Cfg::kSplit, Cfg::kCols, Cfg::kStages, Cfg::kLaneTile,
                      Cfg::kColStep, kMnMajor ? 64 : 128, Cfg::kRingBytes, Cfg::kScaleBytes,
-                     Cfg::kScaleSets, reinterpret_cast<const void*>(&grouped_kernel<Cfg>),
+                     reinterpret_cast<const void*>(&grouped_kernel<Cfg>),
                      Cfg::kSmemBytes, Cfg::kThreads};
 }
 
@@ -44,7 +43,7 @@ const KernelEntry kKernels[4][kVariants] = {
     {make_entry<GroupedConfig<kGroupedDx, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kGroupedDx, 2, 1, 256, 6>>(),
      make_entry<GroupedConfig<kGroupedDx, 1, 2, 128, 8>>()},
     {make_entry<GroupedConfig<kGroupedDw, 1, 1, 128, 5>>(), make_entry<GroupedConfig<kGroupedDw, 2, 1, 256, 5>>(),
-     make_entry<GroupedConfig<kGroupedDw, 1, 4, 128, 5>>()},
+     make_entry<GroupedConfig<kGroupedDw, 1, 4, 128, 4>>()},
     {make_entry<GroupedConfig<kMxNt, 1, 4, 128, 8>>(), make_entry<GroupedConfig<kMxNt, 2, 1, 256, 5>>(),
      make_entry<GroupedConfig<kMxNt, 1, 2, 128, 8>>()},
 };
@@ -201,32 +200,39 @@ int fill_rows(const KernelEntry& k, int64_t groups, int64_t T, int64_t lanes, Gr
   if (k.split > 1) {
     // Slots of two k-blocks where four of them fit: half the waits.
     const int block = 128 * 128 + p->col_box * 128 + k.scale_bytes;
-    p->per_slot = k.ring_bytes / (2 * block) >= 4 ? 2 : 1;
-    p->slots = std::min(k.stages, k.ring_bytes / (p->per_slot * block));
+    // Buffers of partial sums for two tiles of the average or more, up to eight: a buffer is free again some
+    // 1200 to 4200 cycles after it was read.  The ring gets the rest of shared memory (32 groups of 3584 x
+    // 2048, bf16, four-way: 24 rows each 90 us with eight buffers, 83 with four; 64 x 28672 x 8192 in MXFP4
+    // 27 with eight, 43 with two).
+    p->part_bufs = cap <= kPartCols ? 2 : T / groups <= 2 * kPartCols ? 4 : kMaxPartBufs;
+    const int ring_bytes = k.ring_bytes - (p->part_bufs - 2) * kPartBytes;
+    p->per_slot = ring_bytes / (2 * block) >= 4 ? 2 : 1;
+    p->slots = std::min(k.stages, ring_bytes / (p->per_slot * block));
   }
   return NEOGEMM_OK;
 }
 
 // Which kernel serves a product, from the average rows of a group (the groups themselves are known to
-// the GPU only).  Measured, us, four-way / two-way split / pairs:
-//   bf16, 32 groups of 3584 x 2048:  2 rows a group 55.5 56.7 58.0   32: 80.1 81.5 79.6   128: 150 113 88
-//   dX, the same groups:             2: 56.3 57.9 61.5               16: 75.4 72.7 73.0   64: 86.3 82.1 77.0
-//   MXFP4, the same groups:          0.25: 10.6 8.1 8.5              4: 32.5 24.0 23.8    16: 44.4 29.5 25.1
-//   MXFP4, one matrix 28672 x 8192:  16: 23.0 25.5 25.7              64: 25.6 29.8 26.8   128: 38.4 35.3 28.6
+// the GPU only).  Measured, us, four-way / two-way split / pairs, groups of equal length:
+//   bf16, 32 groups of 3584 x 2048:  2 rows a group 71.5 73.2 77.1   16: 78.7 81.3 79.3
+//                                    24: 83.3 84.9 80.0              128: 153 105 90
+//   dX, the same groups:             2: 71.8 70.5 71.6   8: 79 72.6 72.9   15: 77 73.0 72.9   64: 93 85 76.8
+//   MXFP4, the same groups:          0.25: 11.2 8.2 8.1  4: 34.5 25.0 24.9   16: 37.1 25.6 25.1
+//   MXFP4, one matrix 28672 x 8192:  16: 22.8 25.5 25.5  64: 27.0 31.6 26.8  96: 33.6 34.8 27.7
 // MXFP4 tiles of several groups reach over the batch's frame of 128 rows, so the pairs pay off from
 // 8 rows a group on; a single matrix has no such waste.  Where a few long tiles would leave most pairs
 // idle their contraction is split after all: estimated in k-blocks, eight of which stand for a tile's
-// start and end (512 x 1024 x 8192 in MXFP4: 10.5 13.4 14.2; dX of 946 rows, 8 groups of 3704 x 424:
-// 21.1 20.1 27.6); a ratio of 1.4 allows for the exchange of partial sums.  Below, the four-way split is
+// start and end (512 x 1024 x 8192 in MXFP4: 10.7 13.8 14.0; dX of 946 rows, 8 groups of 3704 x 424:
+// 14.5 20.5 26.2); a ratio of 1.4 allows for the exchange of partial sums.  Below, the four-way split is
 // taken where each CTA still has several k-blocks of a tile, or where there is at most about one tile per
-// cluster (8 groups of 1024 x 1024, 2 rows: 4.9 5.7 6.4); many tiles of a short contraction have nothing
-// to split (dX of 373 rows, 52 groups of 112 x 1344: 23.1 14.7 8.1).
+// cluster (8 groups of 1024 x 1024, 2 rows: 4.9 5.7 6.2); many tiles of a short contraction have nothing
+// to split (dX of 373 rows, 52 groups of 112 x 1344: 25.0 14.4 8.1).
 int variant_of(int op, int64_t groups, int64_t T, int64_t lanes, int64_t depth, int sm_count) {
   const int forced = tuning_value(13);
   if (forced >= 0) return forced;
   const bool mx = op == kMxNt;
   const int64_t blocks = ceil_div(depth, mx ? 256 : 64), rows = T / groups;
-  const int64_t wide_from = mx ? (groups == 1 ? 96 : 8) : op == kGroupedDx ? 16 : 32;
+  const int64_t wide_from = mx ? (groups == 1 ? 96 : 8) : op == kGroupedDx ? 8 : 24;
   if (rows >= wide_from) {
     const int64_t tiles = ceil_div(lanes, 256) * groups * ceil_div(rows, 256);
     const int64_t split_tiles = ceil_div(lanes, 128) * groups * ceil_div(rows, 128);
@@ -407,9 +413,9 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   // 2608 x 1032 with 12 rows 37.5 40.8, 128 rows 56.2 54.1; 8 groups of 1024 x 2048 with 64 rows
   // 10.4 11.9; 4 groups of 256 x 512 with 2048 rows 11.4 18.4.
   // Few tiles of a long contraction share it in clusters of four, at the cost of 14 blocks of 64 rows a
-  // tile.  Single / four: one group of 128 x 128 with 1024 rows 5.8 6.6, 2048 rows 8.2 7.3; 4 groups of
-  // 256 x 512 with 1024 rows 7.8 8.1, 2048 rows 11.4 9.4; 8 of them with 2048 rows 12.4 13.9, 4096 rows
-  // 28.2 21.0.
+  // tile.  Single / four: one group of 128 x 128 with 1024 rows 6.4 7.1, 2048 rows 9.5 7.9; 4 groups of
+  // 256 x 512 with 1024 rows 6.8 8.3, 2048 rows 9.9 9.3; 8 of them with 2048 rows 10.2 13.6, 4096 rows
+  // 16.6 16.8; 2 of 840 x 408 with 4627 rows 32.1 23.8.
   const int forced = tuning_value(13);
   const int64_t pair_tiles = groups * ceil_div(N, 256) * ceil_div(K, 256);
   const int64_t single_tiles = groups * ceil_div(N, 128) * ceil_div(K, 128);
@@ -441,6 +447,7 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   if (tiles > kMaxExtent) return NEOGEMM_ERR_UNSUPPORTED;
   p.lane_tiles = static_cast<int>(lane_tiles);
   p.col_tiles = static_cast<int>(col_tiles);
+  p.part_bufs = kMaxPartBufs;
   p.vector_out = K % 8 == 0 && aligned16(dW);
   if (p.vector_out) {
     rc = encode_bf16(dev, &maps.result, dW, K, N, groups, K, N * K, 32);

@@ -39,6 +39,12 @@ enum GroupedOp : int { kGroupedNt = 0, kGroupedDx = 1, kGroupedDw = 2, kMxNt = 3
 
 constexpr int kMaxGroups = 1024;
 
+// A buffer of partial sums: 128 lanes x 16 columns in fp32 (from each CTA of the cluster its share of
+// the lanes).
+constexpr int kPartCols = 16;
+constexpr int kPartBytes = 128 * kPartCols * 4;
+constexpr int kMaxPartBufs = 8;
+
 struct GroupedParams {
   const void* offsets;      // groups + 1 ascending row indices, or null: one group of all rows
   int offsets_are_64;
@@ -52,6 +58,7 @@ struct GroupedParams {
   int col_box;              // rows of the ragged operand's large boxes (a CTA's share of col_cap)
   int small_box;            // and of its small ones
   int slots, per_slot;      // streaming kernels: ring slots, and the k-blocks that each takes
+  int part_bufs;            // buffers of partial sums (2, 4 or 8)
   int col_tiles;            // kGroupedDw: tiles along `cols`
   int zero_rest;            // write zeros to the rows of no group (0: leave them)
   int vector_out;           // 16-byte stores are possible (alignment of base and pitches); for dW the
@@ -116,17 +123,15 @@ struct GroupedConfig {
   // nothing spills (of 227 KB shared memory no cache is left: in the MXFP4 pair a spill of 100 words
   // cost 16 us of 77).
   static constexpr int kPull = kAccs == 1 ? 128 : 64;
-  // Per warp 32 x 32 bf16; streaming: two buffers for the partial sums of 128 lanes x 16 columns in
-  // fp32 (from kSplit CTAs 128 / kSplit lanes each).
-  static constexpr int kPartCols = 16;
-  static constexpr int kPartBytes = 128 * kPartCols * 4;
+  // Per warp 32 x 32 bf16; kSplit > 1: buffers of partial sums instead, part_bufs of them (streaming
+  // kernels: those beyond two at the expense of the ring).
   // dW: one or two boxes of 32 x 64 bf16 per warp.
   static constexpr int kBoxBufs = (kOp == kGroupedDw && kCtaGroup == 1) ? 2 : 1;
-  static constexpr int kEpiWarpBytes = (kOp == kGroupedDw || kStream) ? 4096 * kBoxBufs : 2048;
-  static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
-  static_assert(kSplit == 1 || kEpiBytes >= 2 * kPartBytes, "partial sums");
+  static constexpr int kEpiWarpBytes = kOp == kGroupedDw ? 4096 * kBoxBufs : 2048;
+  static constexpr int kEpiBytes = kStream ? 2 * kPartBytes : kSplit > 1 ? kMaxPartBufs * kPartBytes
+                                                                       : kEpiWarps * kEpiWarpBytes;
   static constexpr int kTableBytes = (3 * kMaxGroups + 1) * 4;
-  static constexpr int kBarrierBytes = (3 * kStages + 4 + 2 + 2 + 2 * kSplit) * 8 + 16;
+  static constexpr int kBarrierBytes = (3 * kStages + 4 + 3 * kMaxPartBufs) * 8 + 16;
   static constexpr int kRestBytes = kEpiBytes + kTableBytes + 12 + kBarrierBytes + 1024;
   static constexpr int kRingBytes = kStream ? (232448 - kRestBytes) / 1024 * 1024 : kStages * kStageBytes;
   static_assert(kEpiBytes % 1024 == 0, "the ring starts on the swizzle's alignment");
@@ -150,7 +155,9 @@ struct GroupedConfig {
   static_assert(kSmemBytes > 116224, "one CTA per SM: tensor memory is not shared");
   static_assert(kTmemNeeded <= 512, "tensor memory");
   static_assert(kCols % 32 == 0 && kCols <= 256 && kHalfCols % 32 == 0, "columns");
-  static_assert(kRingBytes >= 2 * kStageBytes, "two full blocks");
+  static_assert(kRingBytes - (kStream ? kMaxPartBufs - 2 : 0) * kPartBytes >= 2 * kStageBytes,
+                "two full blocks");
+  static_assert(kOp != kMxNt || kScaleSets >= kStages * (kStream ? 2 : 1), "scales of every k-block in the ring");
 };
 
 // What a tile computes.  Every role derives it from the tile's number.
@@ -428,17 +435,17 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const uint32_t epi_base = smem_base;
-  const uint32_t ring = epi_base + Cfg::kEpiBytes;
-  const uint32_t bar_base = ring + Cfg::kRingBytes;
+  const uint32_t ring = epi_base + (Cfg::kStream ? p.part_bufs * kPartBytes : Cfg::kEpiBytes);
+  const uint32_t bar_base = epi_base + Cfg::kEpiBytes + Cfg::kRingBytes;
   const uint32_t full_bar = bar_base;                        // [kStages]
   const uint32_t empty_bar = full_bar + 8 * kStages;         // [kStages]
   const uint32_t clear_bar = empty_bar + 8 * kStages;        // [kStages] dW: last block has landed
   const uint32_t tmem_full_bar = clear_bar + 8 * kStages;    // [2]
   const uint32_t tmem_empty_bar = tmem_full_bar + 16;        // [2]
-  const uint32_t part_full_bar = tmem_empty_bar + 16;        // [2] partial sums have arrived
-  const uint32_t part_read_bar = part_full_bar + 16;         // [2] and have been read by this CTA's warps
-  const uint32_t part_free_bar = part_read_bar + 16;         // [kSplit][2] CTA d's buffer is free
-  uint8_t* tail_gen = smem_gen + (part_free_bar + 16 * Cfg::kSplit - smem_base);
+  const uint32_t part_full_bar = tmem_empty_bar + 16;                // [kMaxPartBufs] have arrived
+  const uint32_t part_read_bar = part_full_bar + 8 * kMaxPartBufs;   // and been read by this CTA's warps
+  const uint32_t part_free_bar = part_read_bar + 8 * kMaxPartBufs;   // all CTAs' may be written again
+  uint8_t* tail_gen = smem_gen + (part_free_bar + 8 * kMaxPartBufs - smem_base);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail_gen);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_gen + 4);
   int* const words = reinterpret_cast<int*>(tail_gen + 16);
@@ -465,13 +472,15 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
     for (int a = 0; a < 2; ++a) {
       mbar_init(tmem_full_bar + 8 * a, 1);
       mbar_init(tmem_empty_bar + 8 * a, Cfg::kEpiWarps * kCtaGroup);
-      mbar_init(part_full_bar + 8 * a, 1);
-      mbar_init(part_read_bar + 8 * a, 4);
-      for (int d = 0; d < Cfg::kSplit; ++d) mbar_init(part_free_bar + 16 * d + 8 * a, 1);
     }
     fence_barrier_init();
-    if (Cfg::kSplit > 1)
-      for (int a = 0; a < 2; ++a) mbar_arrive_expect_tx(part_full_bar + 8 * a, Cfg::kPartBytes);
+  }
+  if (Cfg::kSplit > 1 && threadIdx.x >= 32 * Cfg::kFreeWarp && static_cast<int>(lane) < p.part_bufs) {
+    mbar_init(part_full_bar + 8 * lane, 1);
+    mbar_init(part_read_bar + 8 * lane, 4);
+    mbar_init(part_free_bar + 8 * lane, Cfg::kSplit);
+    fence_barrier_init();
+    mbar_arrive_expect_tx(part_full_bar + 8 * lane, kPartBytes);
   }
   if (warp == 0 && lane == 0 && p.depth > 0) {   // without a contraction there are no maps
     prefetch_tensormap(&maps.lanes);
@@ -873,12 +882,13 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
         // them, [source][four columns][lane][4]; then this warp adds up four columns of the lanes
         // that its own CTA collects.  The next columns are on their way meanwhile.
         constexpr int kSplit = Cfg::kSplit, kOwn = 128 / kSplit;   // lanes that a CTA collects
-        constexpr uint32_t kSource = kOwn * Cfg::kPartCols * 4;
+        constexpr uint32_t kSource = kOwn * kPartCols * 4;
         const uint32_t dest = quad * kSplit / 4;
         const uint32_t dest_lane = (quad * 32) % kOwn + lane;
         const uint32_t dest_base = mapa_u32(epi_base, dest) + split_rank * kSource + dest_lane * 16;
         const uint32_t dest_full = mapa_u32(part_full_bar, dest);
-        const int c_first = t.lo & ~(Cfg::kPartCols - 1);
+        const int part_mask = p.part_bufs - 1, part_shift = __popc(part_mask);
+        const int c_first = t.lo & ~(kPartCols - 1);
         bool ok = true;
         auto send = [&](int c, int n) {
           uint32_t r[16];
@@ -890,28 +900,28 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
 #pragma unroll
             for (int j = 0; j < 16; ++j) r[j] = 0u;
           }
-          const uint32_t b = n & 1;
-          ok = ok && __all_sync(0xffffffffu, wait_cluster(part_free_bar + 16 * dest + 8 * b,
-                                                          ((n >> 1) & 1) ^ 1, abort_flag));
+          const uint32_t b = n & part_mask;
+          ok = ok && __all_sync(0xffffffffu, wait_cluster(part_free_bar + 8 * b,
+                                                          ((n >> part_shift) & 1) ^ 1, abort_flag));
           if (!ok) return;
           // (Ordinary stores and a release at cluster scope took 1500 cycles: the release waits for
           // every store in flight, those of the result included.)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            st_async_v4(dest_base + b * Cfg::kPartBytes + j * (kOwn * 16), dest_full + 8 * b, r[4 * j],
+            st_async_v4(dest_base + b * kPartBytes + j * (kOwn * 16), dest_full + 8 * b, r[4 * j],
                         r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
         };
         auto collect = [&](int c, int n) {
-          const uint32_t b = n & 1;
-          ok = ok &&
-               __all_sync(0xffffffffu, wait_cluster(part_full_bar + 8 * b, (n >> 1) & 1, abort_flag));
+          const uint32_t b = n & part_mask;
+          ok = ok && __all_sync(0xffffffffu, wait_cluster(part_full_bar + 8 * b, (n >> part_shift) & 1,
+                                                          abort_flag));
           if (!ok) return;
           // Arm the buffer for its next use: nothing can arrive before this warp has read it, below.
-          if (quad == 0 && lane == 0) mbar_arrive_expect_tx(part_full_bar + 8 * b, Cfg::kPartBytes);
+          if (quad == 0 && lane == 0) mbar_arrive_expect_tx(part_full_bar + 8 * b, kPartBytes);
           float sum[kOwn / 32][4];
 #pragma unroll
           for (int h = 0; h < kOwn / 32; ++h) {
-            const uint32_t at = epi_base + b * Cfg::kPartBytes + (quad * kOwn + h * 32 + lane) * 16;
+            const uint32_t at = epi_base + b * kPartBytes + (quad * kOwn + h * 32 + lane) * 16;
 #pragma unroll
             for (int q = 0; q < kSplit; ++q) {
               uint32_t v[4];
@@ -948,9 +958,9 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
           }
         };
         send(c_first, parts);
-        for (int c = c_first; c < t.hi; c += Cfg::kPartCols) {
+        for (int c = c_first; c < t.hi; c += kPartCols) {
           const int n = parts++;
-          if (c + Cfg::kPartCols < t.hi) send(c + Cfg::kPartCols, n + 1);
+          if (c + kPartCols < t.hi) send(c + kPartCols, n + 1);
           else hand_back();   // all of the accumulator has been read
           collect(c, n);
         }
@@ -1050,23 +1060,35 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
   } else if (Cfg::kSplit > 1) {
     // ======================= buffers of partial sums: back to the senders =======================
     // The senders overwrite what this CTA's four warps have read, so the loads have to be ordered in front
-    // of their next stores by a release at cluster scope.  That waits for every store that its own warp
-    // has in flight, which in an epilogue warp are those of the result (28.0 -> 30.7 us for 16 x 28672 x
-    // 8192 in MXFP4, 26.8 -> 35.6 for 32 groups of 3584 x 2048 with two rows each); this warp has none.
-    int n = 0;   // column groups of partial sums so far
-    bool ok = true;
-    for (; ok && tiles.take(p, t); ++tile) {
-      for (int c = t.lo & ~(Cfg::kPartCols - 1); ok && c < t.hi; c += Cfg::kPartCols, ++n) {
-        const uint32_t b = n & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(part_read_bar + 8 * b, (n >> 1) & 1, abort_flag));
-        if (!ok) {
-          if (lane == 0) report_error(p.status, abort_flag, kDevTimeoutEpilogue, tile, 3);
-          break;
-        }
-        if (lane < Cfg::kSplit)
-          mbar_arrive_release_cluster(mapa_u32(part_free_bar + 16 * split_rank + 8 * b, lane));
-        __syncwarp();
+    // of their next stores by a release at cluster scope.  That takes 1200 to 4200 cycles while the SM
+    // streams, whichever warp does it (in the epilogue's own, 16 x 28672 x 8192 in MXFP4: 30.7 us with its
+    // quantisation, 27.7 here; 32 groups of 3584 x 2048 with two rows each: 35.6 and 27).  So a warp of its own
+    // does it, once for all that has been read meanwhile, and not at all for buffers that no later step
+    // fills.
+    const int bufs = p.part_bufs, mask = bufs - 1, shift = __popc(mask);
+    int known = 0;   // column groups of the tiles looked at: these are to come
+    bool ok = true, more = true;
+    for (int n = 0; ok;) {
+      while (more && known <= n + 2 * bufs) {
+        more = tiles.take(p, t);
+        if (more) known += (t.hi + kPartCols - 1) / kPartCols - t.lo / kPartCols;
       }
+      if (known <= n + bufs) break;
+      ok = __all_sync(0xffffffffu, mbar_wait(part_read_bar + 8 * (n & mask), (n >> shift) & 1, abort_flag));
+      if (!ok) {
+        if (lane == 0) report_error(p.status, abort_flag, kDevTimeoutEpilogue, n, 3);
+        break;
+      }
+      int end = n + 1;
+      while (end < n + bufs && known > end + bufs &&
+             __all_sync(0xffffffffu, mbar_test_wait(part_read_bar + 8 * (end & mask), (end >> shift) & 1)))
+        ++end;
+      if (lane < Cfg::kSplit) {
+        fence_cluster();
+        for (; n < end; ++n) mbar_arrive_relaxed_cluster(mapa_u32(part_free_bar + 8 * (n & mask), lane));
+      }
+      __syncwarp();
+      n = end;
     }
   }
   __syncwarp();

@@ -106,11 +106,18 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
-// The same with a release at cluster scope, for ordinary shared memory: stores that the other CTA's
-// tensor pipe is going to read (also fenced towards the async proxy by the caller), or loads of what the
-// other CTA is going to overwrite.  The other side waits with cluster scope.
+// The same with a release at cluster scope, for ordinary stores to shared memory that the other CTA's
+// tensor pipe is going to read (also fenced towards the async proxy by the caller).
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+               : "memory");
+}
+
+// A release at cluster scope in two parts, so that one fence serves several barriers.  The other side
+// waits with cluster scope.
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive_relaxed_cluster(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
                : "memory");
 }
 
