@@ -242,19 +242,19 @@ __device__ __forceinline__ bool group_range(const GroupedParams& p, int e, int* 
 
 // Ranges of 32 consecutive groups, one per lane, of offsets that were not in order: an index that descends
 // counts as the largest in front of it (`before`, for the first lane).  So no two groups share a row - two
-// tiles would store it - and there are no more tiles than in order.  Returns the largest index so far.
-__device__ __forceinline__ int in_order(int before, int* begin, int* end) {
+// tiles would store it - and there are no more tiles than in order.  (begin, end, largest index so far.)
+// A call, not inline: inlined, this path that hardly ever runs cost dW of 513 rows, 8 x 1024 x 2048, 11.0 us
+// instead of 10.3.
+__device__ __noinline__ int3 in_order(int before, int begin, int end) {
   const int lane = static_cast<int>(ptx::lane_id());
-  int top = max(*end, before);
+  int top = max(end, before);
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const int other = __shfl_up_sync(0xffffffffu, top, d);
     if (lane >= d) top = max(top, other);
   }
   const int previous = __shfl_up_sync(0xffffffffu, top, 1);
-  *begin = lane > 0 ? previous : max(*begin, before);
-  *end = top;
-  return __shfl_sync(0xffffffffu, top, 31);
+  return make_int3(lane > 0 ? previous : max(begin, before), top, __shfl_sync(0xffffffffu, top, 31));
 }
 
 // Records offsets that were clamped: the launch is not aborted.
@@ -295,7 +295,10 @@ struct GroupedTiles {
     if (p.groups <= 32) {
       const int lane = static_cast<int>(ptx::lane_id());
       good = group_range(p, min(lane, p.groups - 1), &my_begin, &my_end);
-      if (!__all_sync(0xffffffffu, good)) in_order(0, &my_begin, &my_end);
+      if (!__all_sync(0xffffffffu, good)) {
+        const int3 range = in_order(0, my_begin, my_end);
+        my_begin = range.x, my_end = range.y;
+      }
       const int mine = Cfg::kOp == kGroupedDw || lane >= p.groups
                            ? 0 : column_tiles<Cfg>(p, my_begin, my_end) * p.lane_tiles;
       int scan = mine;
@@ -519,9 +522,9 @@ grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) 
       for (int base = 0; base < p.groups; base += 32) {
         const int e = base + static_cast<int>(lane);
         if (bad) {
-          int begin = e < p.groups ? table.begin[e] : 0, end = e < p.groups ? table.end[e] : 0;
-          top = in_order(top, &begin, &end);
-          if (e < p.groups) table.begin[e] = begin, table.end[e] = end;
+          const int3 range = in_order(top, e < p.groups ? table.begin[e] : 0, e < p.groups ? table.end[e] : 0);
+          if (e < p.groups) table.begin[e] = range.x, table.end[e] = range.y;
+          top = range.z;
         }
         const int mine =
             !kDw && e < p.groups ? column_tiles<Cfg>(p, table.begin[e], table.end[e]) * p.lane_tiles : 0;
