@@ -114,6 +114,7 @@ int launch(const DeviceView& dev, const KernelEntry& k, int64_t tiles_at_most,
     std::lock_guard<std::mutex> lock(mu);
     int& known = resident[dev.index][k.op][variant];
     if (known == 0) {
+      RelaxedCapture relaxed;
       if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem_bytes) !=
           cudaSuccess) {
         cudaGetLastError();

@@ -9,6 +9,23 @@
 
 namespace neogemm {
 
+// While one lives, the calling thread may allocate memory and load kernels although a stream is being
+// captured: a process's first call may be made inside a capture.  Nothing that is done under it belongs
+// to the captured work.
+class RelaxedCapture {
+ public:
+  RelaxedCapture() { ok_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+  ~RelaxedCapture() {
+    if (ok_) cudaThreadExchangeStreamCaptureMode(&mode_);
+  }
+  RelaxedCapture(const RelaxedCapture&) = delete;
+  RelaxedCapture& operator=(const RelaxedCapture&) = delete;
+
+ private:
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+  bool ok_;
+};
+
 struct DeviceView {
   int index;          // CUDA device ordinal
   int sm_count;

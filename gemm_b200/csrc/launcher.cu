@@ -197,6 +197,7 @@ DeviceState* device_state(int* code) {
     return st.init_error == NEOGEMM_OK ? &st : nullptr;
   }
   st.ready = true;
+  RelaxedCapture relaxed;
   int major = 0;
   if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
       major != 10 ||
@@ -233,11 +234,16 @@ DeviceState* device_state(int* code) {
   }
   std::memset(st.status_host, 0, 64);
   // Arrival counters of the wave pacing; without them the kernels simply do not pace.
+  // (Cleared on a stream of their own: the default stream may not be used during a capture.)
+  cudaStream_t own = nullptr;
   if (cudaMalloc(reinterpret_cast<void**>(&st.pace_counters), kPaceSlots * 128) != cudaSuccess ||
-      cudaMemset(st.pace_counters, 0, kPaceSlots * 128) != cudaSuccess) {
+      cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) != cudaSuccess ||
+      cudaMemsetAsync(st.pace_counters, 0, kPaceSlots * 128, own) != cudaSuccess ||
+      cudaStreamSynchronize(own) != cudaSuccess) {
     cudaGetLastError();
     st.pace_counters = nullptr;
   }
+  if (own != nullptr) cudaStreamDestroy(own);
   *code = NEOGEMM_OK;
   return &st;
 }
