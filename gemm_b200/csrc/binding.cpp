@@ -10,7 +10,6 @@
 //   * failures raise RuntimeError (the reference prints to stderr, nemgemmV03.cu:387-390).
 #include <torch/extension.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -109,11 +108,56 @@ Rows rows_operand(const torch::Tensor& t, const char* name, const torch::Tensor&
   return Rows{t.size(0), t.size(1), t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 8 * 8};
 }
 
-// A result is written while the operands are read.  (Views whose overlap takes a search are let pass.)
+// The bytes of a tensor as `count` runs of `width` bytes, `pitch` apart; false if they are not such.
+struct Runs {
+  intptr_t begin, end;   // first byte, and the one behind the last
+  int64_t count, width, pitch;
+};
+
+bool runs_of(const torch::Tensor& t, Runs* r) {
+  c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;   // (stride in bytes, size)
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) != 0)
+      dims.emplace_back(t.stride(d) * static_cast<int64_t>(t.element_size()), t.size(d));
+  std::sort(dims.begin(), dims.end());
+  r->begin = r->end = reinterpret_cast<intptr_t>(t.data_ptr());
+  r->count = 1;
+  r->width = r->pitch = t.element_size();
+  r->end += r->width;
+  bool simple = true;
+  for (const auto& [stride, size] : dims) {
+    r->end += stride * (size - 1);
+    if (r->count == 1 && stride <= r->width) {
+      r->width = stride * (size - 1) + r->width;
+    } else if (r->count == 1) {
+      r->pitch = stride;
+      r->count = size;
+    } else if (stride == r->pitch * r->count) {
+      r->count *= size;
+    } else {
+      simple = false;
+    }
+  }
+  return simple;
+}
+
+// Whether two tensors have a byte in common: exactly, if the runs of both are equally far apart or one has
+// a single run; other views count as sharing when their address ranges do.
+bool share_memory(const torch::Tensor& a, const torch::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  Runs x, y;
+  const bool simple = runs_of(a, &x) & runs_of(b, &y);
+  if (x.end <= y.begin || y.end <= x.begin) return false;
+  if (!simple || (x.count > 1 && y.count > 1 && x.pitch != y.pitch)) return true;
+  if (x.count == 1 && y.count == 1) return true;
+  const int64_t pitch = x.count > 1 ? x.pitch : y.pitch;
+  const int64_t apart = ((y.begin - x.begin) % pitch + pitch) % pitch;   // y's run behind x's, in a period
+  return apart < x.width || apart + y.width > pitch;
+}
+
+// A result is written while the operands are read.
 void check_apart(const torch::Tensor& out, const torch::Tensor& operand, const char* name) {
-  const at::MemOverlapStatus s = at::get_overlap_status(out, operand);
-  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial,
-                    "out must not share memory with ", name);
+  TORCH_CHECK_VALUE(!share_memory(out, operand), "out must not share memory with ", name);
 }
 
 struct Result {
@@ -176,6 +220,7 @@ torch::Tensor grouped_rows(RowsFunction fn, const char* name, bool transposed, c
   if (out.has_value()) {
     check_apart(*out, rows, name);
     check_apart(*out, w, "w");
+    check_apart(*out, offsets, "offsets");
   }
   check_status(fn(rows.data_ptr(), w.data_ptr(), y.tensor.data_ptr(), offsets.data_ptr(),
                   offsets.scalar_type() == at::kLong, groups, r.count, N, K, r.pitch,
@@ -211,6 +256,7 @@ torch::Tensor grouped_matmul_dw(const torch::Tensor& dy, const torch::Tensor& x,
                       dy.device());
     check_apart(dw, dy, "dy");
     check_apart(dw, x, "x");
+    check_apart(dw, offsets, "offsets");
   } else {
     dw = empty_beside(dy, {groups, d.width, r.width}, at::kBFloat16);
   }
@@ -307,7 +353,7 @@ torch::Tensor grouped_matmul_mxfp4(const torch::Tensor& x, const torch::Tensor& 
   c10::cuda::CUDAGuard guard(x.device());
   Result y = rows_result(out, x, T, N);
   if (out.has_value())
-    for (const torch::Tensor* t : {&x, &x_scales, &w, &w_scales}) check_apart(*out, *t, "an operand");
+    for (const torch::Tensor* t : {&x, &x_scales, &w, &w_scales, &offsets}) check_apart(*out, *t, "an operand");
   check_status(neogemm_grouped_mxfp4_nt(x.data_ptr(), x_scales.data_ptr(), w.data_ptr(),
                                         w_scales.data_ptr(), y.tensor.data_ptr(), offsets.data_ptr(),
                                         offsets.scalar_type() == at::kLong, groups, T, N, K, y.pitch,
@@ -325,6 +371,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("B"), pybind11::arg("C"));
   m.def("matmul", &matmul, "returns row-major C[M,N] = A * B^T", pybind11::arg("A"),
         pybind11::arg("B"));
+  m.def("_share_memory", &share_memory, "whether two tensors have a byte in common (the check of out=)",
+        pybind11::arg("a"), pybind11::arg("b"));
   m.def("grouped_matmul", &grouped_matmul, "gemm_b200.ops.grouped_matmul", pybind11::arg("x"),
         pybind11::arg("w"), pybind11::arg("offsets"), pybind11::arg("out") = pybind11::none());
   m.def("grouped_matmul_dx", &grouped_matmul_dx, "gemm_b200.ops.grouped_matmul_dx", pybind11::arg("dy"),
