@@ -14,6 +14,8 @@ from __future__ import annotations
 import ctypes
 import importlib
 import sys
+from importlib.machinery import EXTENSION_SUFFIXES
+from importlib.util import module_from_spec, spec_from_file_location
 from pathlib import Path
 from typing import NamedTuple, Optional
 
@@ -188,23 +190,34 @@ def matmul_host(A_host: torch.Tensor, B_host: torch.Tensor, C_host: torch.Tensor
 # ----------------------------------------------------------------------------------------------
 # These calls serve single decoding steps, where the host's time per call counts: their checks and
 # launches live in the neoGEMM extension (over the same C ABI), which costs about half of ctypes.
-class _Extension:
-    """The neoGEMM extension, imported on first use (it needs torch's CUDA libraries and a build)."""
-
-    def __getattr__(self, name):
-        root = str(Path(__file__).resolve().parent.parent)
+def _load_extension():
+    """The neoGEMM extension built beside this package - by its path: another module of that name (the
+    reference's operator is called so too) may be installed, or loaded already."""
+    root = Path(__file__).resolve().parent.parent
+    own = next((p for p in (root / f"neoGEMM{s}" for s in EXTENSION_SUFFIXES) if p.exists()), None)
+    if own is None:   # installed elsewhere
         try:
             module = importlib.import_module("neoGEMM")
         except ImportError:
-            sys.path.append(root)   # built in-tree beside the package
-            try:
-                module = importlib.import_module("neoGEMM")
-            except ImportError as e:
-                raise ImportError("the neoGEMM extension is missing: build it with `python -m "
-                                  "gemm_b200.build` (there is no fallback implementation)") from e
-            finally:
-                sys.path.remove(root)
-        value = getattr(module, name)
+            module = None
+        if not hasattr(module, "grouped_matmul"):
+            raise ImportError("the neoGEMM extension is missing: build it with `python -m gemm_b200.build` "
+                              "(there is no fallback implementation)")
+        return module
+    loaded = sys.modules.get("neoGEMM")
+    if getattr(loaded, "__file__", None) and Path(loaded.__file__).resolve() == own.resolve():
+        return loaded
+    spec = spec_from_file_location("neoGEMM", own)
+    module = module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+class _Extension:
+    """The neoGEMM extension, loaded on first use (it needs torch's CUDA libraries and a build)."""
+
+    def __getattr__(self, name):
+        value = getattr(_load_extension(), name)
         setattr(self, name, value)
         return value
 
