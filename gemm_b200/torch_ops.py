@@ -10,6 +10,8 @@ current stream.  There is no CPU implementation: calling it with CPU tensors rai
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import ops as _ops
@@ -105,20 +107,22 @@ MAX_GROUPS = 1024
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """A matrix in a layout that the kernels read: contiguous rows that start on 16 bytes."""
+    step = 16 // t.element_size()
     if (t.shape[1] <= 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0 and (
-            t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
+            t.shape[0] <= 1 or (t.stride(0) % step == 0 and t.stride(0) >= t.shape[1])):
         return t
     rows, width = t.shape
-    return t.new_empty((rows, (width + 7) // 8 * 8))[:, :width].copy_(t)
+    return t.new_empty((rows, (width + step - 1) // step * step))[:, :width].copy_(t)
 
 
 @torch.library.custom_op(f"{_LIB_NAME}::grouped_linear", mutates_args=())
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """y[t] = x[t] @ weight[e]^T for the rows of group e (``ops.grouped_matmul``); differentiable in
-    ``x`` and ``weight``.  Rows of no group are zero, and so are their gradients.  ``weight``
-    is read in place, so its rows start on multiples of 8 values."""
+    ``x`` and ``weight``.  Rows of no group are zero, and so are their gradients.  ``x`` may have any
+    layout (it is copied if its rows are not contiguous or do not start on 16 bytes); ``weight`` is read in
+    place, so its rows start on multiples of 8 values."""
     _check_grouped(x, weight, offsets)
-    return _ops.grouped_matmul(x, weight, offsets)
+    return _ops.grouped_matmul(_readable(x), weight, offsets)
 
 
 @grouped_linear.register_fake
@@ -139,7 +143,7 @@ def _(dy, weight, offsets):
 
 @torch.library.custom_op(f"{_LIB_NAME}::grouped_linear_dw", mutates_args=())
 def _grouped_linear_dw(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-    return _ops.grouped_matmul_dw(_readable(dy), x, offsets)
+    return _ops.grouped_matmul_dw(_readable(dy), _readable(x), offsets)
 
 
 @_grouped_linear_dw.register_fake
@@ -213,12 +217,10 @@ def _check_mxfp4_grouped(x, codes, scales, offsets) -> None:
 
 @torch.library.custom_op(f"{_LIB_NAME}::mxfp4_linear", mutates_args=())
 def mxfp4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
-    """y = x @ W^T with x[..., K] quantised to MXFP4 on the way and W[N, K] held in it; bf16
+    """y = x @ W^T with x[..., K] (any layout) quantised to MXFP4 on the way and W[N, K] held in it; bf16
     result.  K is a multiple of 64."""
     _check_mxfp4_linear(x, codes, scales, 2)
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.size(1) > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
+    x2 = _readable(x.reshape(math.prod(x.shape[:-1]), x.shape[-1]))
     y = _ops.matmul_mxfp4(_ops.quantize_mxfp4(x2), _ops.MxFp4(codes, scales))
     return y.reshape(*x.shape[:-1], codes.shape[0])
 
@@ -234,7 +236,7 @@ def mxfp4_grouped_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Ten
                          offsets: torch.Tensor) -> torch.Tensor:
     """``grouped_linear`` with x quantised to MXFP4 on the way and the weights held in it."""
     _check_mxfp4_grouped(x, codes, scales, offsets)
-    return _ops.grouped_matmul_mxfp4(_ops.quantize_mxfp4(x), _ops.MxFp4(codes, scales), offsets)
+    return _ops.grouped_matmul_mxfp4(_ops.quantize_mxfp4(_readable(x)), _ops.MxFp4(codes, scales), offsets)
 
 
 @mxfp4_grouped_linear.register_fake
@@ -253,7 +255,8 @@ class NeoLinearMxFp4(torch.nn.Module):
         if weight.dim() not in (2, 3) or weight.shape[-1] % 64 != 0:
             raise ValueError(f"expected a weight [N, K] or [groups, N, K] with K a multiple of 64, got shape "
                              f"{tuple(weight.shape)}")
-        q = _ops.quantize_mxfp4(weight.detach())
+        weight = weight.detach().contiguous()
+        q = _ops.quantize_mxfp4(weight if weight.data_ptr() % 16 == 0 else weight.clone())
         self.register_buffer("codes", q.codes)
         self.register_buffer("scales", q.scales)
 
