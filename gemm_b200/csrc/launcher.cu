@@ -1270,10 +1270,14 @@ const char* neogemm_status_str(int status) {
   switch (status) {
     case NEOGEMM_OK: return "ok";
     case NEOGEMM_ERR_BAD_ARG: return "bad argument (null pointer, negative size or short leading dimension)";
-    case NEOGEMM_ERR_UNSUPPORTED: return "unsupported (K, lda, ldb must be multiples of 8; A, B 16-byte aligned; device must be sm_100)";
+    case NEOGEMM_ERR_UNSUPPORTED: 
+      return "unsupported (K, lda, ldb must be multiples of 8; A, B 16-byte aligned; device must be sm_100; "
+             "grouped: at most 1024 groups; MXFP4: K a multiple of 32, in products of 64)";
     case NEOGEMM_ERR_DESCRIPTOR: return "tensor-map encode failed or CUDA driver entry point unavailable";
     case NEOGEMM_ERR_LAUNCH: return "kernel launch failed";
-    case NEOGEMM_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait expired in an earlier launch (see neogemm_device_status)";
+    case NEOGEMM_ERR_DEVICE_TIMEOUT:
+      return "an earlier launch on this device recorded an error - a bounded wait that expired, or group "
+             "offsets out of order or range (see neogemm_device_status) - and calls fail until it is cleared";
     case NEOGEMM_ERR_WORKSPACE: return "workspace too small, misaligned or could not be allocated";
     case NEOGEMM_ERR_CUDA: return "CUDA runtime error";
     default: return "unknown status";

@@ -31,11 +31,13 @@ extern "C" {
 enum neogemm_status {
   NEOGEMM_OK = 0,
   NEOGEMM_ERR_BAD_ARG = 1,        /* null pointer, negative size, bad leading dimension */
-  NEOGEMM_ERR_UNSUPPORTED = 2,    /* K % 8 != 0, lda/ldb % 8 != 0, misaligned A/B, or not sm_100 */
+  NEOGEMM_ERR_UNSUPPORTED = 2,    /* K % 8 != 0, lda/ldb % 8 != 0, misaligned A/B, or not sm_100;
+                                     grouped and MXFP4 calls: see there */
   NEOGEMM_ERR_DESCRIPTOR = 3,     /* cuTensorMapEncodeTiled failed or is unavailable */
   NEOGEMM_ERR_LAUNCH = 4,         /* cudaLaunchKernelEx / attribute set-up failed */
-  NEOGEMM_ERR_DEVICE_TIMEOUT = 5, /* an earlier launch on this device reported a bounded wait that
-                                     expired; see neogemm_device_status() */
+  NEOGEMM_ERR_DEVICE_TIMEOUT = 5, /* an earlier launch on this device recorded an error: a bounded wait
+                                     that expired, or group offsets that were clamped; see
+                                     neogemm_device_status() */
   NEOGEMM_ERR_WORKSPACE = 6,      /* caller's workspace too small, or internal allocation failed */
   NEOGEMM_ERR_CUDA = 7            /* any other CUDA runtime error (copy, allocation, sync) */
 };
