@@ -160,6 +160,11 @@ void check_apart(const torch::Tensor& out, const torch::Tensor& operand, const c
   TORCH_CHECK_VALUE(!share_memory(out, operand), "out must not share memory with ", name);
 }
 
+// A caller's tensor has other values now: a graph that saved the earlier ones must not use them.
+void note_written(const c10::optional<torch::Tensor>& out) {
+  if (out.has_value() && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
+
 struct Result {
   torch::Tensor tensor;
   int64_t pitch;
@@ -226,6 +231,7 @@ torch::Tensor grouped_rows(RowsFunction fn, const char* name, bool transposed, c
                   offsets.scalar_type() == at::kLong, groups, r.count, N, K, r.pitch,
                   N > 1 ? w.stride(1) : (K + 15) / 8 * 8, groups > 1 ? w.stride(0) : 0, y.pitch,
                   y.zero_rest, stream_of(rows)));
+  note_written(out);
   return y.tensor;
 }
 
@@ -263,6 +269,7 @@ torch::Tensor grouped_matmul_dw(const torch::Tensor& dy, const torch::Tensor& x,
   check_status(neogemm_grouped_dw(dy.data_ptr(), x.data_ptr(), dw.data_ptr(), offsets.data_ptr(),
                                   offsets.scalar_type() == at::kLong, groups, d.count, d.width, r.width,
                                   d.pitch, r.pitch, stream_of(dy)));
+  note_written(out);
   return dw;
 }
 
@@ -337,6 +344,7 @@ torch::Tensor matmul_mxfp4(const torch::Tensor& a, const torch::Tensor& a_scales
     for (const torch::Tensor* t : {&a, &a_scales, &b, &b_scales}) check_apart(*out, *t, "an operand");
   check_status(neogemm_mxfp4_nt(a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(),
                                 c.tensor.data_ptr(), M, N, K, c.pitch, stream_of(a)));
+  note_written(out);
   return c.tensor;
 }
 
@@ -358,6 +366,7 @@ torch::Tensor grouped_matmul_mxfp4(const torch::Tensor& x, const torch::Tensor& 
                                         w_scales.data_ptr(), y.tensor.data_ptr(), offsets.data_ptr(),
                                         offsets.scalar_type() == at::kLong, groups, T, N, K, y.pitch,
                                         y.zero_rest, stream_of(x)));
+  note_written(out);
   return y.tensor;
 }
 

@@ -233,7 +233,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
     ``linear``'s weight), ``offsets`` groups + 1 ascending row indices (int32 or int64) on the same
     device; they are read on the GPU only.  Rows and matrices may be strided (contiguous along K,
     pitches multiples of 8).  Groups may be empty; at most 1024 of them.  Without ``out`` the rows
-    of no group are zero; with ``out`` (bf16 [T, N], contiguous rows) they are left as they are."""
+    of no group are zero; with ``out`` (bf16 [T, N], contiguous rows) they are left as they are.
+    Like every call here it records nothing for autograd: ``torch_ops.grouped_linear`` does."""
     return _ext.grouped_matmul(x, w, offsets, out)
 
 
