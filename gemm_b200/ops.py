@@ -279,7 +279,8 @@ def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
 
 
 def dequantize_mxfp4(q: MxFp4) -> torch.Tensor:
-    """The values of an MXFP4 matrix (or stack) as bf16, which holds them exactly."""
+    """The values of an MXFP4 matrix (or stack) as bf16, which holds them exactly (scale bytes 253 and 254,
+    which :func:`quantize_mxfp4` does not produce, reach past its range: Inf)."""
     return _ext.dequantize_mxfp4(*_mxfp4("q", q))
 
 

@@ -212,7 +212,9 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
  *   holds an Inf or a NaN gets the scale 255 and codes 0.  Padding bytes of `scales` are written
  *   as 0.  X: bf16 (x_is_f32 = 0) or fp32, 16-byte aligned, element (i,r,k) at
  *   x[i*stack_x + r*ldx + k], ldx and stack_x multiples of 16 bytes.  K % 32 == 0.
- * neogemm_mxfp4_dequantize: the values as packed bf16 [stack, rows, K] (exact).  K % 32 == 0.
+ * neogemm_mxfp4_dequantize: the values as packed bf16 [stack, rows, K].  K % 32 == 0.  Exact for scales
+ *   up to 252, the largest that neogemm_mxfp4_quantize writes; with 253 and 254, from elsewhere, magnitudes
+ *   of 2^128 and more become Inf.  Scale 255: NaN.
  * neogemm_mxfp4_nt: C[m,n] = sum_k A[m,k] B[n,k], fp32 accumulation, bf16 result with row pitch
  *   ldc.  K % 64 == 0.  Padding bytes of the scales have no influence.
  * neogemm_grouped_mxfp4_nt: neogemm_grouped_nt with both operands in MXFP4. */
