@@ -245,7 +245,7 @@ int variant_of(int op, int64_t groups, int64_t T, int64_t lanes, int64_t depth, 
     return four < two ? kNarrow : kMiddle;
   }
   const int64_t tiles = ceil_div(lanes, 128) * std::min(groups, T);
-  if (tiles > 148 && blocks < 8) return kWide;
+  if (tiles > sm_count && blocks < 8) return kWide;
   return blocks >= (mx ? 16 : 24) || tiles <= 40 ? kNarrow : kMiddle;
 }
 
@@ -422,7 +422,7 @@ int neogemm_grouped_dw(const void* dY, const void* X, void* dW, const void* offs
   const int64_t single_tiles = groups * ceil_div(N, 128) * ceil_div(K, 128);
   const int64_t blocks = ceil_div(T, 64 * groups), fours = std::max(dev.sm_count * 2 / 9, 1);
   int variant = kNarrow;
-  if (pair_tiles >= 148 && T / groups >= 128) variant = kWide;
+  if (pair_tiles >= dev.sm_count && T / groups >= 128) variant = kWide;
   else if (single_tiles <= dev.sm_count && ceil_div(single_tiles, fours) * (blocks + 56) < 4 * blocks)
     variant = kMiddle;
   if (forced >= 0) variant = forced;

@@ -19,13 +19,17 @@
 // remnant.  dW has no ragged output; there the group's rows are the contraction.
 //
 //   warp 0      TMA producer      warp 1      UMMA issuer (leader CTA of a pair)
-//   warps 2-5   (2-9) epilogue: tcgen05.ld -> bf16 -> shared-memory transpose -> 16-byte row stores,
-//               overlapped with the next tile through a second accumulator
-//   warp 6      kGroupedDw only: clears the rows of a tile's last k-block that belong to the next
+//   next 4 (8)  epilogue: tcgen05.ld -> bf16 -> shared memory (rows of the batch transposed on the way, by
+//               stmatrix) -> 16-byte stores, dW by TMA; overlapped with the next tile through a second
+//               accumulator, which the MXFP4 pair has no room for.  Where CTAs share a tile's
+//               contraction: partial sums to the CTA that adds them up, straight from the accumulator
+//   next one    kGroupedDw only: clears the rows of a tile's last k-block that belong to the next
 //               group (both operands: a zero times a neighbour's Inf would still be NaN)
+//   last one    CTAs that share a contraction only: frees the buffers of partial sums
 //
-// Every CTA (pair) walks tiles worker, worker + workers, ... of the list
-// (group, lane tile, column tile); the list's prefix sums are built in shared memory at the start.
+// Every CTA (pair, cluster) walks tiles worker, worker + workers, ... of the list (group, lane tile,
+// column tile).  Its prefix sums are in registers of each warp (up to 32 groups) or, built at the start,
+// in shared memory.
 // Every wait is bounded; on expiry the role records a code, raises the CTA's abort flag and falls
 // through to the tear-down.
 #pragma once

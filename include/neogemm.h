@@ -183,8 +183,8 @@ int neogemm_noalloc_clear_status(void);
  * zero_rest != 0 writes zeros to the rows of Y or dX that belong to no group (in front of offsets[0],
  * behind offsets[groups]); 0 leaves them as they are.  Sums are added in a fixed order, without
  * atomics: a call's result is the same bits each time.  (The order of a row's sum follows from the
- * kernel, which is chosen from T / groups: a row alone and in a large batch may differ in the last
- * bit.)  No workspace; no counterpart in the reference. */
+ * kernel, which is chosen from T, groups, N, K and the number of SMs, never from the offsets: a row alone
+ * and in a large batch may differ in the last bit.)  No workspace; no counterpart in the reference. */
 int neogemm_grouped_nt(const void* X, const void* W, void* Y, const void* offsets,
                        int offsets_are_64, int64_t groups, int64_t T, int64_t N, int64_t K,
                        int64_t ldx, int64_t ldw, int64_t stack_w, int64_t ldy, int zero_rest,
