@@ -10,7 +10,6 @@ import torch
 from gemm_b200 import ops
 
 pytestmark = pytest.mark.gpu
-E, ROWS = 8, 117
 
 
 @pytest.fixture(params=[0, 2], ids=["narrow", "middle"])
@@ -25,9 +24,11 @@ def whole(*shape, seed):
     return torch.randint(-4, 5, shape, generator=g, device="cuda").bfloat16()
 
 
+@pytest.mark.parametrize("E,ROWS,wide", [(8, 117, 4104), (12, 30, 4104), (30, 5, 2056), (1, 13, 20008)])
 @pytest.mark.parametrize("op", ["nt", "dx", "dw", "mx"])
-def test_every_buffer_arrives_whole_and_is_read_before_it_is_filled_again(op, tiles):
-    N, K = (4104, 1096) if op != "mx" else (4104, 1088)
+def test_every_buffer_arrives_whole_and_is_read_before_it_is_filled_again(op, E, ROWS, wide, tiles):
+    """Eight, four and two buffers; tiles of many and of one column group."""
+    N, K = (1096, wide) if op == "dx" else (wide, 1096 if op != "mx" else 1088)
     T = E * ROWS
     off = torch.arange(0, T + 1, ROWS, dtype=torch.int32, device="cuda")
     x, w, dy = whole(T, K, seed=1), whole(E, N, K, seed=2), whole(T, N, seed=3)
